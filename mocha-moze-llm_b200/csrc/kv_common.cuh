@@ -1,0 +1,458 @@
+// What the paged key/value operators (mocha_kv.h) share: the arguments as the kernels see
+// them, the ranges of visible keys, the split of the attention's work over CTAs with the
+// join of its parts, and the host-side checks.
+//
+// The split.  An attention call is a list of units (a sequence's block of query rows with
+// the heads of one kv head) and a unit is a list of key tiles.  The tiles of all units, in
+// order, are dealt to the CTAs in equal contiguous shares, so that ragged lengths, causal
+// blocks and one long sequence load every SM alike.  Lengths are on the device, so each
+// CTA finds its share itself.  A unit inside one share is finished there; one that is cut
+// leaves an unnormalised part (maximum, sum, output) per share, and the join kernel adds
+// the parts in the order of the shares: the result does not depend on timing.  A CTA
+// leaves at most two parts, one of a unit that it continues and one of a unit that it
+// begins, so the workspace does not grow with the batch.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <limits.h>
+#include <math.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include "mb_async.cuh"
+#include "mb_common.cuh"
+#include "mocha_kv.h"
+
+namespace kv {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMaxGroup = 64;  // query heads per kv head
+
+// n / d for n < 2^31, by a multiplication (round-up method of Granlund and Montgomery).
+struct FastDiv {
+    uint32_t d, mul, s1, s2;
+};
+
+inline FastDiv fast_div(uint32_t d)
+{
+    int l = 0;
+    while ((1ull << l) < d) l++;
+    return FastDiv{d, (uint32_t)((((1ull << l) - d) << 32) / d + 1), (uint32_t)(l < 1 ? l : 1), (uint32_t)(l > 1 ? l - 1 : 0)};
+}
+
+MB_DEV uint32_t div(FastDiv f, uint32_t n)
+{
+    const uint32_t t = __umulhi(f.mul, n);
+    return (t + ((n - t) >> f.s1)) >> f.s2;
+}
+
+// A unit that is cut, left for the join by the CTA in which it begins: parts lie in that
+// CTA's slot 1 and in slot 0 of the CTAs up to c_end.  Row r of the unit is token
+// row0 + r / ng, head head0 + r % ng.
+struct Meta {
+    int c_end;  // -1: no unit is cut here
+    int row0, ntok, head0, ng;
+    int seq, pos0;  // sequence, and position of token row0
+    int pad;
+};
+
+struct Args {
+    const char *k, *v;
+    long long ps, hs, ts;  // elements
+    int pages, kv_heads, d;
+    FastDiv page;
+    const int *table;
+    long long table_stride;
+    int max_len;  // positions that a table row can hold
+    const int *kv_len;
+    int *status;
+    int seqs;
+    int heads, group, window;
+    FastDiv group_div;
+    float scale, cap;
+    const int *prefix;
+    const float *slopes;
+    const char *q;
+    char *out;
+    long long q_row, q_head, o_row, o_head;  // elements
+    float *lse;
+    const int *q_start;  // prefill
+    int rows;
+    Meta *meta;   // [CTAs]
+    float *part;  // [CTAs][2][part rows][2 + padded dim]: outputs of all rows, then (m, l) of all rows
+};
+
+MB_DEV int seq_len(const Args &a, int s) { return min(max(__ldg(a.kv_len + s), 0), a.max_len); }
+MB_DEV int seq_prefix(const Args &a, int s, int len) { return a.prefix ? min(max(__ldg(a.prefix + s), 0), len) : 0; }
+
+// Tiles of T keys that queries at positions [pa, pb] of a sequence see: those of the
+// prefix, [0, pre_t), and those from lo_t on.  At least one tile, so that rows that see
+// nothing are written too.
+template <int T>
+struct Tiles {
+    int pre_t, lo_t, n;
+    MB_DEV void set(const Args &a, int len, int pre, int pa, int pb)
+    {
+        const int hi = min(pb + 1, len), lo = a.window ? max(pa - a.window + 1, 0) : 0;
+        pre_t = (pre + T - 1) / T;
+        lo_t = max(lo / T, pre_t);
+        n = max(pre_t + max((max(hi, 0) + T - 1) / T - lo_t, 0), 1);
+    }
+    MB_DEV int key(int i) const { return (i < pre_t ? i : i - pre_t + lo_t) * T; }
+};
+
+MB_DEV bool visible(int j, int p, int len, int pre, int window)
+{
+    return j < len && ((j <= p && (window == 0 || p - j < window)) || j < pre);
+}
+
+// Page of position j, or -1 for an id outside the pool.
+MB_DEV int page_of(const Args &a, int seq, int j)
+{
+    const int id = __ldg(a.table + (long long)seq * a.table_stride + div(a.page, (uint32_t)j));
+    if ((unsigned)id < (unsigned)a.pages) return id;
+    if (a.status) *a.status = 1;
+    return -1;
+}
+
+// Score in units of log2 from the plain product.
+MB_DEV float score2(const Args &a, float dot, float slope, int p, int j)
+{
+    float z = dot * a.scale;
+    if (a.cap > 0.f) z = a.cap * tanhf(z / a.cap);
+    if (a.slopes) z -= slope * (float)abs(p - j);
+    return z * kLog2e;
+}
+
+template <typename T>
+MB_DEV float to_f32(T x)
+{
+    return (float)x;
+}
+template <typename T>
+MB_DEV T from_f32(float x)
+{
+    return (T)x;
+}
+
+MB_DEV void store4(float *p, float4 x) { *reinterpret_cast<float4 *>(p) = x; }
+MB_DEV void store4(__half *p, float4 x)
+{
+    __half2 h[2] = {__floats2half2_rn(x.x, x.y), __floats2half2_rn(x.z, x.w)};
+    *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<uint2 *>(h);
+}
+MB_DEV void store4(__nv_bfloat16 *p, float4 x)
+{
+    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w)};
+    *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<uint2 *>(h);
+}
+
+// One row of a prompt's attention by a warp, reading only the keys that the row sees: for
+// the rows to which a tile's matrix product carried an infinite or NaN value of a key that
+// they do not see (0 * inf).  Rare, so written for size.
+template <typename T>
+__device__ __noinline__ void lone_row(const Args &a, int seq, int p, int head, int row)
+{
+    const int lane = threadIdx.x & 31, d = a.d, per = d / 32;
+    const int len = seq_len(a, seq), pre = seq_prefix(a, seq, len);
+    const int kvh = div(a.group_div, head);
+    const T *q = reinterpret_cast<const T *>(a.q) + row * a.q_row + head * a.q_head;
+    const float slope = a.slopes ? a.slopes[head] : 0.f;
+    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    const int hi = min(p + 1, len), lo = max(a.window ? max(p - a.window + 1, 0) : 0, pre);
+    for (int part = 0; part < 2; part++) {
+        const int j0 = part ? lo : 0, j1 = part ? hi : pre;
+        for (int jb = j0; jb < j1; jb += 32) {
+            const int j = jb + lane;
+            float z = -INFINITY;
+            long long at = -1;
+            if (j < j1) {
+                const int id = page_of(a, seq, j);
+                float dot = 0.f;
+                if (id >= 0) {
+                    at = id * a.ps + kvh * a.hs + (long long)(j - div(a.page, j) * a.page.d) * a.ts;
+                    const T *kr = reinterpret_cast<const T *>(a.k) + at;
+                    for (int i = 0; i < d; i++) dot = fmaf(to_f32(q[i]), to_f32(kr[i]), dot);
+                }
+                z = score2(a, dot, slope, p, j);
+            }
+            const float mn = fmaxf(m, mb::warp_max(z)), ms = mn == -INFINITY ? 0.f : mn;
+            const float f = exp2f(m - ms), e = j < j1 ? exp2f(z - ms) : 0.f;
+            m = mn;
+            l = l * f + mb::warp_sum(e);
+            for (int i = 0; i < per; i++) acc[i] *= f;
+            for (int t = 0; t < min(32, j1 - jb); t++) {
+                const float w = __shfl_sync(0xffffffffu, e, t);
+                const long long vt = __shfl_sync(0xffffffffu, at, t);
+                if (vt >= 0)
+                    for (int i = 0; i < per; i++)
+                        acc[i] = fmaf(w, to_f32(reinterpret_cast<const T *>(a.v)[vt + lane + 32 * i]), acc[i]);
+            }
+        }
+    }
+    T *o = reinterpret_cast<T *>(a.out) + row * a.o_row + head * a.o_head;
+    for (int i = 0; i < per; i++) o[lane + 32 * i] = from_f32<T>(l == 0.f ? 0.f : acc[i] / l);
+    if (a.lse && lane == 0) a.lse[(long long)row * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// ---- join of the parts of cut units --------------------------------------------------
+// Block (c, y): rows y, y + gridDim.y, ... of the unit that begins and is cut in CTA c; the
+// block's warps take parts in turn, lanes the dims.
+constexpr int kJoinWarps = 8;
+
+template <typename T, bool PREFILL>
+__global__ void __launch_bounds__(32 * kJoinWarps) k_join(const __grid_constant__ Args a, int part_rows, int dp)
+{
+    __shared__ float4 s_acc[kJoinWarps][32];
+    __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
+    mb::as::griddep_wait();
+    const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Meta mt = a.meta[c];
+    if (mt.c_end < 0) return;
+    const size_t slot = (size_t)part_rows * (dp + 2);
+    for (int r = blockIdx.y; r < mt.ntok * mt.ng; r += gridDim.y) {
+        float m = -INFINITY, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int U = 4;  // parts in flight per warp
+        for (int b = c + warp * U; b <= mt.c_end; b += kJoinWarps * U) {
+            float pm[U], pl[U];
+            float4 pv[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                pm[u] = -INFINITY;
+                pl[u] = 0.f;
+                pv[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (b + u <= mt.c_end) {
+                    const float *pp = a.part + ((size_t)(b + u) * 2 + (b + u == c ? 1 : 0)) * slot;
+                    pm[u] = __ldcg(pp + (size_t)part_rows * dp + 2 * r);
+                    pl[u] = __ldcg(pp + (size_t)part_rows * dp + 2 * r + 1);
+                    if (lane * 4 < a.d) pv[u] = __ldcg(reinterpret_cast<const float4 *>(pp + (size_t)r * dp) + lane);
+                }
+            }
+            float mn = m;
+#pragma unroll
+            for (int u = 0; u < U; u++) mn = fmaxf(mn, pm[u]);
+            const float ms = mn == -INFINITY ? 0.f : mn;
+            float f = exp2f(m - ms);
+            l *= f;
+            acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                f = exp2f(pm[u] - ms);
+                l = fmaf(pl[u], f, l);
+                acc.x = fmaf(pv[u].x, f, acc.x);
+                acc.y = fmaf(pv[u].y, f, acc.y);
+                acc.z = fmaf(pv[u].z, f, acc.z);
+                acc.w = fmaf(pv[u].w, f, acc.w);
+            }
+            m = mn;
+        }
+        s_acc[warp][lane] = acc;
+        if (lane == 0) {
+            s_m[warp] = m;
+            s_l[warp] = l;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            float M = s_m[0];
+#pragma unroll
+            for (int w = 1; w < kJoinWarps; w++) M = fmaxf(M, s_m[w]);
+            const float ms = M == -INFINITY ? 0.f : M;
+            l = 0.f;
+            acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kJoinWarps; w++) {
+                const float f = exp2f(s_m[w] - ms);
+                const float4 x = s_acc[w][lane];
+                l = fmaf(s_l[w], f, l);
+                acc.x = fmaf(x.x, f, acc.x);
+                acc.y = fmaf(x.y, f, acc.y);
+                acc.z = fmaf(x.z, f, acc.z);
+                acc.w = fmaf(x.w, f, acc.w);
+            }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const int t = r / mt.ng, head = mt.head0 + r - t * mt.ng;
+            const long long row = mt.row0 + t;
+            acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            bool alone = false;
+            if (PREFILL) {
+                const bool bad = !(isfinite(acc.x) && isfinite(acc.y) && isfinite(acc.z) && isfinite(acc.w));
+                alone = __any_sync(0xffffffffu, bad && lane * 4 < a.d);
+            }
+            if (alone) {
+                lone_row<T>(a, mt.seq, mt.pos0 + t, head, (int)row);
+            } else {
+                if (lane * 4 < a.d) store4(reinterpret_cast<T *>(a.out) + row * a.o_row + head * a.o_head + lane * 4, acc);
+                if (a.lse && lane == 0) a.lse[row * a.heads + head] = l == 0.f ? -INFINITY : (ms + log2f(l)) * kLn2;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------
+
+inline int fail(const char *who, const char *what)
+{
+    fprintf(stderr, "%s: %s\n", who, what);
+    return 1;
+}
+
+// Makes `device` current for a call and puts the caller's back.
+class DeviceGuard {
+  public:
+    int enter(const char *who, int device)
+    {
+        int count = 0, major = 0;
+        if (cudaGetDevice(&old_) != cudaSuccess || cudaGetDeviceCount(&count) != cudaSuccess)
+            return (void)cudaGetLastError(), fail(who, "no CUDA device");
+        if (device < 0 || device >= count) return fail(who, "device out of range");
+        if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) != cudaSuccess || major != 10)
+            return fail(who, "requires a compute capability 10.x (B200) device");
+        if (device != old_) {
+            if (cudaSetDevice(device) != cudaSuccess) return (void)cudaGetLastError(), fail(who, "cudaSetDevice failed");
+            changed_ = true;
+        }
+        return 0;
+    }
+    ~DeviceGuard()
+    {
+        if (changed_) cudaSetDevice(old_);
+    }
+
+  private:
+    int old_ = 0;
+    bool changed_ = false;
+};
+
+inline int type_bytes(int type) { return type == MOCHA_KV_F32 ? 4 : type == MOCHA_KV_F16 || type == MOCHA_KV_BF16 ? 2 : 0; }
+
+inline bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+inline int check_pages(const char *who, const mocha_kv_pages *p)
+{
+    if (!p) return fail(who, "null pages");
+    const int b = type_bytes(p->type);
+    if (!b) return fail(who, "type must be MOCHA_KV_F32, MOCHA_KV_F16 or MOCHA_KV_BF16");
+    if (p->pages < 1 || p->kv_heads < 1) return fail(who, "pages and kv_heads must be positive");
+    if (p->page_size < 8 || p->page_size % 8 || p->page_size > 65536)
+        return fail(who, "page_size must be a multiple of 8 up to 65536");
+    if (p->head_dim < 32 || p->head_dim % 32 || p->head_dim > 128)
+        return fail(who, "head_dim must be 32, 64, 96 or 128");
+    if (p->page_stride < 0 || p->head_stride < 0 || p->token_stride < p->head_dim)
+        return fail(who, "strides must not be negative and token_stride at least head_dim");
+    // the byte strides must stay below 2^40, where the tiled copies can address them
+    const long long most = (1ll << 40) / b - 1;
+    if (p->page_stride > most || p->head_stride > most || p->token_stride > most) return fail(who, "stride too large");
+    if (p->page_stride * b % 16 || p->head_stride * b % 16 || p->token_stride * b % 16)
+        return fail(who, "page, head and token strides must be multiples of 16 bytes");
+    if (!p->k || !p->v || !aligned(p->k) || !aligned(p->v)) return fail(who, "k and v must be 16-byte aligned pointers");
+    return 0;
+}
+
+inline int check_seqs(const char *who, const mocha_kv_seqs *s)
+{
+    if (!s) return fail(who, "null seqs");
+    if (s->seqs < 0) return fail(who, "seqs must not be negative");
+    if (s->table_width < 1 || s->table_stride < s->table_width) return fail(who, "table_width must be positive and table_stride at least that");
+    if (s->seqs && !s->table) return fail(who, "null table");
+    return 0;
+}
+
+inline int check_rows(const char *who, const char *name, const mocha_kv_rows *r, int bytes, int dim, int rows)
+{
+    const long long most = (1ll << 40) / bytes - 1;
+    if (!r || (rows && !r->data)) return fprintf(stderr, "%s: null %s\n", who, name), 1;
+    if (!aligned(r->data) || r->row_stride < 0 || r->head_stride < dim || r->row_stride > most || r->head_stride > most ||
+        r->row_stride * bytes % 16 || r->head_stride * bytes % 16) {
+        fprintf(stderr, "%s: %s must be 16-byte aligned with strides that are multiples of 16 bytes and a head stride of at least head_dim\n", who, name);
+        return 1;
+    }
+    return 0;
+}
+
+inline int check_scores(const char *who, const mocha_kv_pages *p, const mocha_kv_scores *s)
+{
+    if (!s) return fail(who, "null scores");
+    if (s->heads < 1 || s->heads % p->kv_heads || s->heads / p->kv_heads > kMaxGroup)
+        return fail(who, "heads must be a multiple of kv_heads, at most 64 times as many");
+    if (!isfinite(s->scale) || !isfinite(s->cap) || s->cap < 0.f) return fail(who, "scale and cap must be finite and cap not negative");
+    if (s->window < 0) return fail(who, "window must not be negative");
+    return 0;
+}
+
+inline int max_len(const mocha_kv_pages *p, const mocha_kv_seqs *s)
+{
+    const long long n = (long long)s->table_width * p->page_size;
+    return n > INT_MAX - 65536 ? INT_MAX - 65536 : (int)n;  // a tile past the last position must not overflow
+}
+
+inline Args make_args(const mocha_kv_pages *p, const mocha_kv_seqs *s, const mocha_kv_scores *z, const mocha_kv_rows *q,
+                      const mocha_kv_rows *out, float *lse)
+{
+    Args a{};
+    a.k = (const char *)p->k;
+    a.v = (const char *)p->v;
+    a.ps = p->page_stride;
+    a.hs = p->head_stride;
+    a.ts = p->token_stride;
+    a.pages = p->pages;
+    a.kv_heads = p->kv_heads;
+    a.d = p->head_dim;
+    a.page = fast_div(p->page_size);
+    a.table = s->table;
+    a.table_stride = s->table_stride;
+    a.max_len = max_len(p, s);
+    a.kv_len = s->kv_len;
+    a.status = s->status;
+    a.seqs = s->seqs;
+    a.heads = z->heads;
+    a.group = z->heads / p->kv_heads;
+    a.group_div = fast_div(a.group);
+    a.window = z->window;
+    a.scale = z->scale;
+    a.cap = z->cap;
+    a.prefix = z->prefix;
+    a.slopes = z->slopes;
+    a.q = (const char *)q->data;
+    a.q_row = q->row_stride;
+    a.q_head = q->head_stride;
+    a.out = (char *)out->data;
+    a.o_row = out->row_stride;
+    a.o_head = out->head_stride;
+    a.lse = lse;
+    return a;
+}
+
+// Launch with an error message; `after`: the kernel may start while the one before it in
+// the stream ends, and waits for it itself.
+template <typename... K, typename... A>
+int launch(const char *who, void (*kernel)(K...), dim3 grid, int threads, size_t smem, cudaStream_t s, bool after, A &&...args)
+{
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return (void)cudaGetLastError(), fail(who, cudaGetErrorString(e));
+    }
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &at;
+    cfg.numAttrs = after ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+    if (e != cudaSuccess) return (void)cudaGetLastError(), fail(who, cudaGetErrorString(e));
+    return 0;
+}
+
+// Workspace of one call: the CTAs' notes of cut units, then their parts.
+inline size_t meta_bytes(int ctas) { return ((size_t)ctas * sizeof(Meta) + 255) / 256 * 256; }
+inline size_t part_bytes(int ctas, int rows, int dp) { return (size_t)ctas * 2 * rows * (dp + 2) * sizeof(float); }
+inline int padded_dim(int d) { return d <= 64 ? 64 : 128; }
+
+}  // namespace kv
