@@ -4,6 +4,8 @@
 // row r of the unit is token r / group, head r % group, so the heads of a group share the
 // key and value tiles and a short piece still fills a tile.  Its key tiles are shared out
 // over the CTAs (kv_common.cuh).
+#include <type_traits>
+
 #include "kv_common.cuh"
 
 namespace {
@@ -367,6 +369,513 @@ __global__ void __launch_bounds__(kThreads) k_prefill(const __grid_constant__ Ar
     }
 }
 
+
+// ---- 16-bit types: the tensor cores ----------------------------------------------------
+// One CTA per SM with two tiles of 128 query rows.  A producer warp copies queries, keys and
+// values into shared memory by TMA (a page or a part of one per copy, 128-byte swizzle), one
+// thread issues the products, and four warps per tile, a row per thread, turn scores into
+// weights.  Scores S = Q K^T and outputs O += P V are accumulated in TMEM; P goes back to
+// TMEM over the scores it came from and is the second product's first operand there.  While
+// the warps of one tile work on its weights the tensor core has the other tile's products,
+// so the products (4 * 128 * 128 * dim operations per tile and key tile) bound the kernel
+// as long as the weights of a tile take no longer than the other's products.
+//
+// The maximum that a row's weights are taken from is renewed only when it is exceeded by
+// 2^8, so outputs are rescaled a few times per row and not per tile; weights then are at
+// most 2^8, sums and outputs stay exact to their type.
+constexpr int kTcThreads = 320;  // warps 0-3 and 4-7: weights of the two tiles; 8: products; 9: copies
+constexpr int kTcKeys = 128;
+
+struct Maps {
+    CUtensorMap q, k, v;
+};
+
+template <int DP>
+struct SmemTc {
+    static constexpr int kTile = 128 * DP * 2;           // bytes of a tile of 128 rows
+    static constexpr int kStages = DP == 128 ? 5 : 10;   // key and value tiles in flight
+    static constexpr int kTotal = 1024 + 2 * kTile + kStages * kTile;
+};
+
+struct TcBars {
+    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], kv_full[10], kv_empty[10], edge, drain;
+    uint32_t tmem;
+    volatile int abort;
+};
+
+MB_DEV void tma_load_4d(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, int c3, uint64_t *bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(mb::as::smem_u32(bar))
+        : "memory");
+}
+
+// Descriptor of a value tile as the second operand: its rows (keys) are the summed
+// dimension, so the operand is "MN-major": 64 dims in a 128-byte row, `block` bytes on to the
+// next 64 dims, 1024 bytes to the next 8 keys.
+MB_DEV uint64_t mn_desc(uint32_t addr, int block)
+{
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// D[tmem] (+)= A[tmem] * B[smem], issued by one thread.
+MB_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, bool accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+
+#define KV_O8(x, i) "=f"(x[i]), "=f"(x[i + 1]), "=f"(x[i + 2]), "=f"(x[i + 3]), "=f"(x[i + 4]), "=f"(x[i + 5]), "=f"(x[i + 6]), "=f"(x[i + 7])
+#define KV_F8(x, i) "f"(x[i]), "f"(x[i + 1]), "f"(x[i + 2]), "f"(x[i + 3]), "f"(x[i + 4]), "f"(x[i + 5]), "f"(x[i + 6]), "f"(x[i + 7])
+#define KV_I8(x, i) "r"(x[i]), "r"(x[i + 1]), "r"(x[i + 2]), "r"(x[i + 3]), "r"(x[i + 4]), "r"(x[i + 5]), "r"(x[i + 6]), "r"(x[i + 7])
+
+// 32 TMEM columns of this thread's row, to x[I..I + 31].
+template <int I, int N>
+MB_DEV void tmem_ld32(uint32_t addr, float (&x)[N])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : KV_O8(x, I), KV_O8(x, I + 8), KV_O8(x, I + 16), KV_O8(x, I + 24)
+        : "r"(addr));
+}
+template <int I, int N>
+MB_DEV void tmem_st32(uint32_t addr, const float (&x)[N])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::KV_F8(x, I),
+        KV_F8(x, I + 8), KV_F8(x, I + 16), KV_F8(x, I + 24), "r"(addr));
+}
+// 16 TMEM columns.
+MB_DEV void tmem_st16(uint32_t addr, const uint32_t (&x)[16])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::KV_I8(x, 0),
+                 KV_I8(x, 8), "r"(addr));
+}
+MB_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two roundings in one instruction.
+template <typename T>
+MB_DEV uint32_t pack16(float x, float y)
+{
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+
+// 2^x by the hardware's exponential (2 ulp and subnormal results as zero, far below what
+// rounding a weight to 16 bits costs).
+MB_DEV float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// c tanh(z / c) = c - 2 c / (1 + exp(2 z / c)).
+MB_DEV float capped(float z, float cap, float k) { return cap - __fdividef(2.f * cap, 1.f + ex2(z * k)); }
+
+template <typename T, int DP, bool EXTRA>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    k_prefill_tc(const __grid_constant__ Args a, const __grid_constant__ Maps maps, int tok, int box, int min_tiles)
+{
+    using namespace mb::as;
+    using S = SmemTc<DP>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ TcBars bar;
+    ShareSmem &share = *reinterpret_cast<ShareSmem *>(smem);  // before the tiles
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tokens = 2 * tok;
+    griddep_launch();
+    if (tid == 0) {
+        for (int x = 0; x < 2; x++) {
+            mbar_init(&bar.q_full[x], 1);
+            mbar_init(&bar.q_empty[x], 1);
+            mbar_init(&bar.s_full[x], 1);
+            mbar_init(&bar.p_full[x], 128);
+            mbar_init(&bar.o_full[x], 1);
+        }
+        for (int i = 0; i < S::kStages; i++) {
+            mbar_init(&bar.kv_full[i], 1);
+            mbar_init(&bar.kv_empty[i], 1);
+        }
+        mbar_init(&bar.edge, 1);
+        mbar_init(&bar.drain, 1);
+        bar.abort = 0;
+        fence_barrier_init();
+    }
+    const bool any = find_share<kTcKeys, kTcThreads>(a, tokens, min_tiles, share);
+    if (!any) {
+        if (tid == 0) a.meta[blockIdx.x].c_end = -1;
+        return;
+    }
+    const Share h = share.out;
+    if (warp == 8) tmem_alloc(&bar.tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bar.tmem;
+    const uint32_t sq = smem_u32(smem), skv = sq + 2 * S::kTile;
+    Units<kTcKeys> u;
+    u.start(a, h, tokens);
+    int i = h.i;
+    long long left = h.end - h.start;
+    bool ok = true;
+
+    if (warp == 9) {
+        // copies
+        int it = 0, edges = 0, asked[2] = {0, 0};
+        while (left > 0 && ok) {
+            const int tok0 = u.block * tokens, ntok = min(tokens, u.p.nq - tok0);
+            const int stop = (int)min((long long)u.t.n, i + left);
+            const int pa = u.p.pos(tok0), pb = pa + ntok - 1;
+            left -= stop - i;
+            for (int x = 0; x < 2 && x * tok < ntok; x++) {
+                // the tile's queries, once the unit before no longer reads it
+                ok = ok && mbar_wait(&bar.q_empty[x], (asked[x]++ & 1) ^ 1, &bar.abort);
+                if (ok && lane == 0) {
+                    mbar_expect_tx(&bar.q_full[x], (uint32_t)(DP * 2 * tok * a.group));
+                    for (int b = 0; b < DP / 64; b++)
+                        tma_load_4d(sq + x * S::kTile + b * (128 * 128), &maps.q, 64 * b, 0, u.kvh, u.p.q0 + tok0 + x * tok, &bar.q_full[x]);
+                }
+            }
+            for (; i < stop && ok; i++) {
+                const int j0 = u.t.key(i);
+                const int keys = min(kTcKeys, u.p.len - j0);           // keys there are (not positive: none)
+                const int boxes = keys > 0 ? (keys + box - 1) / box : 0;
+                const bool edge = keys < kTcKeys;
+                for (int v = 0; v < 2 && ok; v++, it++) {
+                    const int st = it % S::kStages;
+                    ok = mbar_wait(&bar.kv_empty[st], ((it / S::kStages) & 1) ^ 1, &bar.abort);
+                    if (!ok) break;
+                    const uint32_t dst = skv + st * S::kTile;
+                    uint64_t *full = v && edge ? &bar.edge : &bar.kv_full[st];
+                    if (lane == 0) mbar_expect_tx(full, (uint32_t)(boxes * box * DP * 2));
+                    __syncwarp();
+                    for (int b = lane; b < boxes; b += 32) {
+                        const int j = j0 + b * box;
+                        const uint32_t slot = div(a.page, j);
+                        const int id = __ldg(a.table + u.seq * a.table_stride + slot);
+                        if ((unsigned)id >= (unsigned)a.pages && a.status) {
+                            bool seen = false;
+                            for (int y = 0; y < box && j + y < u.p.len; y++)
+                                seen |= (j + y <= pb && (a.window == 0 || pa - (j + y) < a.window)) || j + y < u.p.pre;
+                            if (seen) *a.status = 1;
+                        }
+                        for (int c = 0; c < DP / 64; c++)
+                            tma_load_4d(dst + c * (128 * 128) + b * box * 128, v ? &maps.v : &maps.k, 64 * c, j - (int)(slot * a.page.d), u.kvh, id, full);
+                    }
+                    if (v && edge) {
+                        // rows past the sequence's end hold anything: 0 * NaN must not reach the sums
+                        ok = mbar_wait(&bar.edge, edges & 1, &bar.abort);
+                        edges++;
+                        const int r0 = max(keys, 0);
+                        for (int e = lane; e < (128 - r0) * (DP / 8); e += 32) {
+                            const int r = r0 + e / (DP / 8), c = e % (DP / 8);
+                            *reinterpret_cast<uint4 *>(smem + 2 * S::kTile + st * S::kTile + (c / 8) * (128 * 128) + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bar.kv_full[st]);
+                    }
+                }
+            }
+            if (left > 0) u.next(a, tokens);
+            i = 0;
+        }
+        if (!ok) bar.abort = 1;
+    } else if (warp == 8) {
+        if (lane == 0) {
+            // products
+            constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
+            constexpr uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
+            constexpr uint32_t id_qk = base | ((128u >> 3) << 17), id_pv = base | (1u << 16) | ((uint32_t)(DP >> 3) << 17);
+            int it = 0, steps[2] = {0, 0}, units[2] = {0, 0};  // steps: weights taken; units: queries taken
+            auto qk = [&](int x, int st) {
+                const uint32_t q = sq + x * S::kTile, k = skv + st * S::kTile;
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; kk++) {
+                    const uint32_t off = (kk / 4) * (128 * 128) + (kk % 4) * 32;
+                    mma_bf16(tmem + x * 128, sw128_desc(q + off), sw128_desc(k + off), id_qk, kk > 0);
+                }
+                mma_commit(&bar.s_full[x]);
+            };
+            auto pv = [&](int x, int st, bool accumulate) {
+                const uint32_t v = skv + st * S::kTile;
+#pragma unroll
+                for (int kk = 0; kk < 8; kk++)
+                    mma_ts(tmem + 256 + x * 128, tmem + x * 128 + 64 + kk * 8, mn_desc(v + kk * 2048, 128 * 128), id_pv, accumulate || kk > 0);
+                mma_commit(&bar.o_full[x]);
+            };
+            auto full = [&](int n) {
+                ok = ok && mbar_wait(&bar.kv_full[n % S::kStages], (n / S::kStages) & 1, &bar.abort);
+                tc_fence_after();
+            };
+            while (left > 0 && ok) {
+                const int ntok = min(tokens, u.p.nq - u.block * tokens);
+                const int stop = (int)min((long long)u.t.n, i + left), n = stop - i;
+                const int tiles = ntok > tok ? 2 : 1;
+                left -= n;
+                full(it);
+                for (int x = 0; x < tiles && ok; x++) {
+                    ok = mbar_wait(&bar.q_full[x], units[x]++ & 1, &bar.abort);
+                    tc_fence_after();
+                    if (ok) qk(x, it % S::kStages);
+                    if (n == 1) mma_commit(&bar.q_empty[x]);
+                }
+                if (ok) mma_commit(&bar.kv_empty[it % S::kStages]);
+                for (int j = 0; j < n && ok; j++) {
+                    const int vt = it + 1, kt = it + 2;
+                    for (int x = 0; x < tiles && ok; x++) {
+                        if (x == 0) full(vt);
+                        ok = ok && mbar_wait(&bar.p_full[x], steps[x]++ & 1, &bar.abort);
+                        tc_fence_after();
+                        if (!ok) break;
+                        pv(x, vt % S::kStages, j > 0);
+                        if (j + 1 < n) {
+                            if (x == 0) full(kt);
+                            if (!ok) break;
+                            qk(x, kt % S::kStages);
+                            if (j + 2 == n) mma_commit(&bar.q_empty[x]);
+                        }
+                    }
+                    if (!ok) break;
+                    mma_commit(&bar.kv_empty[vt % S::kStages]);
+                    if (j + 1 < n) mma_commit(&bar.kv_empty[kt % S::kStages]);
+                    it += 2;
+                }
+                if (left > 0) u.next(a, tokens);
+                i = 0;
+            }
+            if (!ok) bar.abort = 1;
+            mma_commit(&bar.drain);
+            int never = 0;
+            mbar_wait(&bar.drain, 0, &never);
+        }
+    } else {
+        // weights: thread = row of tile x
+        const int x = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + x * 128 + lanes, to = tmem + 256 + x * 128 + lanes;
+        const int t = div(a.group_div, r);
+        const float k2 = EXTRA ? 1.f : a.scale * kLog2e, kcap = EXTRA && a.cap > 0.f ? 2.f * kLog2e / a.cap : 0.f;
+        uint32_t step = 0;
+        while (left > 0 && ok) {
+            const int tok0 = u.block * tokens, ntok = min(tokens, u.p.nq - tok0);
+            const int first = i, stop = (int)min((long long)u.t.n, i + left);
+            left -= stop - i;
+            const bool whole = first == 0 && stop == u.t.n;
+            const int pa = u.p.pos(tok0);
+            if (x * tok < ntok) {
+                const int head = u.kvh * a.group + r - t * a.group;
+                const bool mine = t < tok && x * tok + t < ntok;
+                const int p0 = pa + x * tok, p1 = p0 + min(tok, ntok - x * tok) - 1, p = p0 + t;
+                const int hi = min(p + 1, u.p.len), lo = a.window ? max(p - a.window + 1, 0) : 0;
+                const float slope = EXTRA && a.slopes && mine ? __ldg(a.slopes + head) : 0.f;
+                float m = -INFINITY, l = 0.f;
+                for (; i < stop; i++, step++) {
+                    const int j0 = u.t.key(i);
+                    ok = mbar_wait(&bar.s_full[x], step & 1, &bar.abort);
+                    if (!__all_sync(0xffffffffu, ok)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const bool full = (j0 + kTcKeys <= min(p0 + 1, u.p.len) && (a.window == 0 || p1 - j0 < a.window)) || j0 + kTcKeys <= u.p.pre;
+                    // the scores, 32 columns at a time: once for the maximum, the last 32 kept
+                    // and the others read again for the weights (all 128 do not fit the registers);
+                    // what masks and options change is put back
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    auto first_look = [&](float (&s)[32], int c0) {
+                        if (EXTRA || !full) {
+                            const unsigned span = hi > lo ? hi - lo : 0;
+#pragma unroll
+                            for (int c = 0; c < 32; c++) {
+                                const int j = j0 + c0 + c;
+                                if (EXTRA) {
+                                    float z = s[c] * a.scale;
+                                    if (a.cap > 0.f) z = capped(z, a.cap, kcap);
+                                    s[c] = fmaf(-slope, fabsf((float)(p - j)), z) * kLog2e;
+                                }
+                                if (!((unsigned)(j - lo) < span || j < u.p.pre)) s[c] = -INFINITY;
+                            }
+                            if (c0 < 96) tmem_st32<0>(ts + c0, s);
+                        }
+#pragma unroll
+                        for (int c = 0; c < 32; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+                    };
+                    float sa[32], sb[32];
+                    tmem_ld32<0>(ts, sa);
+                    tmem_wait_ld();
+                    tmem_ld32<0>(ts + 32, sb);
+                    first_look(sa, 0);
+                    tmem_wait_ld();
+                    tmem_ld32<0>(ts + 64, sa);
+                    first_look(sb, 32);
+                    tmem_wait_ld();
+                    tmem_ld32<0>(ts + 96, sb);
+                    first_look(sa, 64);
+                    tmem_wait_ld();
+                    first_look(sb, 96);
+                    if (EXTRA || !full) tmem_wait_st();
+                    const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    // a new maximum, and the output so far to its scale
+                    float f = 1.f;
+                    if ((mn - m) * k2 > 8.f) {
+                        f = ex2((m - mn) * k2);
+                        m = mn;
+                    }
+                    if (i > first && __any_sync(0xffffffffu, f != 1.f)) {
+                        ok = mbar_wait(&bar.o_full[x], (step & 1) ^ 1, &bar.abort);
+                        if (!__all_sync(0xffffffffu, ok)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+#pragma unroll
+                        for (int c = 0; c < DP / 32; c++) {
+                            float o[32];
+                            tmem_ld32<0>(to + 32 * c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] *= f;
+                            tmem_st32<0>(to + 32 * c, o);
+                        }
+                    }
+                    const float sub = m == -INFINITY ? 0.f : -m * k2;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    // weights of columns c0.. go to columns 64 + c0 / 2.., which have been read
+                    auto weigh = [&](const float (&s)[32], int c0) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const float e0 = ex2(fmaf(s[2 * e], k2, sub)), e1 = ex2(fmaf(s[2 * e + 1], k2, sub));
+                            sum[(2 * e) & 3] += e0;
+                            sum[(2 * e + 1) & 3] += e1;
+                            w[e] = pack16<T>(e0, e1);
+                        }
+                        tmem_st16(ts + 64 + c0 / 2, w);
+                    };
+                    tmem_ld32<0>(ts + 64, sa);
+                    weigh(sb, 96);
+                    tmem_wait_ld();
+                    tmem_ld32<0>(ts + 32, sb);
+                    weigh(sa, 64);
+                    tmem_wait_ld();
+                    tmem_ld32<0>(ts, sa);
+                    weigh(sb, 32);
+                    tmem_wait_ld();
+                    weigh(sa, 0);
+                    l = fmaf(l, f, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&bar.p_full[x]);
+                }
+                if (!ok) break;
+                ok = mbar_wait(&bar.o_full[x], (step & 1) ^ 1, &bar.abort);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const int at = (x * tok + t) * a.group + (r - t * a.group);
+                const long long row = u.p.q0 + tok0 + x * tok + t;
+                float *part = a.part + ((size_t)blockIdx.x * 2 + (first == 0 ? 1 : 0)) * ((size_t)256 * (DP + 2));
+                const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+                const float ms = m == -INFINITY ? 0.f : m * k2;
+                bool bad = false;
+#pragma unroll
+                for (int c = 0; c < DP / 32; c++) {
+                    float o[32];
+                    tmem_ld32<0>(to + 32 * c, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        o[e] *= inv;
+                        bad |= !isfinite(o[e]);
+                    }
+                    if (mine && !whole) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            *reinterpret_cast<float4 *>(part + (size_t)at * DP + 32 * c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    } else if (mine && 32 * c < a.d) {
+                        T *dst = reinterpret_cast<T *>(a.out) + row * a.o_row + head * a.o_head + 32 * c;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            uint4 y;
+                            y.x = pack16<T>(o[e], o[e + 1]);
+                            y.y = pack16<T>(o[e + 2], o[e + 3]);
+                            y.z = pack16<T>(o[e + 4], o[e + 5]);
+                            y.w = pack16<T>(o[e + 6], o[e + 7]);
+                            *reinterpret_cast<uint4 *>(dst + e) = y;
+                        }
+                    }
+                }
+                if (mine) {
+                    if (!whole) {
+                        part[(size_t)256 * DP + 2 * at] = m == -INFINITY ? m : ms;
+                        part[(size_t)256 * DP + 2 * at + 1] = l;
+                    } else if (a.lse)
+                        a.lse[row * a.heads + head] = l == 0.f ? -INFINITY : (ms + log2f(l)) * kLn2;
+                }
+                tc_fence_before();
+                unsigned again = __ballot_sync(0xffffffffu, mine && whole && bad);
+                while (again) {
+                    const int f = __ffs(again) - 1;
+                    again &= again - 1;
+                    const int fp = __shfl_sync(0xffffffffu, p, f), fh = __shfl_sync(0xffffffffu, head, f), fr = __shfl_sync(0xffffffffu, (int)row, f);
+                    lone_row<T>(a, u.seq, fp, fh, fr);
+                }
+            }
+            if (left <= 0 && tid == 0) {
+                Meta mt{};
+                mt.c_end = -1;
+                if (first == 0 && !whole) {
+                    mt.c_end = (int)((h.end - 1 + (u.t.n - stop)) / h.per);
+                    mt.row0 = u.p.q0 + tok0;
+                    mt.ntok = ntok;
+                    mt.head0 = u.kvh * a.group;
+                    mt.ng = a.group;
+                    mt.seq = u.seq;
+                    mt.pos0 = pa;
+                }
+                a.meta[blockIdx.x] = mt;
+            }
+            if (left > 0) u.next(a, tokens);
+            i = 0;
+        }
+        if (!ok) bar.abort = 1;
+    }
+    __syncthreads();
+    if (bar.abort) {
+        // a wait ran out: no notes for the join, and the copies in flight land first
+        if (tid == 0) {
+            a.meta[blockIdx.x].c_end = -1;
+            if (a.status) *a.status = 2;
+            const long long t0 = clock64();
+            while (clock64() - t0 < kWaitCycles / 64) {
+            }
+        }
+        __syncthreads();
+    }
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_free(tmem, 512);
+    }
+}
+
 template <typename T, int DP>
 int run(Args &a, int ctas, cudaStream_t s)
 {
@@ -376,15 +885,67 @@ int run(Args &a, int ctas, cudaStream_t s)
     return launch(who, k_join<T, true>, dim3(ctas, 8), 32 * kJoinWarps, 0, s, true, a, kRows, DP);
 }
 
+// ---- tensor maps -----------------------------------------------------------------------
+
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                             const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn()
+{
+    static const EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
+        return (EncodeFn)p;
+    }();
+    return fn;
+}
+
+// A map of [n3][n2][n1][dim] 16-bit values with byte strides s1..s3 and a box of 64 x b1 x 1 x b3;
+// what lies past an extent reads as zeros.
+int encode(CUtensorMap *map, int type, const void *base, const long long (&n)[4], const long long (&s)[3], int b1, int b3)
+{
+    const cuuint64_t dims[4] = {(cuuint64_t)n[0], (cuuint64_t)n[1], (cuuint64_t)n[2], (cuuint64_t)n[3]};
+    cuuint64_t strides[3];
+    for (int i = 0; i < 3; i++) strides[i] = n[i + 1] > 1 ? (cuuint64_t)s[i] : 16;  // of one line: any valid one
+    const cuuint32_t box[4] = {64, (cuuint32_t)b1, 1, (cuuint32_t)b3}, one[4] = {1, 1, 1, 1};
+    const EncodeFn fn = encode_fn();
+    return fn && fn(map, type == MOCHA_KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                    const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DP>
+int run_tc(Args &a, const mocha_kv_pages *p, cudaStream_t s)
+{
+    const char *who = "mocha_kv_prefill";
+    const int tok = 128 / a.group, d = a.d;
+    int box = 128;
+    while (p->page_size % box) box /= 2;
+    Maps maps;
+    if (!encode(&maps.q, p->type, a.q, {d, a.group, a.kv_heads, a.rows}, {a.q_head * 2, a.q_head * 2 * a.group, a.q_row * 2}, a.group, tok) ||
+        !encode(&maps.k, p->type, a.k, {d, p->page_size, a.kv_heads, a.pages}, {a.ts * 2, a.hs * 2, a.ps * 2}, box, 1) ||
+        !encode(&maps.v, p->type, a.v, {d, p->page_size, a.kv_heads, a.pages}, {a.ts * 2, a.hs * 2, a.ps * 2}, box, 1))
+        return fail(who, "the tensor maps cannot be encoded");
+    const bool extra = a.cap > 0.f || a.slopes || !(a.scale > 0.f);
+    const int ctas = mb::kSMs;
+    if (extra ? launch(who, k_prefill_tc<T, DP, true>, dim3(ctas), kTcThreads, SmemTc<DP>::kTotal, s, false, a, maps, tok, box, 4)
+              : launch(who, k_prefill_tc<T, DP, false>, dim3(ctas), kTcThreads, SmemTc<DP>::kTotal, s, false, a, maps, tok, box, 4))
+        return 1;
+    return launch(who, k_join<T, true>, dim3(ctas, 16), 32 * kJoinWarps, 0, s, true, a, 256, DP);
+}
+
 }  // namespace
 
 namespace kv {
 size_t decode_workspace(int type, int group, int d);
 
+static int prefill_ctas(int type) { return type == MOCHA_KV_F32 ? 2 * mb::kSMs : mb::kSMs; }
 static size_t prefill_workspace(int type, int d)
 {
-    (void)type;
-    return meta_bytes(2 * mb::kSMs) + part_bytes(2 * mb::kSMs, kRows, padded_dim(d));
+    const int n = prefill_ctas(type);
+    return meta_bytes(n) + part_bytes(n, type == MOCHA_KV_F32 ? kRows : 256, padded_dim(d));
 }
 }  // namespace kv
 
@@ -418,14 +979,14 @@ extern "C" int mocha_kv_prefill(const mocha_kv_pages *pages, const mocha_kv_seqs
     a.rows = rows;
     if (!workspace || !aligned(workspace) || workspace_bytes < kv::prefill_workspace(pages->type, d))
         return fail(who, "workspace missing, not 16-byte aligned or smaller than mocha_kv_workspace says");
-    const int ctas = 2 * mb::kSMs;
+    const int ctas = kv::prefill_ctas(pages->type);
     a.meta = static_cast<Meta *>(workspace);
     a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + meta_bytes(ctas));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool narrow = padded_dim(d) == 64;
     switch (pages->type) {
     case MOCHA_KV_F32: return narrow ? run<float, 64>(a, ctas, s) : run<float, 128>(a, ctas, s);
-    case MOCHA_KV_F16: return narrow ? run<__half, 64>(a, ctas, s) : run<__half, 128>(a, ctas, s);
-    default: return narrow ? run<__nv_bfloat16, 64>(a, ctas, s) : run<__nv_bfloat16, 128>(a, ctas, s);
+    case MOCHA_KV_F16: return narrow ? run_tc<__half, 64>(a, pages, s) : run_tc<__half, 128>(a, pages, s);
+    default: return narrow ? run_tc<__nv_bfloat16, 64>(a, pages, s) : run_tc<__nv_bfloat16, 128>(a, pages, s);
     }
 }
