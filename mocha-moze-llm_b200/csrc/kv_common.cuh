@@ -198,98 +198,141 @@ __device__ __noinline__ void lone_row(const Args &a, int seq, int p, int head, i
 }
 
 // ---- join of the parts of cut units --------------------------------------------------
-// Block (c, y): rows y, y + gridDim.y, ... of the unit that begins and is cut in CTA c; the
-// block's warps take parts in turn, lanes the dims.
-constexpr int kJoinWarps = 8;
+// The rows of all cut units are dealt to the blocks: a warp takes a row whose parts are
+// few, a block one whose parts are many (more than kJoinSerial), lanes the dims.  Bound by
+// the parts' bytes: each is read once.
+constexpr int kJoinWarps = 8, kJoinSerial = 32, kJoinMetas = 2 * mb::kSMs;
+
+struct Joined {
+    float m, l;
+    float4 acc;
+    MB_DEV void add(float pm, float pl, float4 v, float ms)
+    {
+        const float f = exp2f(pm - ms);
+        l = fmaf(pl, f, l);
+        acc.x = fmaf(v.x, f, acc.x);
+        acc.y = fmaf(v.y, f, acc.y);
+        acc.z = fmaf(v.z, f, acc.z);
+        acc.w = fmaf(v.w, f, acc.w);
+    }
+    MB_DEV void rescale(float mn, float ms)
+    {
+        const float f = exp2f(m - ms);
+        l *= f;
+        acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+        m = mn;
+    }
+};
 
 template <typename T, bool PREFILL>
-__global__ void __launch_bounds__(32 * kJoinWarps) k_join(const __grid_constant__ Args a, int part_rows, int dp)
+__global__ void __launch_bounds__(32 * kJoinWarps) k_join(const __grid_constant__ Args a, int metas, int part_rows, int dp)
 {
-    __shared__ float4 s_acc[kJoinWarps][32];
-    __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
+    __shared__ Joined s_part[kJoinWarps][32];
+    __shared__ int s_items[kJoinMetas], s_warp[kJoinWarps], s_total;
     mb::as::griddep_wait();
-    const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const Meta mt = a.meta[c];
-    if (mt.c_end < 0) return;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // items (a block's work) before each unit's end, in the order of the CTAs
+    int n[2] = {0, 0};
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const int c = 2 * tid + x;
+        if (c >= metas) continue;
+        const int end = __ldcg(&a.meta[c].c_end);
+        if (end < 0) continue;
+        const int rows = __ldcg(&a.meta[c].ntok) * __ldcg(&a.meta[c].ng);
+        n[x] = end - c < kJoinSerial ? (rows + kJoinWarps - 1) / kJoinWarps : rows;
+    }
+    int incl = n[0] + n[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += x;
+    }
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    for (int w = 0; w < warp; w++) incl += s_warp[w];
+    if (2 * tid < metas) s_items[2 * tid] = incl - n[1];
+    if (2 * tid + 1 < metas) s_items[2 * tid + 1] = incl;
+    if (tid == 32 * kJoinWarps - 1) s_total = incl;
+    __syncthreads();
+    const int total = s_total;
     const size_t slot = (size_t)part_rows * (dp + 2);
-    for (int r = blockIdx.y; r < mt.ntok * mt.ng; r += gridDim.y) {
-        float m = -INFINITY, l = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        constexpr int U = 4;  // parts in flight per warp
-        for (int b = c + warp * U; b <= mt.c_end; b += kJoinWarps * U) {
-            float pm[U], pl[U];
-            float4 pv[U];
+    for (int item = blockIdx.x; item < total; item += gridDim.x) {
+        int c = 0;  // the first unit that ends after `item`
+        for (int step = 256; step; step >>= 1)
+            if (c + step <= metas && s_items[c + step - 1] <= item) c += step;
+        const Meta mt = a.meta[c];
+        const int first = c ? s_items[c - 1] : 0;
+        const bool serial = mt.c_end - c < kJoinSerial;
+        const int r = serial ? (item - first) * kJoinWarps + warp : item - first;
+        const bool there = r < mt.ntok * mt.ng;
+        Joined x{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+        constexpr int U = 8;  // parts in flight per warp
+        if (there)
+            for (int b = c + (serial ? 0 : warp * U); b <= mt.c_end; b += serial ? U : kJoinWarps * U) {
+                float pm[U], pl[U];
+                float4 pv[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                pm[u] = -INFINITY;
-                pl[u] = 0.f;
-                pv[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (b + u <= mt.c_end) {
-                    const float *pp = a.part + ((size_t)(b + u) * 2 + (b + u == c ? 1 : 0)) * slot;
-                    pm[u] = __ldcg(pp + (size_t)part_rows * dp + 2 * r);
-                    pl[u] = __ldcg(pp + (size_t)part_rows * dp + 2 * r + 1);
-                    if (lane * 4 < a.d) pv[u] = __ldcg(reinterpret_cast<const float4 *>(pp + (size_t)r * dp) + lane);
+                for (int u = 0; u < U; u++) {
+                    pm[u] = -INFINITY;
+                    pl[u] = 0.f;
+                    pv[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (b + u <= mt.c_end) {
+                        const float *pp = a.part + ((size_t)(b + u) * 2 + (b + u == c ? 1 : 0)) * slot;
+                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(pp + (size_t)part_rows * dp) + r);
+                        pm[u] = ml.x;
+                        pl[u] = ml.y;
+                        if (lane * 4 < a.d) pv[u] = __ldcg(reinterpret_cast<const float4 *>(pp + (size_t)r * dp) + lane);
+                    }
                 }
-            }
-            float mn = m;
+                float mn = x.m;
 #pragma unroll
-            for (int u = 0; u < U; u++) mn = fmaxf(mn, pm[u]);
-            const float ms = mn == -INFINITY ? 0.f : mn;
-            float f = exp2f(m - ms);
-            l *= f;
-            acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+                for (int u = 0; u < U; u++) mn = fmaxf(mn, pm[u]);
+                const float ms = mn == -INFINITY ? 0.f : mn;
+                x.rescale(mn, ms);
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                f = exp2f(pm[u] - ms);
-                l = fmaf(pl[u], f, l);
-                acc.x = fmaf(pv[u].x, f, acc.x);
-                acc.y = fmaf(pv[u].y, f, acc.y);
-                acc.z = fmaf(pv[u].z, f, acc.z);
-                acc.w = fmaf(pv[u].w, f, acc.w);
+                for (int u = 0; u < U; u++) x.add(pm[u], pl[u], pv[u], ms);
             }
-            m = mn;
+        if (!serial) {
+            s_part[warp][lane] = x;
+            __syncthreads();
+            if (warp == 0) {
+                float mn = x.m;
+#pragma unroll
+                for (int w = 1; w < kJoinWarps; w++) mn = fmaxf(mn, s_part[w][0].m);
+                const float ms = mn == -INFINITY ? 0.f : mn;
+                x.rescale(mn, ms);
+#pragma unroll
+                for (int w = 1; w < kJoinWarps; w++) x.add(s_part[w][lane].m, s_part[w][lane].l, s_part[w][lane].acc, ms);
+            }
+            __syncthreads();
         }
-        s_acc[warp][lane] = acc;
-        if (lane == 0) {
-            s_m[warp] = m;
-            s_l[warp] = l;
-        }
-        __syncthreads();
-        if (warp == 0) {
-            float M = s_m[0];
-#pragma unroll
-            for (int w = 1; w < kJoinWarps; w++) M = fmaxf(M, s_m[w]);
-            const float ms = M == -INFINITY ? 0.f : M;
-            l = 0.f;
-            acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < kJoinWarps; w++) {
-                const float f = exp2f(s_m[w] - ms);
-                const float4 x = s_acc[w][lane];
-                l = fmaf(s_l[w], f, l);
-                acc.x = fmaf(x.x, f, acc.x);
-                acc.y = fmaf(x.y, f, acc.y);
-                acc.z = fmaf(x.z, f, acc.z);
-                acc.w = fmaf(x.w, f, acc.w);
-            }
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (there && (serial || warp == 0)) {
+            const float inv = x.l == 0.f ? 0.f : 1.f / x.l;
             const int t = r / mt.ng, head = mt.head0 + r - t * mt.ng;
             const long long row = mt.row0 + t;
-            acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            x.acc = make_float4(x.acc.x * inv, x.acc.y * inv, x.acc.z * inv, x.acc.w * inv);
             bool alone = false;
             if (PREFILL) {
-                const bool bad = !(isfinite(acc.x) && isfinite(acc.y) && isfinite(acc.z) && isfinite(acc.w));
+                const bool bad = !(isfinite(x.acc.x) && isfinite(x.acc.y) && isfinite(x.acc.z) && isfinite(x.acc.w));
                 alone = __any_sync(0xffffffffu, bad && lane * 4 < a.d);
             }
             if (alone) {
                 lone_row<T>(a, mt.seq, mt.pos0 + t, head, (int)row);
             } else {
-                if (lane * 4 < a.d) store4(reinterpret_cast<T *>(a.out) + row * a.o_row + head * a.o_head + lane * 4, acc);
-                if (a.lse && lane == 0) a.lse[row * a.heads + head] = l == 0.f ? -INFINITY : (ms + log2f(l)) * kLn2;
+                if (lane * 4 < a.d) store4(reinterpret_cast<T *>(a.out) + row * a.o_row + head * a.o_head + lane * 4, x.acc);
+                if (a.lse && lane == 0)
+                    a.lse[row * a.heads + head] = x.l == 0.f ? -INFINITY : ((x.m == -INFINITY ? 0.f : x.m) + log2f(x.l)) * kLn2;
             }
         }
-        __syncthreads();
     }
+}
+
+// n / d by 32-bit arithmetic where both fit, as they nearly always do.
+MB_DEV long long div64(long long n, long long d)
+{
+    if (((n | d) >> 32) == 0) return (uint32_t)n / (uint32_t)d;
+    return n / d;
 }
 
 // ---- host ------------------------------------------------------------------------------

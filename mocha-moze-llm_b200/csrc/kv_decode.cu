@@ -161,7 +161,7 @@ MB_DEV bool find_share(const Work &w, int hh_n, long long *s_warp, int *s_seq, l
         if (i < warp) incl += s_warp[i];
         total += s_warp[i];
     }
-    *per = max((total + gridDim.x - 1) / gridDim.x, (long long)w.min_tiles);
+    *per = max(div64(total + gridDim.x - 1, gridDim.x), (long long)w.min_tiles);
     *start = *per * blockIdx.x;
     *end = min(*start + *per, total);
     long long at = incl - sum;
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
     Walk in;  // the next tile to load
     in.seq = s_seq;
     in.load(a);
-    in.hh = (int)(s_rem / in.t.n);
+    in.hh = (int)div64(s_rem, in.t.n);
     in.i = (int)(s_rem - (long long)in.hh * in.t.n);
     Walk it = in;  // the tile to compute
     const uint32_t wring = mb::as::smem_u32(ring) + warp * R::kStages * R::kStage;
@@ -562,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
                 Meta mt{};
                 mt.c_end = -1;
                 if (began && !last) {
-                    mt.c_end = (int)((end - 1 + (it.t.n - 1 - it.i)) / per);
+                    mt.c_end = (int)div64(end - 1 + (it.t.n - 1 - it.i), per);
                     mt.row0 = it.seq;
                     mt.ntok = 1;
                     mt.head0 = head0;
@@ -587,7 +587,7 @@ int run(Work &w, int ctas, cudaStream_t s)
     const char *who = "mocha_kv_decode";
     constexpr int smem = Smem<T, DP, NG>::kTotal;
     if (launch(who, k_decode<T, DP, NG>, dim3(ctas), kThreads, smem, s, false, w)) return 1;
-    return launch(who, k_join<T, false>, dim3(ctas, 8 * NG), 32 * kJoinWarps, 0, s, true, w.a, 8 * NG, DP);
+    return launch(who, k_join<T, false>, dim3(2 * mb::kSMs), 32 * kJoinWarps, 0, s, true, w.a, ctas, 8 * NG, DP);
 }
 
 template <typename T, int DP>

@@ -80,7 +80,7 @@ MB_DEV bool find_share(const Args &a, int tokens, int min_tiles, ShareSmem &sm)
         for (int w = 0; w < W; w++) total += sm.warp[w];
         total *= a.kv_heads;
         Share h{};
-        h.per = max((total + gridDim.x - 1) / gridDim.x, (long long)min_tiles);
+        h.per = max(div64(total + gridDim.x - 1, gridDim.x), (long long)min_tiles);
         h.start = h.per * blockIdx.x;
         h.end = min(h.start + h.per, total);
         if (h.start < total) {
@@ -93,7 +93,7 @@ MB_DEV bool find_share(const Args &a, int tokens, int min_tiles, ShareSmem &sm)
             }
             h.seq = s;
             long long rem = h.start - at;
-            h.kvh = (int)(rem / n);
+            h.kvh = (int)div64(rem, n);
             rem -= h.kvh * n;
             Piece p;
             p.load(a, s, tokens);
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kThreads) k_prefill(const __grid_constant__ Ar
             Meta mt{};
             mt.c_end = -1;
             if (first == 0 && !whole) {
-                mt.c_end = (int)((h.end - 1 + (u.t.n - stop)) / h.per);
+                mt.c_end = (int)div64(h.end - 1 + (u.t.n - stop), h.per);
                 mt.row0 = u.p.q0 + tok0;
                 mt.ntok = ntok;
                 mt.head0 = u.kvh * a.group;
@@ -483,6 +483,76 @@ MB_DEV float ex2(float x)
     return y;
 }
 
+// Pairs of fp32 operations in one instruction, each rounded to nearest.
+MB_DEV void fma2(float &d0, float &d1, float a0, float a1, float b0, float b1, float c0, float c1)
+{
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d0), "=f"(d1)
+        : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+MB_DEV void add2(float &d0, float &d1, float a0, float a1)
+{
+    asm("{\n\t.reg .b64 a, d;\n\tmov.b64 d, {%0, %1};\n\tmov.b64 a, {%2, %3};\n\tadd.rn.f32x2 d, d, a;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "+f"(d0), "+f"(d1)
+        : "f"(a0), "f"(a1));
+}
+
+// 2^x of a pair on the FMA units, for x <= 127: with n the integer nearest to x and
+// f = x - n in [-1/2, 1/2], a polynomial for 2^f (least largest relative error: 2^-13.7 of
+// degree 3 where weights are rounded to 2^-9, 2^-18.5 of degree 4 where to 2^-12) and n
+// added to its exponent.  Results below 2^-126 become 0; of NaN something that is not finite
+// once rounded to 16 bits.
+template <typename T>
+MB_DEV void exp2_fma(float &x0, float &x1)
+{
+    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
+    float r0 = kRound, r1 = kRound, f0 = x0, f1 = x1, y0, y1;
+    add2(r0, r1, x0, x1);
+    float t0 = r0, t1 = r1;
+    add2(t0, t1, -kRound, -kRound);
+    add2(f0, f1, -t0, -t1);
+    if constexpr (std::is_same<T, __half>::value) {
+        y0 = y1 = 0.009570102207362652f;
+        fma2(y0, y1, y0, y1, f0, f1, 0.05591785907745361f, 0.05591785907745361f);
+        fma2(y0, y1, y0, y1, f0, f1, 0.240247443318367f, 0.240247443318367f);
+        fma2(y0, y1, y0, y1, f0, f1, 0.6931217908859253f, 0.6931217908859253f);
+        fma2(y0, y1, y0, y1, f0, f1, 0.9999992847442627f, 0.9999992847442627f);
+    } else {
+        y0 = y1 = 0.0551716685295105f;
+        fma2(y0, y1, y0, y1, f0, f1, 0.2426111251115799f, 0.2426111251115799f);
+        fma2(y0, y1, y0, y1, f0, f1, 0.6932609677314758f, 0.6932609677314758f);
+        fma2(y0, y1, y0, y1, f0, f1, 0.9999280571937561f, 0.9999280571937561f);
+    }
+    x0 = x0 < -126.f ? 0.f : __int_as_float(__float_as_int(y0) + (__float_as_int(r0) << 23));
+    x1 = x1 < -126.f ? 0.f : __int_as_float(__float_as_int(y1) + (__float_as_int(r1) << 23));
+}
+
+// The n lowest bits.
+MB_DEV uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; }
+
+// Four lanes with four units of eight words each (their rows' next 128 bytes) exchange them:
+// lane q of the four then holds unit q of the four rows, so that a store writes whole lines.
+MB_DEV void exchange4(uint32_t (&r)[32])
+{
+    const int q = threadIdx.x & 3;
+#pragma unroll
+    for (int step = 1; step <= 2; step <<= 1) {
+        const bool up = q & step;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (u & step) continue;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                uint32_t &lo = r[8 * u + e], &hi = r[8 * (u + step) + e];
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? lo : hi, step);
+                if (up) lo = got;
+                else hi = got;
+            }
+        }
+    }
+}
+
 // c tanh(z / c) = c - 2 c / (1 + exp(2 z / c)).
 MB_DEV float capped(float z, float cap, float k) { return cap - __fdividef(2.f * cap, 1.f + ex2(z * k)); }
 
@@ -499,6 +569,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int tokens = 2 * tok;
     griddep_launch();
+    if (tid == 32) {
+        prefetch_map(&maps.q);
+        prefetch_map(&maps.k);
+        prefetch_map(&maps.v);
+    }
     if (tid == 0) {
         for (int x = 0; x < 2; x++) {
             mbar_init(&bar.q_full[x], 1);
@@ -542,15 +617,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int stop = (int)min((long long)u.t.n, i + left);
             const int pa = u.p.pos(tok0), pb = pa + ntok - 1;
             left -= stop - i;
-            for (int x = 0; x < 2 && x * tok < ntok; x++) {
-                // the tile's queries, once the unit before no longer reads it
-                ok = ok && mbar_wait(&bar.q_empty[x], (asked[x]++ & 1) ^ 1, &bar.abort);
-                if (ok && lane == 0) {
-                    mbar_expect_tx(&bar.q_full[x], (uint32_t)(DP * 2 * tok * a.group));
-                    for (int b = 0; b < DP / 64; b++)
-                        tma_load_4d(sq + x * S::kTile + b * (128 * 128), &maps.q, 64 * b, 0, u.kvh, u.p.q0 + tok0 + x * tok, &bar.q_full[x]);
-                }
-            }
+            const int begin = i;
             for (; i < stop && ok; i++) {
                 const int j0 = u.t.key(i);
                 const int keys = min(kTcKeys, u.p.len - j0);           // keys there are (not positive: none)
@@ -576,6 +643,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                         for (int c = 0; c < DP / 64; c++)
                             tma_load_4d(dst + c * (128 * 128) + b * box * 128, v ? &maps.v : &maps.k, 64 * c, j - (int)(slot * a.page.d), u.kvh, id, full);
+                    }
+                    if (!v && i == begin) {
+                        // the queries, behind the first keys: once the unit before no longer reads its own
+                        for (int x = 0; x < 2 && x * tok < ntok; x++) {
+                            ok = ok && mbar_wait(&bar.q_empty[x], (asked[x]++ & 1) ^ 1, &bar.abort);
+                            if (ok && lane == 0) {
+                                mbar_expect_tx(&bar.q_full[x], (uint32_t)(DP * 2 * tok * a.group));
+                                for (int b = 0; b < DP / 64; b++)
+                                    tma_load_4d(sq + x * S::kTile + b * (128 * 128), &maps.q, 64 * b, 0, u.kvh, u.p.q0 + tok0 + x * tok, &bar.q_full[x]);
+                            }
+                        }
                     }
                     if (v && edge) {
                         // rows past the sequence's end hold anything: 0 * NaN must not reach the sums
@@ -695,26 +773,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     tc_fence_after();
                     const bool full = (j0 + kTcKeys <= min(p0 + 1, u.p.len) && (a.window == 0 || p1 - j0 < a.window)) || j0 + kTcKeys <= u.p.pre;
                     // the scores, 32 columns at a time: once for the maximum, the last 32 kept
-                    // and the others read again for the weights (all 128 do not fit the registers);
-                    // what masks and options change is put back
+                    // and the others read again for the weights (all 128 do not fit the
+                    // registers); what the options change is put back
+                    uint32_t vis[4];  // the row's visible keys
+                    if (EXTRA || !full) {
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            const int j = j0 + 32 * c;
+                            vis[c] = (low_bits(hi - j) & ~low_bits(lo - j)) | low_bits(u.p.pre - j);
+                        }
+                    }
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    auto hide = [&](float (&s)[32], uint32_t bits) {
+#pragma unroll
+                        for (int c = 0; c < 32; c++)
+                            if (!(bits >> c & 1)) s[c] = -INFINITY;
+                    };
                     auto first_look = [&](float (&s)[32], int c0) {
-                        if (EXTRA || !full) {
-                            const unsigned span = hi > lo ? hi - lo : 0;
+                        if (EXTRA) {
 #pragma unroll
                             for (int c = 0; c < 32; c++) {
-                                const int j = j0 + c0 + c;
-                                if (EXTRA) {
-                                    float z = s[c] * a.scale;
-                                    if (a.cap > 0.f) z = capped(z, a.cap, kcap);
-                                    s[c] = fmaf(-slope, fabsf((float)(p - j)), z) * kLog2e;
-                                }
-                                if (!((unsigned)(j - lo) < span || j < u.p.pre)) s[c] = -INFINITY;
+                                float z = s[c] * a.scale;
+                                if (a.cap > 0.f) z = capped(z, a.cap, kcap);
+                                s[c] = fmaf(-slope, fabsf((float)(p - (j0 + c0 + c))), z) * kLog2e;
                             }
-                            if (c0 < 96) tmem_st32<0>(ts + c0, s);
                         }
+                        if (EXTRA || !full) hide(s, vis[c0 / 32]);
+                        if (EXTRA && c0 < 96) tmem_st32<0>(ts + c0, s);
 #pragma unroll
-                        for (int c = 0; c < 32; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+                        for (int c = 0; c < 32; c += 2) mx[(c / 2) & 3] = fmaxf(mx[(c / 2) & 3], fmaxf(s[c], s[c + 1]));
                     };
                     float sa[32], sb[32];
                     tmem_ld32<0>(ts, sa);
@@ -729,7 +816,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     first_look(sa, 64);
                     tmem_wait_ld();
                     first_look(sb, 96);
-                    if (EXTRA || !full) tmem_wait_st();
+                    if (EXTRA) tmem_wait_st();
                     const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                     // a new maximum, and the output so far to its scale
                     float f = 1.f;
@@ -757,13 +844,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const float sub = m == -INFINITY ? 0.f : -m * k2;
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
                     // weights of columns c0.. go to columns 64 + c0 / 2.., which have been read
-                    auto weigh = [&](const float (&s)[32], int c0) {
+                    auto weigh = [&](float (&s)[32], int c0) {
                         uint32_t w[16];
+                        if (!EXTRA && !full && c0 < 96) hide(s, vis[c0 / 32]);
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
-                            const float e0 = ex2(fmaf(s[2 * e], k2, sub)), e1 = ex2(fmaf(s[2 * e + 1], k2, sub));
-                            sum[(2 * e) & 3] += e0;
-                            sum[(2 * e + 1) & 3] += e1;
+                            float e0, e1;
+                            fma2(e0, e1, s[2 * e], s[2 * e + 1], k2, k2, sub, sub);
+                            if (e % 4 == 3) {  // the exponential unit is the narrowest: part of them on the FMA units
+                                exp2_fma<T>(e0, e1);
+                            } else {
+                                e0 = ex2(e0);
+                                e1 = ex2(e1);
+                            }
+                            add2(sum[(2 * e) & 3], sum[(2 * e + 1) & 3], e0, e1);
                             w[e] = pack16<T>(e0, e1);
                         }
                         tmem_st16(ts + 64 + c0 / 2, w);
@@ -796,31 +890,49 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
                 const float ms = m == -INFINITY ? 0.f : m * k2;
                 bool bad = false;
+                // 128 bytes of a row at a time; the four lanes of a quad write their rows' lines together
+                unsigned char *base = whole ? reinterpret_cast<unsigned char *>(a.out) + (row * a.o_row + head * a.o_head) * 2
+                                            : reinterpret_cast<unsigned char *>(part + (size_t)at * DP);
+                const unsigned ours = __ballot_sync(0xffffffffu, mine);
+                auto put = [&](uint32_t (&w)[32], int line) {
+                    exchange4(w);
 #pragma unroll
-                for (int c = 0; c < DP / 32; c++) {
-                    float o[32];
-                    tmem_ld32<0>(to + 32 * c, o);
+                    for (int f = 0; f < 4; f++) {
+                        const int from = (lane & ~3) + f;
+                        unsigned char *dst = reinterpret_cast<unsigned char *>(__shfl_sync(0xffffffffu, (unsigned long long)base, from)) + line * 128 + (lane & 3) * 32;
+                        if ((ours >> from & 1) && (!whole || line * 128 + (lane & 3) * 32 < a.d * 2)) {
+                            *reinterpret_cast<uint4 *>(dst) = make_uint4(w[8 * f], w[8 * f + 1], w[8 * f + 2], w[8 * f + 3]);
+                            *reinterpret_cast<uint4 *>(dst + 16) = make_uint4(w[8 * f + 4], w[8 * f + 5], w[8 * f + 6], w[8 * f + 7]);
+                        }
+                    }
+                };
+#pragma unroll
+                for (int c = 0; c < DP / 64; c++) {
+                    float o[32], o2[32];
+                    tmem_ld32<0>(to + 64 * c, o);
+                    tmem_ld32<0>(to + 64 * c + 32, o2);
                     tmem_wait_ld();
+                    uint32_t w[32];
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
                         o[e] *= inv;
-                        bad |= !isfinite(o[e]);
+                        o2[e] *= inv;
+                        bad |= !isfinite(o[e]) || !isfinite(o2[e]);
                     }
-                    if (mine && !whole) {
+                    if (whole) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<float4 *>(part + (size_t)at * DP + 32 * c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                    } else if (mine && 32 * c < a.d) {
-                        T *dst = reinterpret_cast<T *>(a.out) + row * a.o_row + head * a.o_head + 32 * c;
-#pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            uint4 y;
-                            y.x = pack16<T>(o[e], o[e + 1]);
-                            y.y = pack16<T>(o[e + 2], o[e + 3]);
-                            y.z = pack16<T>(o[e + 4], o[e + 5]);
-                            y.w = pack16<T>(o[e + 6], o[e + 7]);
-                            *reinterpret_cast<uint4 *>(dst + e) = y;
+                        for (int e = 0; e < 16; e++) {
+                            w[e] = pack16<T>(o[2 * e], o[2 * e + 1]);
+                            w[16 + e] = pack16<T>(o2[2 * e], o2[2 * e + 1]);
                         }
+                        put(w, c);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) w[e] = __float_as_uint(o[e]);
+                        put(w, 2 * c);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) w[e] = __float_as_uint(o2[e]);
+                        put(w, 2 * c + 1);
                     }
                 }
                 if (mine) {
@@ -843,7 +955,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 Meta mt{};
                 mt.c_end = -1;
                 if (first == 0 && !whole) {
-                    mt.c_end = (int)((h.end - 1 + (u.t.n - stop)) / h.per);
+                    mt.c_end = (int)div64(h.end - 1 + (u.t.n - stop), h.per);
                     mt.row0 = u.p.q0 + tok0;
                     mt.ntok = ntok;
                     mt.head0 = u.kvh * a.group;
@@ -882,7 +994,7 @@ int run(Args &a, int ctas, cudaStream_t s)
     const char *who = "mocha_kv_prefill";
     const int tokens = kRows / a.group;
     if (launch(who, k_prefill<T, DP>, dim3(ctas), kThreads, Smem32<DP>::kTotal, s, false, a, tokens, 2)) return 1;
-    return launch(who, k_join<T, true>, dim3(ctas, 8), 32 * kJoinWarps, 0, s, true, a, kRows, DP);
+    return launch(who, k_join<T, true>, dim3(4 * mb::kSMs), 32 * kJoinWarps, 0, s, true, a, ctas, kRows, DP);
 }
 
 // ---- tensor maps -----------------------------------------------------------------------
@@ -933,7 +1045,7 @@ int run_tc(Args &a, const mocha_kv_pages *p, cudaStream_t s)
     if (extra ? launch(who, k_prefill_tc<T, DP, true>, dim3(ctas), kTcThreads, SmemTc<DP>::kTotal, s, false, a, maps, tok, box, 4)
               : launch(who, k_prefill_tc<T, DP, false>, dim3(ctas), kTcThreads, SmemTc<DP>::kTotal, s, false, a, maps, tok, box, 4))
         return 1;
-    return launch(who, k_join<T, true>, dim3(ctas, 16), 32 * kJoinWarps, 0, s, true, a, 256, DP);
+    return launch(who, k_join<T, true>, dim3(4 * mb::kSMs), 32 * kJoinWarps, 0, s, true, a, ctas, 256, DP);
 }
 
 }  // namespace
