@@ -153,7 +153,7 @@ MB_DEV void store4(__nv_bfloat16 *p, float4 x)
 // the rows to which a tile's matrix product carried an infinite or NaN value of a key that
 // they do not see (0 * inf).  Rare, so written for size.
 template <typename T>
-__device__ __noinline__ void lone_row(const Args &a, int seq, int p, int head, int row)
+__device__ __forceinline__ void lone_row(const Args &a, int seq, int p, int head, int row)
 {
     const int lane = threadIdx.x & 31, d = a.d, per = d / 32;
     const int len = seq_len(a, seq), pre = seq_prefix(a, seq, len);
@@ -162,8 +162,10 @@ __device__ __noinline__ void lone_row(const Args &a, int seq, int p, int head, i
     const float slope = a.slopes ? a.slopes[head] : 0.f;
     float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
     const int hi = min(p + 1, len), lo = max(a.window ? max(p - a.window + 1, 0) : 0, pre);
+#pragma unroll 1
     for (int part = 0; part < 2; part++) {
         const int j0 = part ? lo : 0, j1 = part ? hi : pre;
+#pragma unroll 1
         for (int jb = j0; jb < j1; jb += 32) {
             const int j = jb + lane;
             float z = -INFINITY;
@@ -174,6 +176,7 @@ __device__ __noinline__ void lone_row(const Args &a, int seq, int p, int head, i
                 if (id >= 0) {
                     at = id * a.ps + kvh * a.hs + (long long)(j - div(a.page, j) * a.page.d) * a.ts;
                     const T *kr = reinterpret_cast<const T *>(a.k) + at;
+#pragma unroll 1
                     for (int i = 0; i < d; i++) dot = fmaf(to_f32(q[i]), to_f32(kr[i]), dot);
                 }
                 z = score2(a, dot, slope, p, j);
@@ -182,18 +185,23 @@ __device__ __noinline__ void lone_row(const Args &a, int seq, int p, int head, i
             const float f = exp2f(m - ms), e = j < j1 ? exp2f(z - ms) : 0.f;
             m = mn;
             l = l * f + mb::warp_sum(e);
-            for (int i = 0; i < per; i++) acc[i] *= f;
+            #pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] *= f;
+#pragma unroll 1
             for (int t = 0; t < min(32, j1 - jb); t++) {
                 const float w = __shfl_sync(0xffffffffu, e, t);
                 const long long vt = __shfl_sync(0xffffffffu, at, t);
                 if (vt >= 0)
-                    for (int i = 0; i < per; i++)
-                        acc[i] = fmaf(w, to_f32(reinterpret_cast<const T *>(a.v)[vt + lane + 32 * i]), acc[i]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (i < per) acc[i] = fmaf(w, to_f32(reinterpret_cast<const T *>(a.v)[vt + lane + 32 * i]), acc[i]);
             }
         }
     }
     T *o = reinterpret_cast<T *>(a.out) + row * a.o_row + head * a.o_head;
-    for (int i = 0; i < per; i++) o[lane + 32 * i] = from_f32<T>(l == 0.f ? 0.f : acc[i] / l);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i < per) o[lane + 32 * i] = from_f32<T>(l == 0.f ? 0.f : acc[i] / l);
     if (a.lse && lane == 0) a.lse[(long long)row * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 

@@ -383,7 +383,8 @@ __global__ void __launch_bounds__(kThreads) k_prefill(const __grid_constant__ Ar
 // The maximum that a row's weights are taken from is renewed only when it is exceeded by
 // 2^8, so outputs are rescaled a few times per row and not per tile; weights then are at
 // most 2^8, sums and outputs stay exact to their type.
-constexpr int kTcThreads = 320;  // warps 0-3 and 4-7: weights of the two tiles; 8: products; 9: copies
+constexpr int kTcThreads = 384;  // warps 0-3 and 4-7: weights of the two tiles; 8: products; 9: copies; 10, 11: none
+constexpr int kTcUnits = 4;      // units that the copies may be ahead
 constexpr int kTcKeys = 128;
 
 struct Maps {
@@ -394,13 +395,27 @@ template <int DP>
 struct SmemTc {
     static constexpr int kTile = 128 * DP * 2;           // bytes of a tile of 128 rows
     static constexpr int kStages = DP == 128 ? 5 : 10;   // key and value tiles in flight
-    static constexpr int kTotal = 1024 + 2 * kTile + kStages * kTile;
+    static constexpr int kTiles = (2 + kStages) * kTile;
+};
+
+// A unit as the warps see it: the copying warp walks along the share and passes units on.
+struct TcUnit {
+    int ntok;           // tokens of the unit; 0 after the last unit
+    int row0, pos0;     // first token's row and position
+    int kvh, seq, len, pre;
+    int pre_t, lo_t;    // tiles, as in Tiles
+    int first, stop, n; // tiles of this share, and of the unit
+    MB_DEV int key(int i) const { return (i < pre_t ? i : i - pre_t + lo_t) * kTcKeys; }
+    MB_DEV bool whole() const { return first == 0 && stop == n; }
 };
 
 struct TcBars {
-    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], kv_full[10], kv_empty[10], edge, drain;
+    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], o_full[2], kv_full[10], kv_empty[10], unit_full[kTcUnits],
+        unit_empty[kTcUnits], edge, drain;
+    TcUnit unit[kTcUnits];
+    Share share;
     uint32_t tmem;
-    volatile int abort;
+    volatile int abort, bad;  // a wait ran out; an output is not finite
 };
 
 MB_DEV void tma_load_4d(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, int c3, uint64_t *bar)
@@ -445,19 +460,22 @@ MB_DEV void tmem_ld32(uint32_t addr, float (&x)[N])
         : KV_O8(x, I), KV_O8(x, I + 8), KV_O8(x, I + 16), KV_O8(x, I + 24)
         : "r"(addr));
 }
-template <int I, int N>
-MB_DEV void tmem_st32(uint32_t addr, const float (&x)[N])
-{
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::KV_F8(x, I),
-        KV_F8(x, I + 8), KV_F8(x, I + 16), KV_F8(x, I + 24), "r"(addr));
-}
 // 16 TMEM columns.
 MB_DEV void tmem_st16(uint32_t addr, const uint32_t (&x)[16])
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::KV_I8(x, 0),
                  KV_I8(x, 8), "r"(addr));
+}
+MB_DEV void tmem_ld16f(uint32_t addr, float (&x)[16])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : KV_O8(x, 0), KV_O8(x, 8)
+                 : "r"(addr));
+}
+MB_DEV void tmem_st16f(uint32_t addr, const float (&x)[16])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::KV_F8(x, 0),
+                 KV_F8(x, 8), "r"(addr));
 }
 MB_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -501,17 +519,19 @@ MB_DEV void add2(float &d0, float &d1, float a0, float a1)
 // 2^x of a pair on the FMA units, for x <= 127: with n the integer nearest to x and
 // f = x - n in [-1/2, 1/2], a polynomial for 2^f (least largest relative error: 2^-13.7 of
 // degree 3 where weights are rounded to 2^-9, 2^-18.5 of degree 4 where to 2^-12) and n
-// added to its exponent.  Results below 2^-126 become 0; of NaN something that is not finite
-// once rounded to 16 bits.
+// added to its exponent.  Results below 2^-126 become 2^-126; of NaN something that is not
+// finite once rounded to 16 bits.
 template <typename T>
 MB_DEV void exp2_fma(float &x0, float &x1)
 {
     constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
-    float r0 = kRound, r1 = kRound, f0 = x0, f1 = x1, y0, y1;
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x0));
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x1));
+    float r0 = kRound, r1 = kRound, f0, f1, y0, y1;
     add2(r0, r1, x0, x1);
     float t0 = r0, t1 = r1;
     add2(t0, t1, -kRound, -kRound);
-    add2(f0, f1, -t0, -t1);
+    fma2(f0, f1, t0, t1, -1.f, -1.f, x0, x1);
     if constexpr (std::is_same<T, __half>::value) {
         y0 = y1 = 0.009570102207362652f;
         fma2(y0, y1, y0, y1, f0, f1, 0.05591785907745361f, 0.05591785907745361f);
@@ -524,9 +544,12 @@ MB_DEV void exp2_fma(float &x0, float &x1)
         fma2(y0, y1, y0, y1, f0, f1, 0.6932609677314758f, 0.6932609677314758f);
         fma2(y0, y1, y0, y1, f0, f1, 0.9999280571937561f, 0.9999280571937561f);
     }
-    x0 = x0 < -126.f ? 0.f : __int_as_float(__float_as_int(y0) + (__float_as_int(r0) << 23));
-    x1 = x1 < -126.f ? 0.f : __int_as_float(__float_as_int(y1) + (__float_as_int(r1) << 23));
+    x0 = __int_as_float(__float_as_int(y0) + (__float_as_int(r0) << 23));
+    x1 = __int_as_float(__float_as_int(y1) + (__float_as_int(r1) << 23));
 }
+
+// Pairs of exponentials on the FMA units: kOnFma of every kMixed.
+constexpr int kMixed = 4, kOnFma = 1;
 
 // The n lowest bits.
 MB_DEV uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; }
@@ -562,9 +585,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 {
     using namespace mb::as;
     using S = SmemTc<DP>;
-    extern __shared__ unsigned char smem_raw[];
-    unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ TcBars bar;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    TcBars &bar = *reinterpret_cast<TcBars *>(smem + S::kTiles);
     ShareSmem &share = *reinterpret_cast<ShareSmem *>(smem);  // before the tiles
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int tokens = 2 * tok;
@@ -579,45 +601,72 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&bar.q_full[x], 1);
             mbar_init(&bar.q_empty[x], 1);
             mbar_init(&bar.s_full[x], 1);
-            mbar_init(&bar.p_full[x], 128);
+            mbar_init(&bar.p_full[x][0], 128);
+            mbar_init(&bar.p_full[x][1], 128);
             mbar_init(&bar.o_full[x], 1);
         }
         for (int i = 0; i < S::kStages; i++) {
             mbar_init(&bar.kv_full[i], 1);
             mbar_init(&bar.kv_empty[i], 1);
         }
+        for (int i = 0; i < kTcUnits; i++) {
+            mbar_init(&bar.unit_full[i], 1);
+            mbar_init(&bar.unit_empty[i], 9);  // eight warps of weights and the thread of products
+        }
         mbar_init(&bar.edge, 1);
         mbar_init(&bar.drain, 1);
-        bar.abort = 0;
+        bar.abort = bar.bad = 0;
         fence_barrier_init();
     }
-    const bool any = find_share<kTcKeys, kTcThreads>(a, tokens, min_tiles, share);
-    if (!any) {
+    // swizzled tiles are laid out by address: their base has to be a multiple of 1024
+    const bool any = find_share<kTcKeys, kTcThreads>(a, tokens, min_tiles, share), placed = (smem_u32(smem) & 1023) == 0;
+    if (!any || !placed) {
+        if (!placed && tid == 0 && a.status) *a.status = 2;
         if (tid == 0) a.meta[blockIdx.x].c_end = -1;
         return;
     }
-    const Share h = share.out;
+    if (tid == 0) bar.share = share.out;
     if (warp == 8) tmem_alloc(&bar.tmem, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = bar.tmem;
     const uint32_t sq = smem_u32(smem), skv = sq + 2 * S::kTile;
-    Units<kTcKeys> u;
-    u.start(a, h, tokens);
-    int i = h.i;
-    long long left = h.end - h.start;
     bool ok = true;
 
+    // 12 warps of 168 registers at launch: 128 threads of 88 and 256 of 208 fit in those
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 9) {
         // copies
-        int it = 0, edges = 0, asked[2] = {0, 0};
-        while (left > 0 && ok) {
-            const int tok0 = u.block * tokens, ntok = min(tokens, u.p.nq - tok0);
-            const int stop = (int)min((long long)u.t.n, i + left);
-            const int pa = u.p.pos(tok0), pb = pa + ntok - 1;
+        Units<kTcKeys> u;
+        u.start(a, bar.share, tokens);
+        int i = bar.share.i, it = 0, edges = 0, units = 0, asked[2] = {0, 0};
+        long long left = bar.share.end - bar.share.start;
+        for (;; units++) {
+            const bool more = left > 0;
+            const int stop = more ? (int)min((long long)u.t.n, i + left) : 0, begin = i;
+            const int tok0 = u.block * tokens, ntok = min(tokens, u.p.nq - tok0), pa = u.p.pos(tok0), pb = pa + ntok - 1;
+            ok = mbar_wait(&bar.unit_empty[units % kTcUnits], ((units / kTcUnits) & 1) ^ 1, &bar.abort);
+            if (!ok) break;
+            if (lane == 0) {
+                TcUnit &d = bar.unit[units % kTcUnits];
+                d.ntok = more ? ntok : 0;
+                d.row0 = u.p.q0 + tok0;
+                d.pos0 = pa;
+                d.kvh = u.kvh;
+                d.seq = u.seq;
+                d.len = u.p.len;
+                d.pre = u.p.pre;
+                d.pre_t = u.t.pre_t;
+                d.lo_t = u.t.lo_t;
+                d.first = i;
+                d.stop = stop;
+                d.n = u.t.n;
+                mbar_arrive(&bar.unit_full[units % kTcUnits]);
+            }
+            if (!more) break;
             left -= stop - i;
-            const int begin = i;
             for (; i < stop && ok; i++) {
                 const int j0 = u.t.key(i);
                 const int keys = min(kTcKeys, u.p.len - j0);           // keys there are (not positive: none)
@@ -670,6 +719,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
             }
+            if (!ok) break;
             if (left > 0) u.next(a, tokens);
             i = 0;
         }
@@ -680,293 +730,248 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
             constexpr uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
             constexpr uint32_t id_qk = base | ((128u >> 3) << 17), id_pv = base | (1u << 16) | ((uint32_t)(DP >> 3) << 17);
-            int it = 0, steps[2] = {0, 0}, units[2] = {0, 0};  // steps: weights taken; units: queries taken
+            int it = 0, steps[2] = {0, 0}, asked[2] = {0, 0};  // steps: weights taken; asked: queries taken
+            auto wait = [&](uint64_t *b, uint32_t parity) {
+                ok = ok && mbar_wait(b, parity, &bar.abort);
+                tc_fence_after();
+                return ok;
+            };
+            auto full = [&](int n) { return wait(&bar.kv_full[n % S::kStages], (n / S::kStages) & 1); };
             auto qk = [&](int x, int st) {
-                const uint32_t q = sq + x * S::kTile, k = skv + st * S::kTile;
+                const uint64_t q = sw128_desc(sq + x * S::kTile), k = sw128_desc(skv + st * S::kTile);
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; kk++) {
-                    const uint32_t off = (kk / 4) * (128 * 128) + (kk % 4) * 32;
-                    mma_bf16(tmem + x * 128, sw128_desc(q + off), sw128_desc(k + off), id_qk, kk > 0);
+                    const uint32_t off = ((kk / 4) * (128 * 128) + (kk % 4) * 32) >> 4;
+                    mma_bf16(tmem + x * 128, q + off, k + off, id_qk, kk > 0);
                 }
                 mma_commit(&bar.s_full[x]);
             };
-            auto pv = [&](int x, int st, bool accumulate) {
-                const uint32_t v = skv + st * S::kTile;
-#pragma unroll
-                for (int kk = 0; kk < 8; kk++)
-                    mma_ts(tmem + 256 + x * 128, tmem + x * 128 + 64 + kk * 8, mn_desc(v + kk * 2048, 128 * 128), id_pv, accumulate || kk > 0);
-                mma_commit(&bar.o_full[x]);
-            };
-            auto full = [&](int n) {
-                ok = ok && mbar_wait(&bar.kv_full[n % S::kStages], (n / S::kStages) & 1, &bar.abort);
-                tc_fence_after();
-            };
-            while (left > 0 && ok) {
-                const int ntok = min(tokens, u.p.nq - u.block * tokens);
-                const int stop = (int)min((long long)u.t.n, i + left), n = stop - i;
-                const int tiles = ntok > tok ? 2 : 1;
-                left -= n;
-                full(it);
-                for (int x = 0; x < tiles && ok; x++) {
-                    ok = mbar_wait(&bar.q_full[x], units[x]++ & 1, &bar.abort);
-                    tc_fence_after();
-                    if (ok) qk(x, it % S::kStages);
+            for (int units = 0; wait(&bar.unit_full[units % kTcUnits], (units / kTcUnits) & 1); units++) {
+                const TcUnit &d = bar.unit[units % kTcUnits];
+                const int n = d.stop - d.first, tiles = d.ntok > tok ? 2 : 1;
+                const bool done = d.ntok == 0;
+                mbar_arrive(&bar.unit_empty[units % kTcUnits]);
+                if (done || !full(it)) break;
+                for (int x = 0; x < tiles && wait(&bar.q_full[x], asked[x]++ & 1); x++) {
+                    qk(x, it % S::kStages);
                     if (n == 1) mma_commit(&bar.q_empty[x]);
                 }
-                if (ok) mma_commit(&bar.kv_empty[it % S::kStages]);
-                for (int j = 0; j < n && ok; j++) {
-                    const int vt = it + 1, kt = it + 2;
-                    for (int x = 0; x < tiles && ok; x++) {
-                        if (x == 0) full(vt);
-                        ok = ok && mbar_wait(&bar.p_full[x], steps[x]++ & 1, &bar.abort);
-                        tc_fence_after();
+                mma_commit(&bar.kv_empty[it % S::kStages]);
+                for (int j = 0; j < n && ok; j++, it += 2) {
+                    const int vt = (it + 1) % S::kStages, kt = (it + 2) % S::kStages;
+                    for (int x = 0; x < tiles; x++) {
+                        // the first 64 keys' weights are used while the others' are made
+                        const uint64_t v = mn_desc(skv + vt * S::kTile, 128 * 128);
+                        const uint32_t step = steps[x]++ & 1;
+                        if (x == 0 && !full(it + 1)) break;
+#pragma unroll
+                        for (int hf = 0; hf < 2; hf++) {
+                            if (!wait(&bar.p_full[x][hf], step)) break;
+#pragma unroll
+                            for (int kk = 4 * hf; kk < 4 * hf + 4; kk++)
+                                mma_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, v + (kk * 2048 >> 4), id_pv, j > 0 || kk > 0);
+                        }
                         if (!ok) break;
-                        pv(x, vt % S::kStages, j > 0);
+                        mma_commit(&bar.o_full[x]);
                         if (j + 1 < n) {
-                            if (x == 0) full(kt);
-                            if (!ok) break;
-                            qk(x, kt % S::kStages);
+                            if (x == 0 && !full(it + 2)) break;
+                            qk(x, kt);
                             if (j + 2 == n) mma_commit(&bar.q_empty[x]);
                         }
                     }
                     if (!ok) break;
-                    mma_commit(&bar.kv_empty[vt % S::kStages]);
-                    if (j + 1 < n) mma_commit(&bar.kv_empty[kt % S::kStages]);
-                    it += 2;
+                    mma_commit(&bar.kv_empty[vt]);
+                    if (j + 1 < n) mma_commit(&bar.kv_empty[kt]);
                 }
-                if (left > 0) u.next(a, tokens);
-                i = 0;
             }
             if (!ok) bar.abort = 1;
             mma_commit(&bar.drain);
             int never = 0;
             mbar_wait(&bar.drain, 0, &never);
         }
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // weights: thread = row of tile x
         const int x = warp >> 2, r = (warp & 3) * 32 + lane;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + x * 128 + lanes, to = tmem + 256 + x * 128 + lanes;
-        const int t = div(a.group_div, r);
-        const float k2 = EXTRA ? 1.f : a.scale * kLog2e, kcap = EXTRA && a.cap > 0.f ? 2.f * kLog2e / a.cap : 0.f;
+        const uint32_t ts = tmem + x * 128 + ((uint32_t)((warp & 3) * 32) << 16), to = ts + 256;
+        const float k2 = EXTRA ? 1.f : a.scale * kLog2e;
         uint32_t step = 0;
-        while (left > 0 && ok) {
-            const int tok0 = u.block * tokens, ntok = min(tokens, u.p.nq - tok0);
-            const int first = i, stop = (int)min((long long)u.t.n, i + left);
-            left -= stop - i;
-            const bool whole = first == 0 && stop == u.t.n;
-            const int pa = u.p.pos(tok0);
-            if (x * tok < ntok) {
-                const int head = u.kvh * a.group + r - t * a.group;
-                const bool mine = t < tok && x * tok + t < ntok;
-                const int p0 = pa + x * tok, p1 = p0 + min(tok, ntok - x * tok) - 1, p = p0 + t;
-                const int hi = min(p + 1, u.p.len), lo = a.window ? max(p - a.window + 1, 0) : 0;
-                const float slope = EXTRA && a.slopes && mine ? __ldg(a.slopes + head) : 0.f;
+        // false when a wait has run out, here or elsewhere in the CTA
+        auto wait = [&](uint64_t *b, uint32_t parity) {
+            ok = __all_sync(0xffffffffu, mbar_wait(b, parity, &bar.abort));
+            tc_fence_after();
+            return ok;
+        };
+        for (int units = 0; wait(&bar.unit_full[units % kTcUnits], (units / kTcUnits) & 1); units++) {
+            const TcUnit &d = bar.unit[units % kTcUnits];
+            if (d.ntok == 0) break;
+            if (x * tok < d.ntok) {
+                const int t = div(a.group_div, r);
                 float m = -INFINITY, l = 0.f;
-                for (; i < stop; i++, step++) {
-                    const int j0 = u.t.key(i);
-                    ok = mbar_wait(&bar.s_full[x], step & 1, &bar.abort);
-                    if (!__all_sync(0xffffffffu, ok)) {
-                        ok = false;
-                        break;
+                {
+                    const int p0 = d.pos0 + x * tok, p1 = p0 + min(tok, d.ntok - x * tok) - 1, p = p0 + t, pre = d.pre;
+                    const int hi = min(p + 1, d.len), lo = a.window ? max(p - a.window + 1, 0) : 0;
+                    const int full_hi = min(p0 + 1, d.len) - kTcKeys, full_lo = a.window ? p1 - a.window + 1 : 0;
+                    const int first = d.first, stop = d.stop;
+                    float slope = 0.f, kcap = 0.f;
+                    if (EXTRA) {
+                        if (a.slopes && t < tok) slope = __ldg(a.slopes + d.kvh * a.group + r - t * a.group);
+                        if (a.cap > 0.f) kcap = 2.f * kLog2e / a.cap;
                     }
-                    tc_fence_after();
-                    const bool full = (j0 + kTcKeys <= min(p0 + 1, u.p.len) && (a.window == 0 || p1 - j0 < a.window)) || j0 + kTcKeys <= u.p.pre;
-                    // the scores, 32 columns at a time: once for the maximum, the last 32 kept
-                    // and the others read again for the weights (all 128 do not fit the
-                    // registers); what the options change is put back
-                    uint32_t vis[4];  // the row's visible keys
-                    if (EXTRA || !full) {
-#pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            const int j = j0 + 32 * c;
-                            vis[c] = (low_bits(hi - j) & ~low_bits(lo - j)) | low_bits(u.p.pre - j);
-                        }
-                    }
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    auto hide = [&](float (&s)[32], uint32_t bits) {
-#pragma unroll
-                        for (int c = 0; c < 32; c++)
-                            if (!(bits >> c & 1)) s[c] = -INFINITY;
-                    };
-                    auto first_look = [&](float (&s)[32], int c0) {
+                    for (int i = first; i < stop; i++, step++) {
+                        const int j0 = d.key(i);
+                        const bool full = (j0 <= full_hi && j0 >= full_lo) || j0 + kTcKeys <= pre;
+                        if (!wait(&bar.s_full[x], step & 1)) break;
+                        float s[128];
+                        tmem_ld32<0>(ts, s);
+                        tmem_ld32<32>(ts + 32, s);
+                        tmem_ld32<64>(ts + 64, s);
+                        tmem_ld32<96>(ts + 96, s);
+                        tmem_wait_ld();
                         if (EXTRA) {
 #pragma unroll
-                            for (int c = 0; c < 32; c++) {
+                            for (int c = 0; c < 128; c++) {
                                 float z = s[c] * a.scale;
                                 if (a.cap > 0.f) z = capped(z, a.cap, kcap);
-                                s[c] = fmaf(-slope, fabsf((float)(p - (j0 + c0 + c))), z) * kLog2e;
+                                s[c] = fmaf(-slope, fabsf((float)(p - (j0 + c))), z) * kLog2e;
                             }
                         }
-                        if (EXTRA || !full) hide(s, vis[c0 / 32]);
-                        if (EXTRA && c0 < 96) tmem_st32<0>(ts + c0, s);
+                        if (!full) {
 #pragma unroll
-                        for (int c = 0; c < 32; c += 2) mx[(c / 2) & 3] = fmaxf(mx[(c / 2) & 3], fmaxf(s[c], s[c + 1]));
-                    };
-                    float sa[32], sb[32];
-                    tmem_ld32<0>(ts, sa);
-                    tmem_wait_ld();
-                    tmem_ld32<0>(ts + 32, sb);
-                    first_look(sa, 0);
-                    tmem_wait_ld();
-                    tmem_ld32<0>(ts + 64, sa);
-                    first_look(sb, 32);
-                    tmem_wait_ld();
-                    tmem_ld32<0>(ts + 96, sb);
-                    first_look(sa, 64);
-                    tmem_wait_ld();
-                    first_look(sb, 96);
-                    if (EXTRA) tmem_wait_st();
-                    const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                    // a new maximum, and the output so far to its scale
-                    float f = 1.f;
-                    if ((mn - m) * k2 > 8.f) {
-                        f = ex2((m - mn) * k2);
-                        m = mn;
-                    }
-                    if (i > first && __any_sync(0xffffffffu, f != 1.f)) {
-                        ok = mbar_wait(&bar.o_full[x], (step & 1) ^ 1, &bar.abort);
-                        if (!__all_sync(0xffffffffu, ok)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
+                            for (int b = 0; b < 4; b++) {
+                                const int j = j0 + 32 * b;
+                                const uint32_t vis = (low_bits(hi - j) & ~low_bits(lo - j)) | low_bits(pre - j);
 #pragma unroll
-                        for (int c = 0; c < DP / 32; c++) {
-                            float o[32];
-                            tmem_ld32<0>(to + 32 * c, o);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 32; e++) o[e] *= f;
-                            tmem_st32<0>(to + 32 * c, o);
-                        }
-                    }
-                    const float sub = m == -INFINITY ? 0.f : -m * k2;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                    // weights of columns c0.. go to columns 64 + c0 / 2.., which have been read
-                    auto weigh = [&](float (&s)[32], int c0) {
-                        uint32_t w[16];
-                        if (!EXTRA && !full && c0 < 96) hide(s, vis[c0 / 32]);
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            float e0, e1;
-                            fma2(e0, e1, s[2 * e], s[2 * e + 1], k2, k2, sub, sub);
-                            if (e % 4 == 3) {  // the exponential unit is the narrowest: part of them on the FMA units
-                                exp2_fma<T>(e0, e1);
-                            } else {
-                                e0 = ex2(e0);
-                                e1 = ex2(e1);
+                                for (int c = 0; c < 32; c++)
+                                    if (!(vis >> c & 1)) s[32 * b + c] = -INFINITY;
                             }
-                            add2(sum[(2 * e) & 3], sum[(2 * e + 1) & 3], e0, e1);
-                            w[e] = pack16<T>(e0, e1);
                         }
-                        tmem_st16(ts + 64 + c0 / 2, w);
-                    };
-                    tmem_ld32<0>(ts + 64, sa);
-                    weigh(sb, 96);
-                    tmem_wait_ld();
-                    tmem_ld32<0>(ts + 32, sb);
-                    weigh(sa, 64);
-                    tmem_wait_ld();
-                    tmem_ld32<0>(ts, sa);
-                    weigh(sb, 32);
-                    tmem_wait_ld();
-                    weigh(sa, 0);
-                    l = fmaf(l, f, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-                    tmem_wait_st();
-                    tc_fence_before();
-                    mbar_arrive(&bar.p_full[x]);
+                        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int c = 0; c < 128; c += 2) mx[(c / 2) & 3] = fmaxf(mx[(c / 2) & 3], fmaxf(s[c], s[c + 1]));
+                        const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                        // a new maximum, and the output so far to its scale
+                        float f = 1.f;
+                        if ((mn - m) * k2 > 8.f) {
+                            f = ex2((m - mn) * k2);
+                            m = mn;
+                        }
+                        if (i > first && __any_sync(0xffffffffu, f != 1.f)) {
+                            if (!wait(&bar.o_full[x], (step & 1) ^ 1)) break;
+#pragma unroll
+                            for (int c = 0; c < DP; c += 16) {
+                                float o[16];
+                                tmem_ld16f(to + c, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 16; e++) o[e] *= f;
+                                tmem_st16f(to + c, o);
+                            }
+                        }
+                        const float sub = m == -INFINITY ? 0.f : -m * k2;
+                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int b = 0; b < 4; b++) {
+                            uint32_t w[16];  // over scores that have been read
+#pragma unroll
+                            for (int e = 0; e < 16; e++) {
+                                float e0, e1;
+                                fma2(e0, e1, s[32 * b + 2 * e], s[32 * b + 2 * e + 1], k2, k2, sub, sub);
+                                if (e % kMixed < kOnFma) {
+                                    exp2_fma<T>(e0, e1);
+                                } else {
+                                    e0 = ex2(e0);
+                                    e1 = ex2(e1);
+                                }
+                                add2(sum[(2 * e) & 3], sum[(2 * e + 1) & 3], e0, e1);
+                                w[e] = pack16<T>(e0, e1);
+                            }
+                            tmem_st16(ts + 16 * b, w);
+                            if (b & 1) {
+                                tmem_wait_st();
+                                tc_fence_before();
+                                mbar_arrive(&bar.p_full[x][b / 2]);
+                            }
+                        }
+                        l = fmaf(l, f, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                    }
                 }
-                if (!ok) break;
-                ok = mbar_wait(&bar.o_full[x], (step & 1) ^ 1, &bar.abort);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const int at = (x * tok + t) * a.group + (r - t * a.group);
-                const long long row = u.p.q0 + tok0 + x * tok + t;
-                float *part = a.part + ((size_t)blockIdx.x * 2 + (first == 0 ? 1 : 0)) * ((size_t)256 * (DP + 2));
-                const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
-                const float ms = m == -INFINITY ? 0.f : m * k2;
+                if (!ok || !wait(&bar.o_full[x], (step & 1) ^ 1)) break;
+                const bool mine = t < tok && x * tok + t < d.ntok, whole = d.whole();
+                const int g = r - t * a.group, head = d.kvh * a.group + g;
+                const int at = (x * tok + t) * a.group + g;
+                const long long row = d.row0 + x * tok + t;
+                float *part = a.part + ((size_t)blockIdx.x * 2 + (d.first == 0 ? 1 : 0)) * ((size_t)256 * (DP + 2));
+                // a row whose maximum is still -infinity has seen nothing (its weights are 2^-126)
+                const float inv = !whole ? 1.f : m == -INFINITY ? 0.f : 1.f / l;
                 bool bad = false;
                 // 128 bytes of a row at a time; the four lanes of a quad write their rows' lines together
                 unsigned char *base = whole ? reinterpret_cast<unsigned char *>(a.out) + (row * a.o_row + head * a.o_head) * 2
                                             : reinterpret_cast<unsigned char *>(part + (size_t)at * DP);
                 const unsigned ours = __ballot_sync(0xffffffffu, mine);
-                auto put = [&](uint32_t (&w)[32], int line) {
+#pragma unroll 1
+                for (int line = 0; line < (whole ? DP / 64 : DP / 32); line++) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        float o[32];
+                        tmem_ld32<0>(to + (whole ? 64 * line + 32 * c : 32 * line), o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            o[e] *= inv;
+                            bad |= !isfinite(o[e]);
+                        }
+                        if (whole) {
+#pragma unroll
+                            for (int e = 0; e < 16; e++) w[16 * c + e] = pack16<T>(o[2 * e], o[2 * e + 1]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; e++) w[e] = __float_as_uint(o[e]);
+                            break;
+                        }
+                    }
                     exchange4(w);
+                    const int byte = line * 128 + (lane & 3) * 32;
 #pragma unroll
                     for (int f = 0; f < 4; f++) {
                         const int from = (lane & ~3) + f;
-                        unsigned char *dst = reinterpret_cast<unsigned char *>(__shfl_sync(0xffffffffu, (unsigned long long)base, from)) + line * 128 + (lane & 3) * 32;
-                        if ((ours >> from & 1) && (!whole || line * 128 + (lane & 3) * 32 < a.d * 2)) {
+                        unsigned char *dst = reinterpret_cast<unsigned char *>(__shfl_sync(0xffffffffu, (unsigned long long)base, from)) + byte;
+                        if ((ours >> from & 1) && (!whole || byte < a.d * 2)) {
                             *reinterpret_cast<uint4 *>(dst) = make_uint4(w[8 * f], w[8 * f + 1], w[8 * f + 2], w[8 * f + 3]);
                             *reinterpret_cast<uint4 *>(dst + 16) = make_uint4(w[8 * f + 4], w[8 * f + 5], w[8 * f + 6], w[8 * f + 7]);
                         }
                     }
-                };
-#pragma unroll
-                for (int c = 0; c < DP / 64; c++) {
-                    float o[32], o2[32];
-                    tmem_ld32<0>(to + 64 * c, o);
-                    tmem_ld32<0>(to + 64 * c + 32, o2);
-                    tmem_wait_ld();
-                    uint32_t w[32];
-#pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        o[e] *= inv;
-                        o2[e] *= inv;
-                        bad |= !isfinite(o[e]) || !isfinite(o2[e]);
-                    }
-                    if (whole) {
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            w[e] = pack16<T>(o[2 * e], o[2 * e + 1]);
-                            w[16 + e] = pack16<T>(o2[2 * e], o2[2 * e + 1]);
-                        }
-                        put(w, c);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; e++) w[e] = __float_as_uint(o[e]);
-                        put(w, 2 * c);
-#pragma unroll
-                        for (int e = 0; e < 32; e++) w[e] = __float_as_uint(o2[e]);
-                        put(w, 2 * c + 1);
-                    }
                 }
                 if (mine) {
                     if (!whole) {
-                        part[(size_t)256 * DP + 2 * at] = m == -INFINITY ? m : ms;
+                        part[(size_t)256 * DP + 2 * at] = m == -INFINITY ? m : m * k2;
                         part[(size_t)256 * DP + 2 * at + 1] = l;
-                    } else if (a.lse)
-                        a.lse[row * a.heads + head] = l == 0.f ? -INFINITY : (ms + log2f(l)) * kLn2;
+                    } else {
+                        if (a.lse) a.lse[row * a.heads + head] = m == -INFINITY ? m : (m * k2 + log2f(l)) * kLn2;
+                        if (bad) bar.bad = 1;
+                    }
                 }
                 tc_fence_before();
-                unsigned again = __ballot_sync(0xffffffffu, mine && whole && bad);
-                while (again) {
-                    const int f = __ffs(again) - 1;
-                    again &= again - 1;
-                    const int fp = __shfl_sync(0xffffffffu, p, f), fh = __shfl_sync(0xffffffffu, head, f), fr = __shfl_sync(0xffffffffu, (int)row, f);
-                    lone_row<T>(a, u.seq, fp, fh, fr);
-                }
             }
-            if (left <= 0 && tid == 0) {
+            if (tid == 0) {
+                // the share's last unit leaves the last note
                 Meta mt{};
                 mt.c_end = -1;
-                if (first == 0 && !whole) {
-                    mt.c_end = (int)div64(h.end - 1 + (u.t.n - stop), h.per);
-                    mt.row0 = u.p.q0 + tok0;
-                    mt.ntok = ntok;
-                    mt.head0 = u.kvh * a.group;
+                if (d.first == 0 && d.stop < d.n) {
+                    mt.c_end = (int)div64(bar.share.end - 1 + (d.n - d.stop), bar.share.per);
+                    mt.row0 = d.row0;
+                    mt.ntok = d.ntok;
+                    mt.head0 = d.kvh * a.group;
                     mt.ng = a.group;
-                    mt.seq = u.seq;
-                    mt.pos0 = pa;
+                    mt.seq = d.seq;
+                    mt.pos0 = d.pos0;
                 }
                 a.meta[blockIdx.x] = mt;
             }
-            if (left > 0) u.next(a, tokens);
-            i = 0;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.unit_empty[units % kTcUnits]);
         }
         if (!ok) bar.abort = 1;
     }
@@ -985,6 +990,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (warp == 8) {
         tc_fence_after();
         tmem_free(tmem, 512);
+    }
+    if (!bar.bad || bar.abort) return;
+    // rows of whole units that are not finite, once more without the keys that they do not see
+    Units<kTcKeys> u;
+    u.start(a, bar.share, tokens);
+    int i = bar.share.i;
+    for (long long left = bar.share.end - bar.share.start; left > 0; i = 0) {
+        const int tok0 = u.block * tokens, ntok = min(tokens, u.p.nq - tok0);
+        if (i == 0 && left >= u.t.n)
+            for (int r = warp; r < ntok * a.group; r += kTcThreads / 32) {
+                const int t = div(a.group_div, r), head = u.kvh * a.group + r - t * a.group, row = u.p.q0 + tok0 + t;
+                const T *o = reinterpret_cast<const T *>(a.out) + row * a.o_row + head * a.o_head;
+                bool bad = false;
+                for (int e = lane; e < a.d; e += 32) bad |= !isfinite(to_f32(o[e]));
+                if (__any_sync(0xffffffffu, bad)) lone_row<T>(a, u.seq, u.p.pos(tok0 + t), head, row);
+            }
+        left -= u.t.n - i;
+        if (left > 0) u.next(a, tokens);
     }
 }
 
@@ -1042,8 +1065,8 @@ int run_tc(Args &a, const mocha_kv_pages *p, cudaStream_t s)
         return fail(who, "the tensor maps cannot be encoded");
     const bool extra = a.cap > 0.f || a.slopes || !(a.scale > 0.f);
     const int ctas = mb::kSMs;
-    if (extra ? launch(who, k_prefill_tc<T, DP, true>, dim3(ctas), kTcThreads, SmemTc<DP>::kTotal, s, false, a, maps, tok, box, 4)
-              : launch(who, k_prefill_tc<T, DP, false>, dim3(ctas), kTcThreads, SmemTc<DP>::kTotal, s, false, a, maps, tok, box, 4))
+    if (extra ? launch(who, k_prefill_tc<T, DP, true>, dim3(ctas), kTcThreads, SmemTc<DP>::kTiles + sizeof(TcBars), s, false, a, maps, tok, box, 4)
+              : launch(who, k_prefill_tc<T, DP, false>, dim3(ctas), kTcThreads, SmemTc<DP>::kTiles + sizeof(TcBars), s, false, a, maps, tok, box, 4))
         return 1;
     return launch(who, k_join<T, true>, dim3(4 * mb::kSMs), 32 * kJoinWarps, 0, s, true, a, ctas, 256, DP);
 }
