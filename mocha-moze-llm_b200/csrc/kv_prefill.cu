@@ -446,6 +446,13 @@ MB_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, bool 
         : "memory");
 }
 
+MB_DEV bool elect_one()
+{
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 #define KV_O8(x, i) "=f"(x[i]), "=f"(x[i + 1]), "=f"(x[i + 2]), "=f"(x[i + 3]), "=f"(x[i + 4]), "=f"(x[i + 5]), "=f"(x[i + 6]), "=f"(x[i + 7])
 #define KV_F8(x, i) "f"(x[i]), "f"(x[i + 1]), "f"(x[i + 2]), "f"(x[i + 3]), "f"(x[i + 4]), "f"(x[i + 5]), "f"(x[i + 6]), "f"(x[i + 7])
 #define KV_I8(x, i) "r"(x[i]), "r"(x[i + 1]), "r"(x[i + 2]), "r"(x[i + 3]), "r"(x[i + 4]), "r"(x[i + 5]), "r"(x[i + 6]), "r"(x[i + 7])
@@ -725,70 +732,77 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (!ok) bar.abort = 1;
     } else if (warp == 8) {
-        if (lane == 0) {
-            // products
-            constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
-            constexpr uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
-            constexpr uint32_t id_qk = base | ((128u >> 3) << 17), id_pv = base | (1u << 16) | ((uint32_t)(DP >> 3) << 17);
-            int it = 0, steps[2] = {0, 0}, asked[2] = {0, 0};  // steps: weights taken; asked: queries taken
-            auto wait = [&](uint64_t *b, uint32_t parity) {
-                ok = ok && mbar_wait(b, parity, &bar.abort);
-                tc_fence_after();
-                return ok;
-            };
-            auto full = [&](int n) { return wait(&bar.kv_full[n % S::kStages], (n / S::kStages) & 1); };
-            auto qk = [&](int x, int st) {
-                const uint64_t q = sw128_desc(sq + x * S::kTile), k = sw128_desc(skv + st * S::kTile);
+        // products: the warp goes along together, one elected lane issues
+        constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
+        constexpr uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
+        constexpr uint32_t id_qk = base | ((128u >> 3) << 17), id_pv = base | (1u << 16) | ((uint32_t)(DP >> 3) << 17);
+        int it = 0, steps[2] = {0, 0}, asked[2] = {0, 0};  // steps: weights taken; asked: queries taken
+        auto wait = [&](uint64_t *b, uint32_t parity) {
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(b, parity, &bar.abort));
+            tc_fence_after();
+            return ok;
+        };
+        auto full = [&](int n) { return wait(&bar.kv_full[n % S::kStages], (n / S::kStages) & 1); };
+        auto qk = [&](int x, int st, bool last) {
+            const uint64_t q = sw128_desc(sq + x * S::kTile), k = sw128_desc(skv + st * S::kTile);
+            if (elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; kk++) {
                     const uint32_t off = ((kk / 4) * (128 * 128) + (kk % 4) * 32) >> 4;
                     mma_bf16(tmem + x * 128, q + off, k + off, id_qk, kk > 0);
                 }
                 mma_commit(&bar.s_full[x]);
-            };
-            for (int units = 0; wait(&bar.unit_full[units % kTcUnits], (units / kTcUnits) & 1); units++) {
-                const TcUnit &d = bar.unit[units % kTcUnits];
-                const int n = d.stop - d.first, tiles = d.ntok > tok ? 2 : 1;
-                const bool done = d.ntok == 0;
-                mbar_arrive(&bar.unit_empty[units % kTcUnits]);
-                if (done || !full(it)) break;
-                for (int x = 0; x < tiles && wait(&bar.q_full[x], asked[x]++ & 1); x++) {
-                    qk(x, it % S::kStages);
-                    if (n == 1) mma_commit(&bar.q_empty[x]);
-                }
-                mma_commit(&bar.kv_empty[it % S::kStages]);
-                for (int j = 0; j < n && ok; j++, it += 2) {
-                    const int vt = (it + 1) % S::kStages, kt = (it + 2) % S::kStages;
-                    for (int x = 0; x < tiles; x++) {
-                        // the first 64 keys' weights are used while the others' are made
-                        const uint64_t v = mn_desc(skv + vt * S::kTile, 128 * 128);
-                        const uint32_t step = steps[x]++ & 1;
-                        if (x == 0 && !full(it + 1)) break;
+                if (last) mma_commit(&bar.q_empty[x]);
+            }
+            __syncwarp();
+        };
+        for (int units = 0; wait(&bar.unit_full[units % kTcUnits], (units / kTcUnits) & 1); units++) {
+            const TcUnit &d = bar.unit[units % kTcUnits];
+            const int n = d.stop - d.first, tiles = d.ntok > tok ? 2 : 1;
+            const bool done = d.ntok == 0;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.unit_empty[units % kTcUnits]);
+            if (done || !full(it)) break;
+            for (int x = 0; x < tiles && wait(&bar.q_full[x], asked[x]++ & 1); x++) qk(x, it % S::kStages, n == 1);
+            if (elect_one()) mma_commit(&bar.kv_empty[it % S::kStages]);
+            for (int j = 0; j < n && ok; j++, it += 2) {
+                const int vt = (it + 1) % S::kStages, kt = (it + 2) % S::kStages;
 #pragma unroll
-                        for (int hf = 0; hf < 2; hf++) {
-                            if (!wait(&bar.p_full[x][hf], step)) break;
+                for (int x = 0; x < 2; x++) {
+                    if (x == tiles) break;
+                    // the first 64 keys' weights are used while the others' are made
+                    const uint64_t v = mn_desc(skv + vt * S::kTile, 128 * 128);
+                    const uint32_t step = steps[x]++ & 1;
+                    if (x == 0 && !full(it + 1)) break;
+#pragma unroll
+                    for (int hf = 0; hf < 2; hf++) {
+                        if (!wait(&bar.p_full[x][hf], step)) break;
+                        if (elect_one()) {
 #pragma unroll
                             for (int kk = 4 * hf; kk < 4 * hf + 4; kk++)
                                 mma_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, v + (kk * 2048 >> 4), id_pv, j > 0 || kk > 0);
+                            if (hf) mma_commit(&bar.o_full[x]);
                         }
-                        if (!ok) break;
-                        mma_commit(&bar.o_full[x]);
-                        if (j + 1 < n) {
-                            if (x == 0 && !full(it + 2)) break;
-                            qk(x, kt);
-                            if (j + 2 == n) mma_commit(&bar.q_empty[x]);
-                        }
+                        __syncwarp();
                     }
                     if (!ok) break;
+                    if (j + 1 < n) {
+                        if (x == 0 && !full(it + 2)) break;
+                        qk(x, kt, j + 2 == n);
+                    }
+                }
+                if (!ok) break;
+                if (elect_one()) {
                     mma_commit(&bar.kv_empty[vt]);
                     if (j + 1 < n) mma_commit(&bar.kv_empty[kt]);
                 }
+                __syncwarp();
             }
-            if (!ok) bar.abort = 1;
-            mma_commit(&bar.drain);
-            int never = 0;
-            mbar_wait(&bar.drain, 0, &never);
         }
+        if (!ok) bar.abort = 1;
+        if (elect_one()) mma_commit(&bar.drain);
+        int never = 0;
+        mbar_wait(&bar.drain, 0, &never);
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
