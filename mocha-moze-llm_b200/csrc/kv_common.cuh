@@ -126,6 +126,18 @@ MB_DEV float score2(const Args &a, float dot, float slope, int p, int j)
     return z * kLog2e;
 }
 
+// 2^x by the hardware's exponential (2 ulp and subnormal results as zero, far below what
+// rounding a weight to 16 bits costs).
+MB_DEV float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// c tanh(z / c) = c - 2 c / (1 + exp(2 z / c)), k = 2 log2(e) / c.
+MB_DEV float capped(float z, float cap, float k) { return cap - __fdividef(2.f * cap, 1.f + ex2(z * k)); }
+
 template <typename T>
 MB_DEV float to_f32(T x)
 {

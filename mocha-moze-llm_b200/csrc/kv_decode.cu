@@ -2,18 +2,22 @@
 //
 // Each cached value is used by heads / kv heads queries only (4 flops per element and
 // head), so the kernel is bound by reading the visible keys and values once.  A unit is a
-// sequence and one kv head with up to 8 NG of its query heads; its key tiles of 64 are
-// shared out over the CTAs (kv_common.cuh).  The four warps of a CTA take 16 keys each of
-// every tile and run on their own: each keeps a ring of tiles in flight in its own part of
-// shared memory (16-byte asynchronous copies, which also fill the rows of keys that are
-// not visible with zeros, so nothing of them can reach a sum), an online softmax and an
+// sequence and one kv head with up to 8 NG of its query heads; its key tiles are shared out
+// over the CTAs (kv_common.cuh).  The four warps of a CTA take a quarter of every tile's
+// keys each and run on their own: each keeps a ring of tiles in flight in its own part of
+// shared memory (16-byte asynchronous copies, which also fill the rows of keys that are not
+// visible with zeros, so nothing of them can reach a sum), and softmax statistics and an
 // output in registers; they meet when a unit ends.
 //
-// 16-bit types: scores are K q^T and outputs V^T p^T by m16n8k16 products, so the eight
-// (or 16, 32) heads of the group are the narrow side and no lane computes on padding when
-// a group has 8 heads.  The weights are rounded to the cache's type for the second
-// product; their sum is taken before that, in fp32.  fp32: the same tiles on the FMA
-// units, a lane holding half a key's products with 8 heads.
+// 16-bit types: scores are K q^T and outputs V^T p^T by m16n8k16 products, so the heads of
+// the group are the narrow side of 8 and no lane computes on padding when a group has 8.
+// The weights are rounded to the cache's type for the second product; their sum is taken
+// before that, in fp32.  fp32: the same tiles on the FMA units, a lane holding half a key's
+// products with 8 heads.  Either way the value that weights are taken from is renewed only
+// when a score passes it by 2^8, which a vote finds: no shuffles and no rescaling on most
+// tiles.
+#include <type_traits>
+
 #include "kv_common.cuh"
 
 namespace {
@@ -21,28 +25,26 @@ namespace {
 using namespace kv;
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kKeys = 16;              // keys of a warp's tile
-constexpr int kTile = kKeys * kWarps;  // keys of a CTA's tile
 
-// CTAs of an SM, and the stages of a warp's ring (keys then values): 192 KB of rings per
-// SM.  Two CTAs overlap one's unit ends with the other's tiles; wide groups (registers) and
-// fp32 rows of 128 (three stages at least) leave room for one.
+// CTAs of an SM, keys of a warp's tile, and the stages of its ring (keys then values): 192
+// KB of rings per SM, 8 KB (fp32: 8 or 16 KB) a stage, so that two or more stages per warp
+// are in flight, which covers the memory's latency, while one is computed.  Two CTAs overlap
+// one's unit ends with the other's tiles; wide groups (registers) and fp32 rows of 128
+// leave room for one.
 template <typename T, int DP, int NG>
 struct Ring {
+    static constexpr bool kF32 = sizeof(T) == 4;
+    static constexpr int kKeys = DP == 64 && !kF32 ? 32 : 16, kTile = kWarps * kKeys;
     static constexpr int kHalf = kKeys * DP * (int)sizeof(T), kStage = 2 * kHalf;
-    static constexpr int kCtas = NG > 1 || (sizeof(T) == 4 && DP == 128) ? 1 : 2;
+    static constexpr int kCtas = NG > 1 || (kF32 && DP == 128) ? 1 : 2;
     static constexpr int kStages = 192 * 1024 / kCtas / kWarps / kStage;
-};
-
-template <typename T, int DP, int NG>
-struct Smem {
+    static constexpr int kRings = kWarps * kStages * kStage;
     static constexpr int kPad = DP + 4;  // floats of a head's row in the merge buffers
-    static constexpr int kQ = 8 * NG * DP * (int)sizeof(T);
-    static constexpr int kRing = kWarps * Ring<T, DP, NG>::kStages * Ring<T, DP, NG>::kStage;
-    static constexpr int kMerge = 3 * 8 * kPad * 4;
-    static constexpr int kStat = 2 * kWarps * 8 * NG * 2 * 4;  // two buffers of (m, l)
-    static constexpr int kW = sizeof(T) == 4 ? kWarps * 8 * kKeys * 4 : 0;
-    static constexpr int kTotal = kRing + 2 * kQ + kMerge + kStat + kW;
+    static constexpr int kMerge = kWarps * 8 * kPad * 4;
+    static constexpr int kStat = kWarps * 8 * NG * 8;              // (m, l)
+    static constexpr int kQ = kF32 ? 8 * DP * 4 : 0;               // fp32: the unit's queries,
+    static constexpr int kW = kF32 ? kWarps * 8 * kKeys * 4 : 0;  // and a tile's weights
+    static constexpr int kTotal = kRings + kMerge + kStat + kQ + kW;
 };
 
 struct Work {
@@ -52,10 +54,11 @@ struct Work {
 };
 
 // A walk along a CTA's tiles.
+template <int TILE>
 struct Walk {
     int seq, hh, i;
     int len, pre;
-    Tiles<kTile> t;
+    Tiles<TILE> t;
     MB_DEV void load(const Args &a)
     {
         len = pre = 0;
@@ -74,11 +77,16 @@ struct Walk {
         seq++;
         load(a);
     }
+    MB_DEV int low(const Args &a) const { return a.window ? max(len - a.window, 0) : 0; }
 };
 
 MB_DEV void cp_async16(uint32_t dst, const void *src, bool ok)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+MB_DEV void cp_async16(uint32_t dst, const void *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 MB_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -111,7 +119,7 @@ MB_DEV uint32_t transpose8(uint32_t x)
 template <typename T>
 MB_DEV void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
+    if constexpr (std::is_same<T, __half>::value)
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -135,13 +143,14 @@ MB_DEV uint32_t pack2(float x, float y)
 
 // The share of this CTA: its first tile as (sequence, tile within the sequence) in *s_seq
 // and *s_rem, and [start, end) in tiles of the whole call.
+template <int TILE>
 MB_DEV bool find_share(const Work &w, int hh_n, long long *s_warp, int *s_seq, long long *s_rem, long long *start,
                        long long *end, long long *per)
 {
     const Args &a = w.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int chunk = (a.seqs + kThreads - 1) / kThreads, b0 = min(tid * chunk, a.seqs), b1 = min(b0 + chunk, a.seqs);
-    Walk k;
+    Walk<TILE> k;
     long long sum = 0;
     for (k.seq = b0; k.seq < b1; k.seq++) {
         k.load(a);
@@ -182,17 +191,19 @@ MB_DEV bool find_share(const Work &w, int hh_n, long long *s_warp, int *s_seq, l
 template <typename T, int DP, int NG>
 __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(const __grid_constant__ Work w)
 {
-    constexpr bool F32 = sizeof(T) == 4;
     using R = Ring<T, DP, NG>;
-    using S = Smem<T, DP, NG>;
-    constexpr int CH = DP * (int)sizeof(T) / 16;  // 16-byte pieces of a row
-    constexpr int H = 8 * NG;
+    constexpr bool F32 = R::kF32;
+    constexpr int KEYS = R::kKeys, H = 8 * NG;
+    constexpr int CH = DP * (int)sizeof(T) / 16;     // 16-byte pieces of a row
+    constexpr int RPI = 32 / CH, X = KEYS / RPI;     // rows of a warp's copy, copies of a half stage
+    constexpr int GROUPS = KEYS / 8;                 // of 8 keys, which lie in one page
+    constexpr int ROW = DP * (int)sizeof(T);
+    constexpr int NM = F32 ? 8 : 2 * NG, NACC = F32 ? 8 : NG * DP / 16;
     extern __shared__ __align__(128) unsigned char smem[];
-    unsigned char *ring = smem;
-    unsigned char *sq = smem + S::kRing;
-    float *merge = reinterpret_cast<float *>(sq + 2 * S::kQ);
-    float *stat = merge + S::kMerge / 4;
-    float *sw = stat + S::kStat / 4;
+    float *merge = reinterpret_cast<float *>(smem + R::kRings);
+    float2 *stat = reinterpret_cast<float2 *>(smem + R::kRings + R::kMerge);
+    float *sq = reinterpret_cast<float *>(smem + R::kRings + R::kMerge + R::kStat);
+    float *sw = sq + R::kQ / 4;
     __shared__ long long s_warp[kWarps], s_rem;
     __shared__ int s_seq;
     const Args &a = w.a;
@@ -200,92 +211,130 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
     const int hh_n = a.kv_heads * w.hgroups;
     mb::as::griddep_launch();
     long long start, end, per;
-    if (!find_share(w, hh_n, s_warp, &s_seq, &s_rem, &start, &end, &per)) {
+    if (!find_share<R::kTile>(w, hh_n, s_warp, &s_seq, &s_rem, &start, &end, &per)) {
         if (tid == 0) a.meta[blockIdx.x].c_end = -1;
         return;
     }
-    Walk in;  // the next tile to load
+    Walk<R::kTile> in;  // the next tile to load
     in.seq = s_seq;
     in.load(a);
     in.hh = (int)div64(s_rem, in.t.n);
     in.i = (int)(s_rem - (long long)in.hh * in.t.n);
-    Walk it = in;  // the tile to compute
-    const uint32_t wring = mb::as::smem_u32(ring) + warp * R::kStages * R::kStage;
+    Walk<R::kTile> it = in;  // the tile to compute
+    const uint32_t wring = mb::as::smem_u32(smem) + warp * R::kStages * R::kStage;
 
-    int pg[2];  // pages of the two halves of this warp's keys of tile `in`
-    auto pages = [&]() {
-        const int j = in.t.key(in.i) + warp * kKeys;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int jh = j + 8 * h;
-            pg[h] = jh < in.len ? __ldg(a.table + in.seq * a.table_stride + div(a.page, jh)) : 0;
-        }
+    // a lane copies piece `c` of rows r0, r0 + RPI, ...; pieces of a row are spread by its
+    // number so that eight rows' equal pieces lie in different banks
+    const int r0 = lane / CH, c = lane % CH;
+    const bool dims = c * 16 < a.d * (int)sizeof(T);
+    const long long lane_off = (r0 * a.ts + c * (16 / (int)sizeof(T))) * (long long)sizeof(T), row_step = RPI * a.ts * (long long)sizeof(T);
+    const uint32_t lane_row = r0 * ROW, lane_piece = (c ^ r0) * 16;
+
+    // page of group `lane` of this warp's keys of tile `in`
+    int page = 0;
+    auto look_up = [&]() {
+        const int j = in.t.key(in.i) + warp * KEYS + 8 * (lane % GROUPS);
+        page = j < in.len ? __ldg(a.table + in.seq * a.table_stride + div(a.page, j)) : 0;
     };
     auto issue = [&](int slot) {
-        const int j = in.t.key(in.i) + warp * kKeys;
+        const int j = in.t.key(in.i) + warp * KEYS;
         const int kvh = w.hgroups == 1 ? in.hh : in.hh / w.hgroups;
-        const int p = in.len - 1;
-        const uint32_t dst = wring + slot * R::kStage;
-        long long off[2];
-        bool ok[2];
+        const int p = in.len - 1, lo = in.low(a);
+        const uint32_t dst = wring + slot * R::kStage + lane_row;
+        const bool good = (unsigned)page < (unsigned)a.pages;
+        const bool full = j + KEYS <= in.len && (j >= lo || j + KEYS <= in.pre) && __all_sync(0xffffffffu, good);
+        const int jg = j + 8 * (lane % GROUPS);
+        const long long mine = (good ? page * a.ps + (jg - (int)(div(a.page, jg) * a.page.d)) * a.ts : 0) + kvh * a.hs;
+        if (full) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int jh = j + 8 * h;
-            const int row = jh - (int)(div(a.page, jh) * a.page.d);
-            ok[h] = jh < in.len && (unsigned)pg[h] < (unsigned)a.pages;
-            if (jh < in.len && !ok[h] && a.status &&
-                (visible(jh, p, in.len, in.pre, a.window) || visible(min(jh + 7, p), p, in.len, in.pre, a.window)))
+            for (int g = 0; g < GROUPS; g++) {
+                long long off = __shfl_sync(0xffffffffu, mine, g) * (long long)sizeof(T) + lane_off;
+#pragma unroll
+                for (int y = 0; y < 8 / RPI; y++, off += row_step) {
+                    const uint32_t to = dst + (8 * g + RPI * y) * ROW + (lane_piece ^ ((RPI * y) & 7) * 16);
+                    if (dims) {
+                        cp_async16(to, a.k + off);
+                        cp_async16(to + R::kHalf, a.v + off);
+                    } else {
+                        cp_async16(to, a.k, false);
+                        cp_async16(to + R::kHalf, a.v, false);
+                    }
+                }
+            }
+        } else {
+            if (!good && jg < in.len && a.status &&
+                (visible(jg, p, in.len, in.pre, a.window) || visible(min(jg + 7, p), p, in.len, in.pre, a.window)))
                 *a.status = 1;
-            off[h] = ok[h] ? pg[h] * a.ps + kvh * a.hs + row * a.ts : 0;
-        }
 #pragma unroll
-        for (int x = 0; x < kKeys * CH / 32; x++) {
-            const int r = (lane + 32 * x) / CH, c = (lane + 32 * x) % CH;
-            const bool use = ok[r / 8] && c * 16 < a.d * (int)sizeof(T) && visible(j + r, p, in.len, in.pre, a.window);
-            const long long e = use ? off[r / 8] + (r & 7) * a.ts + c * (16 / (int)sizeof(T)) : 0;
-            const uint32_t to = dst + r * DP * (int)sizeof(T) + ((c ^ (r & 7)) * 16);
-            cp_async16(to, a.k + e * (long long)sizeof(T), use);
-            cp_async16(to + R::kHalf, a.v + e * (long long)sizeof(T), use);
+            for (int x = 0; x < X; x++) {
+                const int g = RPI * x / 8, r = r0 + RPI * x;
+                const bool use = __shfl_sync(0xffffffffu, (int)good, g) && dims && visible(j + r, p, in.len, in.pre, a.window);
+                const long long off = __shfl_sync(0xffffffffu, mine, g) * (long long)sizeof(T) + lane_off + (RPI * x % 8 / RPI) * row_step;
+                const uint32_t to = dst + RPI * x * ROW + (lane_piece ^ ((RPI * x) & 7) * 16);
+                cp_async16(to, a.k + (use ? off : 0), use);
+                cp_async16(to + R::kHalf, a.v + (use ? off : 0), use);
+            }
         }
     };
 
     const int tiles = (int)(end - start);
-    pages();
+    look_up();
 #pragma unroll
     for (int x = 0; x < R::kStages - 1; x++) {
         if (x < tiles) {
             issue(x);
             in.next(a, hh_n);
-            pages();
+            look_up();
         }
         cp_commit();
     }
 
+    // the unit's heads and queries: 16-bit, the products' narrow operand in registers
+    int head0 = 0, ng = 0;
+    uint32_t q[F32 ? 1 : NG][F32 ? 1 : DP / 16][2];
+    auto queries = [&]() {
+        const int kvh = w.hgroups == 1 ? it.hh : it.hh / w.hgroups, hg = it.hh - kvh * w.hgroups;
+        head0 = kvh * a.group + hg * w.unit_heads;
+        ng = min(w.unit_heads, a.group - hg * w.unit_heads);
+        if constexpr (!F32) {
+#pragma unroll
+            for (int n = 0; n < NG; n++) {
+                const int h = n * 8 + (lane >> 2);
+                const T *row = reinterpret_cast<const T *>(a.q) + it.seq * a.q_row + (head0 + h) * a.q_head + 2 * (lane & 3);
+#pragma unroll
+                for (int k = 0; k < DP / 16; k++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        q[n][k][e] = h < ng && 16 * k < a.d ? __ldg(reinterpret_cast<const uint32_t *>(row + 16 * k + 8 * e)) : 0;
+            }
+        }
+    };
+    queries();
+
+    const float k2 = a.scale * kLog2e, kcap = a.cap > 0.f ? 2.f * kLog2e / a.cap : 0.f;
+    const bool extra = a.cap > 0.f || a.slopes;
+    const uint32_t k_lane = (lane & 15) * ROW, k_piece = ((lane >> 4) ^ (lane & 7)) * 16;
+    const uint32_t v_lane = ((lane & 7) + ((lane >> 4) << 3)) * ROW, v_piece = (((lane >> 3) & 1) ^ (lane & 7)) * 16;
     bool began = it.i == 0;  // the unit's first tile lies in this share
     bool fresh = true;
-    int buf = 0, head0 = 0, ng = 0, kvh = 0;
-    float m[F32 ? 8 : 2 * NG], l[F32 ? 8 : 2 * NG];
-    float acc[F32 ? 8 : NG * DP / 16][4];
+    float m[NM], l[NM];  // value that weights are taken from (log2), sums of this lane's weights
+    float acc[NACC][4];
     for (int x = 0; x < tiles; x++) {
         if (fresh) {
-            // the unit's queries, one buffer per other unit: the last unit's may still be read
-            kvh = w.hgroups == 1 ? it.hh : it.hh / w.hgroups;
-            const int hg = it.hh - kvh * w.hgroups;
-            head0 = kvh * a.group + hg * w.unit_heads;
-            ng = min(w.unit_heads, a.group - hg * w.unit_heads);
-            unsigned char *q = sq + buf * S::kQ;
-            for (int e = tid; e < H * CH; e += kThreads) {
-                const int h = e / CH, c = e % CH;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (h < ng && c * 16 < a.d * (int)sizeof(T))
-                    v = *reinterpret_cast<const uint4 *>(a.q + (it.seq * a.q_row + (head0 + h) * a.q_head) * (long long)sizeof(T) + c * 16);
-                *reinterpret_cast<uint4 *>(q + h * DP * sizeof(T) + (F32 ? c : c ^ (h & 7)) * 16) = v;
+            if constexpr (F32) {
+                // the last unit's queries are no longer read: its end was met
+                for (int e = tid; e < 8 * CH; e += kThreads) {
+                    const int h = e / CH, cc = e % CH;
+                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (h < ng && cc * 4 < a.d) y = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + it.seq * a.q_row + (head0 + h) * a.q_head + cc * 4);
+                    *reinterpret_cast<float4 *>(sq + h * DP + cc * 4) = y;
+                }
+                __syncthreads();
             }
-            __syncthreads();
 #pragma unroll
-            for (int i = 0; i < (F32 ? 8 : 2 * NG); i++) m[i] = -INFINITY, l[i] = 0.f;
+            for (int i = 0; i < NM; i++) m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < (F32 ? 8 : NG * DP / 16); i++)
+            for (int i = 0; i < NACC; i++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[i][e] = 0.f;
             fresh = false;
@@ -295,133 +344,165 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
         if (x + R::kStages - 1 < tiles) {
             issue((x + R::kStages - 1) % R::kStages);
             in.next(a, hh_n);
-            pages();
+            look_up();
         }
         cp_commit();
-        const int j = it.t.key(it.i) + warp * kKeys, p = it.len - 1;
+        const int j = it.t.key(it.i) + warp * KEYS, p = it.len - 1;
         const uint32_t kb = wring + (x % R::kStages) * R::kStage, vb = kb + R::kHalf;
+        const bool full = j + KEYS <= it.len && (j >= it.low(a) || j + KEYS <= it.pre);
         if constexpr (!F32) {
-            float s[NG][4];
+            constexpr int MT = KEYS / 16;
+            float s[MT][NG][4];
 #pragma unroll
-            for (int n = 0; n < NG; n++)
+            for (int t = 0; t < MT; t++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[n][e] = 0.f;
-            const uint32_t qb = mb::as::smem_u32(sq + buf * S::kQ);
+                for (int n = 0; n < NG; n++)
 #pragma unroll
-            for (int kk = 0; kk < DP / 32; kk++) {
-                uint32_t k0[4], k1[4];
-                const int r = lane & 15, c = 4 * kk + (lane >> 4);
-                ldsm4(kb + r * DP * 2 + ((c ^ (r & 7)) * 16), k0);
-                ldsm4(kb + r * DP * 2 + (((c + 2) ^ (r & 7)) * 16), k1);
+                    for (int e = 0; e < 4; e++) s[t][n][e] = 0.f;
 #pragma unroll
-                for (int n = 0; n < NG; n++) {
-                    uint32_t q[4];
-                    const int h = lane & 7;
-                    ldsm4(qb + (n * 8 + h) * DP * 2 + (((4 * kk + (lane >> 3)) ^ h) * 16), q);
-                    mma<T>(s[n], k0, q[0], q[1]);
-                    mma<T>(s[n], k1, q[2], q[3]);
+            for (int k = 0; k < DP / 16; k++)
+#pragma unroll
+                for (int t = 0; t < MT; t++) {
+                    uint32_t kf[4];
+                    ldsm4(kb + t * 16 * ROW + k_lane + (k_piece ^ k * 32), kf);
+#pragma unroll
+                    for (int n = 0; n < NG; n++) mma<T>(s[t][n], kf, q[n][k][0], q[n][k][1]);
                 }
-            }
-            const int ja = j + (lane >> 2), jb = ja + 8;
-            const bool va = visible(ja, p, it.len, it.pre, a.window), vb_ = visible(jb, p, it.len, it.pre, a.window);
-            uint32_t pt[NG][2];
+            // scores in log2; element e of tile t: key 16 t + lane / 4 (+ 8 for e > 1), head 2 (lane % 4) + e % 2
 #pragma unroll
-            for (int n = 0; n < NG; n++) {
-                if (a.cap > 0.f || a.slopes) {
+            for (int t = 0; t < MT; t++)
+#pragma unroll
+                for (int n = 0; n < NG; n++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const int h = n * 8 + 2 * (lane & 3) + (e & 1);
-                        const float slope = a.slopes && h < ng ? __ldg(a.slopes + head0 + h) : 0.f;
-                        s[n][e] = score2(a, s[n][e], slope, p, e < 2 ? ja : jb);
+                        const int jj = j + 16 * t + (lane >> 2) + (e >> 1) * 8;
+                        float z = s[t][n][e];
+                        if (extra) {
+                            const int h = n * 8 + 2 * (lane & 3) + (e & 1);
+                            z *= a.scale;
+                            if (a.cap > 0.f) z = capped(z, a.cap, kcap);
+                            if (a.slopes && h < ng) z -= __ldg(a.slopes + head0 + h) * (float)(p - jj);
+                            z *= kLog2e;
+                        } else
+                            z *= k2;
+                        if (!full && !visible(jj, p, it.len, it.pre, a.window)) z = -INFINITY;
+                        s[t][n][e] = z;
                     }
-                } else {
+            bool past = false;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) s[n][e] *= a.scale * kLog2e;
-                }
+            for (int t = 0; t < MT; t++)
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (!(e < 2 ? va : vb_)) s[n][e] = -INFINITY;
+                for (int n = 0; n < NG; n++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    float mx = fmaxf(s[n][e], s[n][e + 2]);
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    const float mn = fmaxf(m[2 * n + e], mx), ms = mn == -INFINITY ? 0.f : mn;
-                    const float f = exp2f(m[2 * n + e] - ms);
-                    m[2 * n + e] = mn;
-                    s[n][e] = exp2f(s[n][e] - ms);
-                    s[n][e + 2] = exp2f(s[n][e + 2] - ms);
-                    l[2 * n + e] = fmaf(l[2 * n + e], f, s[n][e] + s[n][e + 2]);
+                    for (int e = 0; e < 4; e++) past |= s[t][n][e] > m[2 * n + (e & 1)] + 8.f;
+            if (__any_sync(0xffffffffu, past)) {
 #pragma unroll
-                    for (int dd = 0; dd < DP / 16; dd++) {
-                        acc[n * (DP / 16) + dd][e] *= f;
-                        acc[n * (DP / 16) + dd][e + 2] *= f;
+                for (int n = 0; n < NG; n++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float mx = m[2 * n + e];
+#pragma unroll
+                        for (int t = 0; t < MT; t++) mx = fmaxf(mx, fmaxf(s[t][n][e], s[t][n][e + 2]));
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        const float f = mx == -INFINITY ? 1.f : ex2(m[2 * n + e] - mx);
+                        m[2 * n + e] = mx;
+                        l[2 * n + e] *= f;
+#pragma unroll
+                        for (int d = 0; d < DP / 16; d++) {
+                            acc[n * (DP / 16) + d][e] *= f;
+                            acc[n * (DP / 16) + d][e + 2] *= f;
+                        }
                     }
+            }
+            uint32_t pt[MT][NG][2];
+#pragma unroll
+            for (int n = 0; n < NG; n++) {
+                const float m0 = m[2 * n] == -INFINITY ? 0.f : m[2 * n], m1 = m[2 * n + 1] == -INFINITY ? 0.f : m[2 * n + 1];
+#pragma unroll
+                for (int t = 0; t < MT; t++) {
+                    float(&z)[4] = s[t][n];
+                    z[0] = ex2(z[0] - m0);
+                    z[1] = ex2(z[1] - m1);
+                    z[2] = ex2(z[2] - m0);
+                    z[3] = ex2(z[3] - m1);
+                    l[2 * n] += z[0] + z[2];
+                    l[2 * n + 1] += z[1] + z[3];
+                    pt[t][n][0] = transpose8(pack2<T>(z[0], z[1]));
+                    pt[t][n][1] = transpose8(pack2<T>(z[2], z[3]));
                 }
-                pt[n][0] = transpose8(pack2<T>(s[n][0], s[n][1]));
-                pt[n][1] = transpose8(pack2<T>(s[n][2], s[n][3]));
             }
 #pragma unroll
-            for (int dd = 0; dd < DP / 16; dd++) {
-                uint32_t v[4];
-                const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * dd + ((lane >> 3) & 1);
-                ldsm4_t(vb + r * DP * 2 + ((c ^ (r & 7)) * 16), v);
+            for (int d = 0; d < DP / 16; d++)
 #pragma unroll
-                for (int n = 0; n < NG; n++) mma<T>(acc[n * (DP / 16) + dd], v, pt[n][0], pt[n][1]);
-            }
+                for (int t = 0; t < MT; t++) {
+                    uint32_t vf[4];
+                    ldsm4_t(vb + t * 16 * ROW + v_lane + (v_piece ^ d * 32), vf);
+#pragma unroll
+                    for (int n = 0; n < NG; n++) mma<T>(acc[n * (DP / 16) + d], vf, pt[t][n][0], pt[t][n][1]);
+                }
         } else {
             // scores: lane = key (16) x half of the dims, 8 heads each
             const int r = lane & 15, half = lane >> 4;
             float s[8];
 #pragma unroll
             for (int h = 0; h < 8; h++) s[h] = 0.f;
-            const float *q = reinterpret_cast<const float *>(sq + buf * S::kQ);
-            const float *kr = reinterpret_cast<const float *>(ring + warp * R::kStages * R::kStage + (x % R::kStages) * R::kStage);
+            const float *kr = reinterpret_cast<const float *>(smem + warp * R::kStages * R::kStage + (x % R::kStages) * R::kStage);
 #pragma unroll 4
-            for (int c = 0; c < CH / 2; c++) {
-                const int cc = half * (CH / 2) + c;
+            for (int i = 0; i < CH / 2; i++) {
+                const int cc = half * (CH / 2) + i;
                 const float4 kx = *reinterpret_cast<const float4 *>(kr + r * DP + ((cc ^ (r & 7)) * 4));
 #pragma unroll
                 for (int h = 0; h < 8; h++) {
-                    const float4 qx = *reinterpret_cast<const float4 *>(q + h * DP + cc * 4);
+                    const float4 qx = *reinterpret_cast<const float4 *>(sq + h * DP + cc * 4);
                     s[h] = fmaf(kx.x, qx.x, s[h]);
                     s[h] = fmaf(kx.y, qx.y, s[h]);
                     s[h] = fmaf(kx.z, qx.z, s[h]);
                     s[h] = fmaf(kx.w, qx.w, s[h]);
                 }
             }
-            const bool see = visible(j + r, p, it.len, it.pre, a.window);
-            float *wt = sw + warp * 8 * kKeys;
+            const bool see = full || visible(j + r, p, it.len, it.pre, a.window);
+            float *wt = sw + warp * 8 * KEYS;
+            bool past = false;
 #pragma unroll
             for (int h = 0; h < 8; h++) {
                 s[h] += __shfl_xor_sync(0xffffffffu, s[h], 16);
                 const float slope = a.slopes && h < ng ? __ldg(a.slopes + head0 + h) : 0.f;
-                const float z = see ? score2(a, s[h], slope, p, j + r) : -INFINITY;
-                const float mn = fmaxf(m[h], mb::warp_max(z)), ms = mn == -INFINITY ? 0.f : mn;
-                const float f = exp2f(m[h] - ms), e = exp2f(z - ms);
-                m[h] = mn;
-                l[h] = fmaf(l[h], f, e);  // every key counts in two lanes
+                s[h] = !see ? -INFINITY : extra ? score2(a, s[h], slope, p, j + r) : s[h] * a.scale * kLog2e;
+                past |= s[h] > m[h] + 8.f;
+            }
+            if (__any_sync(0xffffffffu, past)) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[h][i] *= f;
-                if (!half) wt[h * kKeys + r] = e;
+                for (int h = 0; h < 8; h++) {
+                    const float mx = fmaxf(m[h], mb::warp_max(s[h])), f = mx == -INFINITY ? 1.f : exp2f(m[h] - mx);
+                    m[h] = mx;
+                    l[h] *= f;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[h][i] *= f;
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 8; h++) {
+                const float e = exp2f(s[h] - (m[h] == -INFINITY ? 0.f : m[h]));
+                l[h] += e;  // every key counts in two lanes
+                if (!half) wt[h * KEYS + r] = e;
             }
             __syncwarp();
             // outputs: a lane holds 4 dims; with 64 dims the half-warps take 8 keys each
             const float *vr = kr + R::kHalf / 4;
-            constexpr int KK = DP == 128 ? kKeys : kKeys / 2;
-            const int c = DP == 128 ? lane : lane & 15, k0 = DP == 128 ? 0 : half * KK;
+            constexpr int KK = DP == 128 ? KEYS : KEYS / 2;
+            const int cv = DP == 128 ? lane : lane & 15, k0 = DP == 128 ? 0 : half * KK;
 #pragma unroll
             for (int g = 0; g < KK / 4; g++) {
                 float4 v[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int row = k0 + 4 * g + i;
-                    v[i] = *reinterpret_cast<const float4 *>(vr + row * DP + ((c ^ (row & 7)) * 4));
+                    v[i] = *reinterpret_cast<const float4 *>(vr + row * DP + ((cv ^ (row & 7)) * 4));
                 }
 #pragma unroll
                 for (int h = 0; h < 8; h++) {
-                    const float4 e = *reinterpret_cast<const float4 *>(wt + h * kKeys + k0 + 4 * g);
+                    const float4 e = *reinterpret_cast<const float4 *>(wt + h * KEYS + k0 + 4 * g);
                     const float ew[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
@@ -437,19 +518,18 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
 
         const bool last = it.i == it.t.n - 1;
         if (last || x == tiles - 1) {
+            const int seq = it.seq, h0 = head0, hn = ng, rest = it.t.n - 1 - it.i;
+            const bool whole = began && last, noted = began && !last;
+            it.next(a, hh_n);
+            if (x + 1 < tiles) queries();  // the next unit's, on their way while this one ends
             // the four warps' (m, l, output) into one, in the order of the warps
-            float *st = stat + buf * kWarps * H * 2;
             if constexpr (!F32) {
 #pragma unroll
-                for (int i = 0; i < 2 * NG; i++) {
+                for (int i = 0; i < NM; i++) {
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 4);
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 8);
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 16);
-                    if (lane < 4) {
-                        const int h = (i / 2) * 8 + 2 * lane + (i & 1);
-                        st[(warp * H + h) * 2] = m[i];
-                        st[(warp * H + h) * 2 + 1] = l[i];
-                    }
+                    if (lane < 4) stat[warp * H + (i / 2) * 8 + 2 * lane + (i & 1)] = make_float2(m[i], l[i]);
                 }
             } else {
 #pragma unroll
@@ -459,124 +539,78 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
 #pragma unroll
                         for (int i = 0; i < 4; i++) acc[h][i] += __shfl_xor_sync(0xffffffffu, acc[h][i], 16);
                     }
-                    if (lane == h) {
-                        st[(warp * H + h) * 2] = m[h];
-                        st[(warp * H + h) * 2 + 1] = l[h];
-                    }
+                    if (lane == h) stat[warp * H + h] = make_float2(m[h], l[h]);
                 }
             }
-            __syncthreads();
-            auto joined = [&](int h, float *M, float *L) {
-                *M = -INFINITY;
-                *L = 0.f;
-#pragma unroll
-                for (int i = 0; i < kWarps; i++) *M = fmaxf(*M, st[(i * H + h) * 2]);
-#pragma unroll
-                for (int i = 0; i < kWarps; i++)
-                    *L = fmaf(st[(i * H + h) * 2 + 1], exp2f(st[(i * H + h) * 2] - (*M == -INFINITY ? 0.f : *M)), *L);
-            };
-            const bool whole = began && last;
             float *part = a.part + ((size_t)blockIdx.x * 2 + (began ? 1 : 0)) * ((size_t)H * (DP + 2));
+            float *mine = merge + warp * 8 * R::kPad;
 #pragma unroll
             for (int n = 0; n < NG; n++) {
-                float *mine = merge + (warp ? warp - 1 : 0) * 8 * S::kPad;
                 if constexpr (!F32) {
-                    float f[2];
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float M, L;
-                        joined(n * 8 + 2 * (lane & 3) + e, &M, &L);
-                        f[e] = exp2f(m[2 * n + e] - (M == -INFINITY ? 0.f : M));
-                    }
+                    for (int d = 0; d < DP / 16; d++)
 #pragma unroll
-                    for (int dd = 0; dd < DP / 16; dd++)
+                        for (int e = 0; e < 4; e++)
+                            mine[(2 * (lane & 3) + (e & 1)) * R::kPad + d * 16 + (lane >> 2) + (e >> 1) * 8] = acc[n * (DP / 16) + d][e];
+                } else if (lane * 4 < DP) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            float &y = acc[n * (DP / 16) + dd][e];
-                            y *= f[e & 1];
-                            if (warp) mine[(2 * (lane & 3) + (e & 1)) * S::kPad + dd * 16 + (lane >> 2) + (e >> 1) * 8] = y;
-                        }
-                } else {
-#pragma unroll
-                    for (int h = 0; h < 8; h++) {
-                        float M, L;
-                        joined(h, &M, &L);
-                        const float f = exp2f(m[h] - (M == -INFINITY ? 0.f : M));
-#pragma unroll
-                        for (int i = 0; i < 4; i++) acc[h][i] *= f;
-                        if (warp && lane * 4 < DP)
-                            *reinterpret_cast<float4 *>(mine + h * S::kPad + lane * 4) = make_float4(acc[h][0], acc[h][1], acc[h][2], acc[h][3]);
-                    }
-                }
-                __syncthreads();
-                if (warp == 0) {
-                    if constexpr (!F32) {
-#pragma unroll
-                        for (int dd = 0; dd < DP / 16; dd++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const int at = (2 * (lane & 3) + (e & 1)) * S::kPad + dd * 16 + (lane >> 2) + (e >> 1) * 8;
-                                float y = acc[n * (DP / 16) + dd][e];
-#pragma unroll
-                                for (int i = 0; i < 3; i++) y += merge[i * 8 * S::kPad + at];
-                                merge[at] = y;
-                            }
-                    } else if (lane * 4 < DP) {
-#pragma unroll
-                        for (int h = 0; h < 8; h++) {
-                            float4 y = make_float4(acc[h][0], acc[h][1], acc[h][2], acc[h][3]);
-#pragma unroll
-                            for (int i = 0; i < 3; i++) {
-                                const float4 z = *reinterpret_cast<const float4 *>(merge + (i * 8 + h) * S::kPad + lane * 4);
-                                y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
-                            }
-                            *reinterpret_cast<float4 *>(merge + h * S::kPad + lane * 4) = y;
-                        }
-                    }
+                    for (int h = 0; h < 8; h++)
+                        *reinterpret_cast<float4 *>(mine + h * R::kPad + lane * 4) = make_float4(acc[h][0], acc[h][1], acc[h][2], acc[h][3]);
                 }
                 __syncthreads();
                 for (int e = tid; e < 8 * (DP / 4); e += kThreads) {
-                    const int hl = e / (DP / 4), c = e % (DP / 4), h = n * 8 + hl;
-                    if (h >= ng) break;
-                    float4 y = *reinterpret_cast<const float4 *>(merge + hl * S::kPad + c * 4);
-                    float M, L;
-                    joined(h, &M, &L);
+                    const int hl = e / (DP / 4), cc = e % (DP / 4), h = n * 8 + hl;
+                    if (h >= hn) break;
+                    float M = -INFINITY, L = 0.f;
+                    float2 ml[kWarps];
+#pragma unroll
+                    for (int i = 0; i < kWarps; i++) {
+                        ml[i] = stat[i * H + h];
+                        M = fmaxf(M, ml[i].x);
+                    }
+                    const float ms = M == -INFINITY ? 0.f : M;
+                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int i = 0; i < kWarps; i++) {
+                        const float f = exp2f(ml[i].x - ms);
+                        const float4 z = *reinterpret_cast<const float4 *>(merge + (i * 8 + hl) * R::kPad + cc * 4);
+                        L = fmaf(ml[i].y, f, L);
+                        y.x = fmaf(z.x, f, y.x);
+                        y.y = fmaf(z.y, f, y.y);
+                        y.z = fmaf(z.z, f, y.z);
+                        y.w = fmaf(z.w, f, y.w);
+                    }
                     if (whole) {
                         const float inv = L == 0.f ? 0.f : 1.f / L;
-                        if (c * 4 < a.d)
-                            store4(reinterpret_cast<T *>(a.out) + it.seq * a.o_row + (head0 + h) * a.o_head + c * 4,
+                        if (cc * 4 < a.d)
+                            store4(reinterpret_cast<T *>(a.out) + seq * a.o_row + (h0 + h) * a.o_head + cc * 4,
                                    make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
-                        if (a.lse && c == 0)
-                            a.lse[(long long)it.seq * a.heads + head0 + h] = L == 0.f ? -INFINITY : ((M == -INFINITY ? 0.f : M) + log2f(L)) * kLn2;
+                        if (a.lse && cc == 0) a.lse[(long long)seq * a.heads + h0 + h] = L == 0.f ? -INFINITY : (ms + log2f(L)) * kLn2;
                     } else {
-                        *reinterpret_cast<float4 *>(part + (size_t)h * DP + c * 4) = y;
-                        if (c == 0) {
-                            part[(size_t)H * DP + 2 * h] = M;
-                            part[(size_t)H * DP + 2 * h + 1] = L;
-                        }
+                        *reinterpret_cast<float4 *>(part + (size_t)h * DP + cc * 4) = y;
+                        if (cc == 0) *reinterpret_cast<float2 *>(part + (size_t)H * DP + 2 * h) = make_float2(M, L);
                     }
                 }
-                if (n + 1 < NG) __syncthreads();  // the merge buffers are written again
+                __syncthreads();  // the buffers are written again
             }
             if (x == tiles - 1 && tid == 0) {
                 Meta mt{};
                 mt.c_end = -1;
-                if (began && !last) {
-                    mt.c_end = (int)div64(end - 1 + (it.t.n - 1 - it.i), per);
-                    mt.row0 = it.seq;
+                if (noted) {
+                    mt.c_end = (int)div64(end - 1 + rest, per);
+                    mt.row0 = seq;
                     mt.ntok = 1;
-                    mt.head0 = head0;
-                    mt.ng = ng;
-                    mt.seq = it.seq;
+                    mt.head0 = h0;
+                    mt.ng = hn;
+                    mt.seq = seq;
                     mt.pos0 = p;
                 }
                 a.meta[blockIdx.x] = mt;
             }
             began = true;
             fresh = true;
-            buf ^= 1;
-        }
-        it.next(a, hh_n);
+        } else
+            it.next(a, hh_n);
     }
     cp_wait<0>();
 }
@@ -585,8 +619,7 @@ template <typename T, int DP, int NG>
 int run(Work &w, int ctas, cudaStream_t s)
 {
     const char *who = "mocha_kv_decode";
-    constexpr int smem = Smem<T, DP, NG>::kTotal;
-    if (launch(who, k_decode<T, DP, NG>, dim3(ctas), kThreads, smem, s, false, w)) return 1;
+    if (launch(who, k_decode<T, DP, NG>, dim3(ctas), kThreads, Ring<T, DP, NG>::kTotal, s, false, w)) return 1;
     return launch(who, k_join<T, false>, dim3(2 * mb::kSMs), 32 * kJoinWarps, 0, s, true, w.a, ctas, 8 * NG, DP);
 }
 

@@ -499,15 +499,6 @@ MB_DEV uint32_t pack16(float x, float y)
     }
 }
 
-// 2^x by the hardware's exponential (2 ulp and subnormal results as zero, far below what
-// rounding a weight to 16 bits costs).
-MB_DEV float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // Pairs of fp32 operations in one instruction, each rounded to nearest.
 MB_DEV void fma2(float &d0, float &d1, float a0, float a1, float b0, float b1, float c0, float c1)
 {
@@ -582,9 +573,6 @@ MB_DEV void exchange4(uint32_t (&r)[32])
         }
     }
 }
-
-// c tanh(z / c) = c - 2 c / (1 + exp(2 z / c)).
-MB_DEV float capped(float z, float cap, float k) { return cap - __fdividef(2.f * cap, 1.f + ex2(z * k)); }
 
 template <typename T, int DP, bool EXTRA>
 __global__ void __launch_bounds__(kTcThreads, 1)
