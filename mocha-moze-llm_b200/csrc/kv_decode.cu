@@ -51,13 +51,14 @@ struct Work {
     Args a;
     int hgroups, unit_heads;  // units per kv head, and query heads of a unit (the last may have fewer)
     int min_tiles;            // of a share
+    bool one_page;            // a warp's keys of a tile lie in one page
 };
 
-// A walk along a CTA's tiles.
+// A walk along a CTA's tiles; j is the tile's first key.
 template <int TILE>
 struct Walk {
-    int seq, hh, i;
-    int len, pre;
+    int seq, hh, i, j;
+    int len, pre, lo;  // lo: first key of the window
     Tiles<TILE> t;
     MB_DEV void load(const Args &a)
     {
@@ -66,18 +67,30 @@ struct Walk {
             len = seq_len(a, seq);
             pre = seq_prefix(a, seq, len);
         }
+        lo = a.window ? max(len - a.window, 0) : 0;
         t.set(a, len, pre, len - 1, len - 1);
+    }
+    MB_DEV void at(int tile)
+    {
+        i = tile;
+        j = t.key(tile);
     }
     MB_DEV void next(const Args &a, int hh_n)
     {
-        if (++i < t.n) return;
-        i = 0;
-        if (++hh < hh_n) return;
-        hh = 0;
-        seq++;
-        load(a);
+        if (++i < t.n) {
+            j = i == t.pre_t ? t.lo_t * TILE : j + TILE;
+            return;
+        }
+        if (++hh == hh_n) {
+            hh = 0;
+            seq++;
+            load(a);
+        }
+        at(0);
     }
-    MB_DEV int low(const Args &a) const { return a.window ? max(len - a.window, 0) : 0; }
+    // whether all of n keys from k on are visible; whether key k is
+    MB_DEV bool all_visible(int k, int n) const { return k + n <= len && (k >= lo || k + n <= pre); }
+    MB_DEV bool sees(int k) const { return k < len && (k >= lo || k < pre); }
 };
 
 MB_DEV void cp_async16(uint32_t dst, const void *src, bool ok)
@@ -195,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
     constexpr bool F32 = R::kF32;
     constexpr int KEYS = R::kKeys, H = 8 * NG;
     constexpr int CH = DP * (int)sizeof(T) / 16;     // 16-byte pieces of a row
-    constexpr int RPI = 32 / CH, X = KEYS / RPI;     // rows of a warp's copy, copies of a half stage
+    constexpr int RPI = 32 / CH;                     // rows of a warp's copy
     constexpr int GROUPS = KEYS / 8;                 // of 8 keys, which lie in one page
     constexpr int ROW = DP * (int)sizeof(T);
     constexpr int NM = F32 ? 8 : 2 * NG, NACC = F32 ? 8 : NG * DP / 16;
@@ -219,60 +232,61 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
     in.seq = s_seq;
     in.load(a);
     in.hh = (int)div64(s_rem, in.t.n);
-    in.i = (int)(s_rem - (long long)in.hh * in.t.n);
+    in.at((int)(s_rem - (long long)in.hh * in.t.n));
     Walk<R::kTile> it = in;  // the tile to compute
     const uint32_t wring = mb::as::smem_u32(smem) + warp * R::kStages * R::kStage;
 
-    // a lane copies piece `c` of rows r0, r0 + RPI, ...; pieces of a row are spread by its
+    // a lane copies piece c of rows r0, r0 + RPI, ...; pieces of a row are spread by its
     // number so that eight rows' equal pieces lie in different banks
     const int r0 = lane / CH, c = lane % CH;
     const bool dims = c * 16 < a.d * (int)sizeof(T);
-    const long long lane_off = (r0 * a.ts + c * (16 / (int)sizeof(T))) * (long long)sizeof(T), row_step = RPI * a.ts * (long long)sizeof(T);
-    const uint32_t lane_row = r0 * ROW, lane_piece = (c ^ r0) * 16;
+    const char *k_lane0 = a.k + (r0 * a.ts + c * (16 / (int)sizeof(T))) * (long long)sizeof(T);
+    const long long row_step = RPI * a.ts * (long long)sizeof(T), v_off = a.v - a.k;
+    uint32_t to_lane[8 / RPI];
+#pragma unroll
+    for (int y = 0; y < 8 / RPI; y++) to_lane[y] = wring + (r0 + RPI * y) * ROW + ((c ^ r0 ^ (RPI * y)) & (CH - 1)) * 16;
 
-    // page of group `lane` of this warp's keys of tile `in`
-    int page = 0;
+    // pages of the groups of this warp's keys of tile `in`; one when pages hold whole tiles
+    int pages[GROUPS];
     auto look_up = [&]() {
-        const int j = in.t.key(in.i) + warp * KEYS + 8 * (lane % GROUPS);
-        page = j < in.len ? __ldg(a.table + in.seq * a.table_stride + div(a.page, j)) : 0;
+        const int j = in.j + warp * KEYS;
+        const int *row = a.table + in.seq * a.table_stride;
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++)
+            if (g == 0 || !w.one_page) pages[g] = j + 8 * g < in.len ? __ldg(row + div(a.page, j + 8 * g)) : 0;
     };
-    auto issue = [&](int slot) {
-        const int j = in.t.key(in.i) + warp * KEYS;
+    auto issue = [&](uint32_t slot) {
+        const int j = in.j + warp * KEYS;
         const int kvh = w.hgroups == 1 ? in.hh : in.hh / w.hgroups;
-        const int p = in.len - 1, lo = in.low(a);
-        const uint32_t dst = wring + slot * R::kStage + lane_row;
-        const bool good = (unsigned)page < (unsigned)a.pages;
-        const bool full = j + KEYS <= in.len && (j >= lo || j + KEYS <= in.pre) && __all_sync(0xffffffffu, good);
-        const int jg = j + 8 * (lane % GROUPS);
-        const long long mine = (good ? page * a.ps + (jg - (int)(div(a.page, jg) * a.page.d)) * a.ts : 0) + kvh * a.hs;
-        if (full) {
+        const bool full = in.all_visible(j, KEYS);
+        long long head = kvh * a.hs;
+        const char *from = nullptr;
 #pragma unroll
-            for (int g = 0; g < GROUPS; g++) {
-                long long off = __shfl_sync(0xffffffffu, mine, g) * (long long)sizeof(T) + lane_off;
-#pragma unroll
-                for (int y = 0; y < 8 / RPI; y++, off += row_step) {
-                    const uint32_t to = dst + (8 * g + RPI * y) * ROW + (lane_piece ^ ((RPI * y) & 7) * 16);
-                    if (dims) {
-                        cp_async16(to, a.k + off);
-                        cp_async16(to + R::kHalf, a.v + off);
-                    } else {
-                        cp_async16(to, a.k, false);
-                        cp_async16(to + R::kHalf, a.v, false);
-                    }
-                }
+        for (int g = 0; g < GROUPS; g++) {
+            const int jg = j + 8 * g;
+            bool good = true;
+            if (g == 0 || !w.one_page) {
+                const int id = pages[g];
+                good = (unsigned)id < (unsigned)a.pages;
+                const int row = jg - (int)(div(a.page, jg) * a.page.d);
+                from = k_lane0 + (id * a.ps + head + row * a.ts) * (long long)sizeof(T);
             }
-        } else {
-            if (!good && jg < in.len && a.status &&
-                (visible(jg, p, in.len, in.pre, a.window) || visible(min(jg + 7, p), p, in.len, in.pre, a.window)))
-                *a.status = 1;
+            if (w.one_page) good = (unsigned)pages[0] < (unsigned)a.pages;
+            const uint32_t group = slot + g * 8 * ROW;
+            if (full && good && dims) {
 #pragma unroll
-            for (int x = 0; x < X; x++) {
-                const int g = RPI * x / 8, r = r0 + RPI * x;
-                const bool use = __shfl_sync(0xffffffffu, (int)good, g) && dims && visible(j + r, p, in.len, in.pre, a.window);
-                const long long off = __shfl_sync(0xffffffffu, mine, g) * (long long)sizeof(T) + lane_off + (RPI * x % 8 / RPI) * row_step;
-                const uint32_t to = dst + RPI * x * ROW + (lane_piece ^ ((RPI * x) & 7) * 16);
-                cp_async16(to, a.k + (use ? off : 0), use);
-                cp_async16(to + R::kHalf, a.v + (use ? off : 0), use);
+                for (int y = 0; y < 8 / RPI; y++, from += row_step) {
+                    cp_async16(group + to_lane[y], from);
+                    cp_async16(group + to_lane[y] + R::kHalf, from + v_off);
+                }
+            } else {
+                if (!good && jg < in.len && a.status && (in.sees(jg) || in.sees(min(jg + 7, in.len - 1)))) *a.status = 1;
+#pragma unroll
+                for (int y = 0; y < 8 / RPI; y++, from += row_step) {
+                    const bool use = good && dims && in.sees(jg + r0 + RPI * y);
+                    cp_async16(group + to_lane[y], use ? from : a.k, use);
+                    cp_async16(group + to_lane[y] + R::kHalf, use ? from + v_off : a.v, use);
+                }
             }
         }
     };
@@ -282,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
 #pragma unroll
     for (int x = 0; x < R::kStages - 1; x++) {
         if (x < tiles) {
-            issue(x);
+            issue(x * R::kStage);
             in.next(a, hh_n);
             look_up();
         }
@@ -311,13 +325,22 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
     };
     queries();
 
-    const float k2 = a.scale * kLog2e, kcap = a.cap > 0.f ? 2.f * kLog2e / a.cap : 0.f;
-    const bool extra = a.cap > 0.f || a.slopes;
-    const uint32_t k_lane = (lane & 15) * ROW, k_piece = ((lane >> 4) ^ (lane & 7)) * 16;
-    const uint32_t v_lane = ((lane & 7) + ((lane >> 4) << 3)) * ROW, v_piece = (((lane >> 3) & 1) ^ (lane & 7)) * 16;
+    const bool extra = a.cap > 0.f || a.slopes || !(a.scale > 0.f);  // scores are more than a positive multiple of products
+    const float k2 = extra && !F32 ? 1.f : a.scale * kLog2e, kcap = a.cap > 0.f ? 2.f * kLog2e / a.cap : 0.f;
+    // where a lane's matrices of the products lie in a stage
+    uint32_t k_at[F32 ? 1 : DP / 16], v_at[F32 ? 1 : DP / 16];
+    if constexpr (!F32) {
+#pragma unroll
+        for (int i = 0; i < DP / 16; i++) {
+            k_at[i] = wring + (lane & 15) * ROW + ((((lane >> 4) ^ (lane & 7)) * 16) ^ i * 32);
+            v_at[i] = wring + R::kHalf + ((lane & 7) + ((lane >> 4) << 3)) * ROW + (((((lane >> 3) & 1) ^ (lane & 7)) * 16) ^ i * 32);
+        }
+    }
+    uint32_t slot = 0, slot_in = (R::kStages - 1) * R::kStage;  // of the tile to compute and to load
     bool began = it.i == 0;  // the unit's first tile lies in this share
     bool fresh = true;
     float m[NM], l[NM];  // value that weights are taken from (log2), sums of this lane's weights
+    uint32_t seen = 0;   // heads that have such a value
     float acc[NACC][4];
     for (int x = 0; x < tiles; x++) {
         if (fresh) {
@@ -332,7 +355,8 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
                 __syncthreads();
             }
 #pragma unroll
-            for (int i = 0; i < NM; i++) m[i] = -INFINITY, l[i] = 0.f;
+            for (int i = 0; i < NM; i++) m[i] = F32 ? -INFINITY : 0.f, l[i] = 0.f;
+            seen = 0;
 #pragma unroll
             for (int i = 0; i < NACC; i++)
 #pragma unroll
@@ -342,14 +366,13 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
         cp_wait<R::kStages - 2>();
         __syncwarp();
         if (x + R::kStages - 1 < tiles) {
-            issue((x + R::kStages - 1) % R::kStages);
+            issue(slot_in);
             in.next(a, hh_n);
             look_up();
         }
         cp_commit();
-        const int j = it.t.key(it.i) + warp * KEYS, p = it.len - 1;
-        const uint32_t kb = wring + (x % R::kStages) * R::kStage, vb = kb + R::kHalf;
-        const bool full = j + KEYS <= it.len && (j >= it.low(a) || j + KEYS <= it.pre);
+        const int j = it.j + warp * KEYS, p = it.len - 1;
+        const bool full = it.all_visible(j, KEYS);
         if constexpr (!F32) {
             constexpr int MT = KEYS / 16;
             float s[MT][NG][4];
@@ -364,68 +387,78 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
 #pragma unroll
                 for (int t = 0; t < MT; t++) {
                     uint32_t kf[4];
-                    ldsm4(kb + t * 16 * ROW + k_lane + (k_piece ^ k * 32), kf);
+                    ldsm4(slot + t * 16 * ROW + k_at[k], kf);
 #pragma unroll
                     for (int n = 0; n < NG; n++) mma<T>(s[t][n], kf, q[n][k][0], q[n][k][1]);
                 }
-            // scores in log2; element e of tile t: key 16 t + lane / 4 (+ 8 for e > 1), head 2 (lane % 4) + e % 2
+            // element e of tile t: key 16 t + lane / 4 (+ 8 for e > 1), head 2 (lane % 4) + e % 2
+            if (extra || !full) {
+#pragma unroll
+                for (int t = 0; t < MT; t++)
+#pragma unroll
+                    for (int n = 0; n < NG; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int jj = j + 16 * t + (lane >> 2) + (e >> 1) * 8;
+                            float z = s[t][n][e];
+                            if (extra) {
+                                const int h = n * 8 + 2 * (lane & 3) + (e & 1);
+                                z *= a.scale;
+                                if (a.cap > 0.f) z = capped(z, a.cap, kcap);
+                                if (a.slopes && h < ng) z -= __ldg(a.slopes + head0 + h) * (float)(p - jj);
+                                z *= kLog2e;
+                            }
+                            if (!full && !it.sees(jj)) z = -INFINITY;
+                            s[t][n][e] = z;
+                        }
+            }
+            // exponents: scores in log2 less the value that weights are taken from
+            bool past = seen != (1u << NM) - 1;
 #pragma unroll
             for (int t = 0; t < MT; t++)
 #pragma unroll
                 for (int n = 0; n < NG; n++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const int jj = j + 16 * t + (lane >> 2) + (e >> 1) * 8;
-                        float z = s[t][n][e];
-                        if (extra) {
-                            const int h = n * 8 + 2 * (lane & 3) + (e & 1);
-                            z *= a.scale;
-                            if (a.cap > 0.f) z = capped(z, a.cap, kcap);
-                            if (a.slopes && h < ng) z -= __ldg(a.slopes + head0 + h) * (float)(p - jj);
-                            z *= kLog2e;
-                        } else
-                            z *= k2;
-                        if (!full && !visible(jj, p, it.len, it.pre, a.window)) z = -INFINITY;
-                        s[t][n][e] = z;
+                        s[t][n][e] = fmaf(s[t][n][e], k2, -m[2 * n + (e & 1)]);
+                        past |= s[t][n][e] > 8.f;
                     }
-            bool past = false;
-#pragma unroll
-            for (int t = 0; t < MT; t++)
-#pragma unroll
-                for (int n = 0; n < NG; n++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) past |= s[t][n][e] > m[2 * n + (e & 1)] + 8.f;
             if (__any_sync(0xffffffffu, past)) {
 #pragma unroll
-                for (int n = 0; n < NG; n++)
+                for (int i = 0; i < NM; i++) {
+                    const int n = i / 2, e = i & 1;
+                    float by = -INFINITY;  // how far the largest score passes m
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float mx = m[2 * n + e];
+                    for (int t = 0; t < MT; t++) by = fmaxf(by, fmaxf(s[t][n][e], s[t][n][e + 2]));
 #pragma unroll
-                        for (int t = 0; t < MT; t++) mx = fmaxf(mx, fmaxf(s[t][n][e], s[t][n][e + 2]));
-#pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                        const float f = mx == -INFINITY ? 1.f : ex2(m[2 * n + e] - mx);
-                        m[2 * n + e] = mx;
-                        l[2 * n + e] *= f;
+                    for (int o = 4; o < 32; o <<= 1) by = fmaxf(by, __shfl_xor_sync(0xffffffffu, by, o));
+                    const bool first = !(seen >> i & 1);
+                    if (first ? by > -INFINITY : by > 0.f) {
+                        const float f = first ? 0.f : ex2(-by);
+                        seen |= 1u << i;
+                        m[i] += by;
+                        l[i] *= f;
 #pragma unroll
                         for (int d = 0; d < DP / 16; d++) {
                             acc[n * (DP / 16) + d][e] *= f;
                             acc[n * (DP / 16) + d][e + 2] *= f;
                         }
+#pragma unroll
+                        for (int t = 0; t < MT; t++) {
+                            s[t][n][e] -= by;
+                            s[t][n][e + 2] -= by;
+                        }
                     }
+                }
             }
             uint32_t pt[MT][NG][2];
 #pragma unroll
             for (int n = 0; n < NG; n++) {
-                const float m0 = m[2 * n] == -INFINITY ? 0.f : m[2 * n], m1 = m[2 * n + 1] == -INFINITY ? 0.f : m[2 * n + 1];
 #pragma unroll
                 for (int t = 0; t < MT; t++) {
                     float(&z)[4] = s[t][n];
-                    z[0] = ex2(z[0] - m0);
-                    z[1] = ex2(z[1] - m1);
-                    z[2] = ex2(z[2] - m0);
-                    z[3] = ex2(z[3] - m1);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) z[e] = ex2(z[e]);
                     l[2 * n] += z[0] + z[2];
                     l[2 * n + 1] += z[1] + z[3];
                     pt[t][n][0] = transpose8(pack2<T>(z[0], z[1]));
@@ -437,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
 #pragma unroll
                 for (int t = 0; t < MT; t++) {
                     uint32_t vf[4];
-                    ldsm4_t(vb + t * 16 * ROW + v_lane + (v_piece ^ d * 32), vf);
+                    ldsm4_t(slot + t * 16 * ROW + v_at[d], vf);
 #pragma unroll
                     for (int n = 0; n < NG; n++) mma<T>(acc[n * (DP / 16) + d], vf, pt[t][n][0], pt[t][n][1]);
                 }
@@ -447,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
             float s[8];
 #pragma unroll
             for (int h = 0; h < 8; h++) s[h] = 0.f;
-            const float *kr = reinterpret_cast<const float *>(smem + warp * R::kStages * R::kStage + (x % R::kStages) * R::kStage);
+            const float *kr = reinterpret_cast<const float *>(smem + warp * R::kStages * R::kStage + slot);
 #pragma unroll 4
             for (int i = 0; i < CH / 2; i++) {
                 const int cc = half * (CH / 2) + i;
@@ -461,14 +494,14 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
                     s[h] = fmaf(kx.w, qx.w, s[h]);
                 }
             }
-            const bool see = full || visible(j + r, p, it.len, it.pre, a.window);
+            const bool see = full || it.sees(j + r);
             float *wt = sw + warp * 8 * KEYS;
             bool past = false;
 #pragma unroll
             for (int h = 0; h < 8; h++) {
                 s[h] += __shfl_xor_sync(0xffffffffu, s[h], 16);
                 const float slope = a.slopes && h < ng ? __ldg(a.slopes + head0 + h) : 0.f;
-                s[h] = !see ? -INFINITY : extra ? score2(a, s[h], slope, p, j + r) : s[h] * a.scale * kLog2e;
+                s[h] = !see ? -INFINITY : extra ? score2(a, s[h], slope, p, j + r) : s[h] * k2;
                 past |= s[h] > m[h] + 8.f;
             }
             if (__any_sync(0xffffffffu, past)) {
@@ -516,6 +549,8 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
             __syncwarp();
         }
 
+        slot = slot == (R::kStages - 1) * R::kStage ? 0 : slot + R::kStage;
+        slot_in = slot_in == (R::kStages - 1) * R::kStage ? 0 : slot_in + R::kStage;
         const bool last = it.i == it.t.n - 1;
         if (last || x == tiles - 1) {
             const int seq = it.seq, h0 = head0, hn = ng, rest = it.t.n - 1 - it.i;
@@ -529,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 4);
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 8);
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 16);
-                    if (lane < 4) stat[warp * H + (i / 2) * 8 + 2 * lane + (i & 1)] = make_float2(m[i], l[i]);
+                    if (lane < 4) stat[warp * H + (i / 2) * 8 + 2 * lane + (i & 1)] = make_float2(seen >> i & 1 ? m[i] : -INFINITY, l[i]);
                 }
             } else {
 #pragma unroll
@@ -679,6 +714,7 @@ extern "C" int mocha_kv_decode(const mocha_kv_pages *pages, const mocha_kv_seqs 
     w.unit_heads = 8 * ng;
     w.hgroups = (w.a.group + w.unit_heads - 1) / w.unit_heads;
     w.min_tiles = 2;
+    w.one_page = pages->page_size % (b == 2 && dp == 64 ? 32 : 16) == 0;
     w.a.meta = static_cast<Meta *>(workspace);
     w.a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + meta_bytes(ctas));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
