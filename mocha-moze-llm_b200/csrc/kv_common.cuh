@@ -20,6 +20,9 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+#include <utility>
+
 #include "mb_async.cuh"
 #include "mb_common.cuh"
 #include "mocha_kv.h"
@@ -52,10 +55,8 @@ MB_DEV uint32_t div(FastDiv f, uint32_t n)
 // CTA's slot 1 and in slot 0 of the CTAs up to c_end.  Row r of the unit is token
 // row0 + r / ng, head head0 + r % ng.
 struct Meta {
-    int c_end;  // -1: no unit is cut here
-    int row0, ntok, head0, ng;
+    int row0, head0, ng;
     int seq, pos0;  // sequence, and position of token row0
-    int pad;
 };
 
 struct Args {
@@ -80,6 +81,7 @@ struct Args {
     float *lse;
     const int *q_start;  // prefill
     int rows;
+    int2 *note;   // [CTAs] c_end, or -1 where no unit is cut, and rows of the unit
     Meta *meta;   // [CTAs]
     float *part;  // [CTAs][2][part rows][2 + padded dim]: outputs of all rows, then (m, l) of all rows
 };
@@ -221,7 +223,8 @@ __device__ __forceinline__ void lone_row(const Args &a, int seq, int p, int head
 // The rows of all cut units are dealt to the blocks: a warp takes a row whose parts are
 // few, a block one whose parts are many (more than kJoinSerial), lanes the dims.  Bound by
 // the parts' bytes: each is read once.
-constexpr int kJoinWarps = 8, kJoinSerial = 32, kJoinMetas = 2 * mb::kSMs;
+// Two large blocks an SM: every block reads all notes, and more would queue for their lines.
+constexpr int kJoinWarps = 16, kJoinSerial = 16, kJoinMetas = 2 * mb::kSMs, kJoinBlocks = 2 * mb::kSMs;
 
 struct Joined {
     float m, l;
@@ -245,24 +248,20 @@ struct Joined {
 };
 
 template <typename T, bool PREFILL>
-__global__ void __launch_bounds__(32 * kJoinWarps) k_join(const __grid_constant__ Args a, int metas, int part_rows, int dp)
+__global__ void __launch_bounds__(32 * kJoinWarps, 2) k_join(const __grid_constant__ Args a, int metas, int part_rows, int dp)
 {
     __shared__ Joined s_part[kJoinWarps][32];
     __shared__ int s_items[kJoinMetas], s_warp[kJoinWarps], s_total;
     mb::as::griddep_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     // items (a block's work) before each unit's end, in the order of the CTAs
-    int n[2] = {0, 0};
-#pragma unroll
-    for (int x = 0; x < 2; x++) {
-        const int c = 2 * tid + x;
-        if (c >= metas) continue;
-        const int end = __ldcg(&a.meta[c].c_end);
-        if (end < 0) continue;
-        const int rows = __ldcg(&a.meta[c].ntok) * __ldcg(&a.meta[c].ng);
-        n[x] = end - c < kJoinSerial ? (rows + kJoinWarps - 1) / kJoinWarps : rows;
+    static_assert(kJoinMetas <= 32 * kJoinWarps, "a thread per note");
+    int n = 0;
+    if (tid < metas) {
+        const int2 note = __ldcg(a.note + tid);
+        if (note.x >= 0) n = note.x - tid < kJoinSerial ? (note.y + kJoinWarps - 1) / kJoinWarps : note.y;
     }
-    int incl = n[0] + n[1];
+    int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int x = __shfl_up_sync(0xffffffffu, incl, o);
@@ -271,8 +270,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_join(const __grid_constant_
     if (lane == 31) s_warp[warp] = incl;
     __syncthreads();
     for (int w = 0; w < warp; w++) incl += s_warp[w];
-    if (2 * tid < metas) s_items[2 * tid] = incl - n[1];
-    if (2 * tid + 1 < metas) s_items[2 * tid + 1] = incl;
+    if (tid < metas) s_items[tid] = incl;
     if (tid == 32 * kJoinWarps - 1) s_total = incl;
     __syncthreads();
     const int total = s_total;
@@ -281,15 +279,16 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_join(const __grid_constant_
         int c = 0;  // the first unit that ends after `item`
         for (int step = 256; step; step >>= 1)
             if (c + step <= metas && s_items[c + step - 1] <= item) c += step;
+        const int2 note = __ldcg(a.note + c);
         const Meta mt = a.meta[c];
-        const int first = c ? s_items[c - 1] : 0;
-        const bool serial = mt.c_end - c < kJoinSerial;
+        const int first = c ? s_items[c - 1] : 0, c_end = note.x;
+        const bool serial = c_end - c < kJoinSerial;
         const int r = serial ? (item - first) * kJoinWarps + warp : item - first;
-        const bool there = r < mt.ntok * mt.ng;
+        const bool there = r < note.y;
         Joined x{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-        constexpr int U = 8;  // parts in flight per warp
+        constexpr int U = 4;  // parts in flight per warp
         if (there)
-            for (int b = c + (serial ? 0 : warp * U); b <= mt.c_end; b += serial ? U : kJoinWarps * U) {
+            for (int b = c + (serial ? 0 : warp * U); b <= c_end; b += serial ? U : kJoinWarps * U) {
                 float pm[U], pl[U];
                 float4 pv[U];
 #pragma unroll
@@ -297,7 +296,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_join(const __grid_constant_
                     pm[u] = -INFINITY;
                     pl[u] = 0.f;
                     pv[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (b + u <= mt.c_end) {
+                    if (b + u <= c_end) {
                         const float *pp = a.part + ((size_t)(b + u) * 2 + (b + u == c ? 1 : 0)) * slot;
                         const float2 ml = __ldcg(reinterpret_cast<const float2 *>(pp + (size_t)part_rows * dp) + r);
                         pm[u] = ml.x;
@@ -363,30 +362,38 @@ inline int fail(const char *who, const char *what)
     return 1;
 }
 
-// Makes `device` current for a call and puts the caller's back.
+// Makes `device` current for a call and puts the caller's back.  What a device is does not
+// change, so it is asked once (two threads that ask at once find the same).
 class DeviceGuard {
   public:
     int enter(const char *who, int device)
     {
-        int count = 0, major = 0;
-        if (cudaGetDevice(&old_) != cudaSuccess || cudaGetDeviceCount(&count) != cudaSuccess)
-            return (void)cudaGetLastError(), fail(who, "no CUDA device");
-        if (device < 0 || device >= count) return fail(who, "device out of range");
-        if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) != cudaSuccess || major != 10)
-            return fail(who, "requires a compute capability 10.x (B200) device");
+        static std::atomic<unsigned long long> known{0};
+        if (cudaGetDevice(&old_) != cudaSuccess) return (void)cudaGetLastError(), fail(who, "no CUDA device");
+        const unsigned long long bit = device >= 0 && device < 64 ? 1ull << device : 0;
+        if (!(known.load(std::memory_order_relaxed) & bit)) {
+            int count = 0, major = 0;
+            if (cudaGetDeviceCount(&count) != cudaSuccess) return (void)cudaGetLastError(), fail(who, "no CUDA device");
+            if (device < 0 || device >= count) return fail(who, "device out of range");
+            if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) != cudaSuccess || major != 10)
+                return fail(who, "requires a compute capability 10.x (B200) device");
+            known.fetch_or(bit, std::memory_order_relaxed);
+        }
         if (device != old_) {
             if (cudaSetDevice(device) != cudaSuccess) return (void)cudaGetLastError(), fail(who, "cudaSetDevice failed");
             changed_ = true;
         }
+        device_ = device;
         return 0;
     }
+    int device() const { return device_; }
     ~DeviceGuard()
     {
         if (changed_) cudaSetDevice(old_);
     }
 
   private:
-    int old_ = 0;
+    int old_ = 0, device_ = 0;
     bool changed_ = false;
 };
 
@@ -489,15 +496,11 @@ inline Args make_args(const mocha_kv_pages *p, const mocha_kv_seqs *s, const moc
     return a;
 }
 
-// Launch with an error message; `after`: the kernel may start while the one before it in
-// the stream ends, and waits for it itself.
+// Launch on the current device with an error message; `after`: the kernel may start while
+// the one before it in the stream ends, and waits for it itself.
 template <typename... K, typename... A>
 int launch(const char *who, void (*kernel)(K...), dim3 grid, int threads, size_t smem, cudaStream_t s, bool after, A &&...args)
 {
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return (void)cudaGetLastError(), fail(who, cudaGetErrorString(e));
-    }
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -513,8 +516,27 @@ int launch(const char *who, void (*kernel)(K...), dim3 grid, int threads, size_t
     return 0;
 }
 
+// More than 48 KB of shared memory for a kernel, asked for once per kernel and device:
+// `allowed` is the kernel's own.
+template <typename... K>
+int allow_smem(const char *who, void (*kernel)(K...), size_t smem, int device, std::atomic<unsigned long long> &allowed)
+{
+    const unsigned long long bit = device < 64 ? 1ull << device : 0;
+    if (allowed.load(std::memory_order_relaxed) & bit) return 0;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (void)cudaGetLastError(), fail(who, cudaGetErrorString(e));
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+    return 0;
+}
+
 // Workspace of one call: the CTAs' notes of cut units, then their parts.
-inline size_t meta_bytes(int ctas) { return ((size_t)ctas * sizeof(Meta) + 255) / 256 * 256; }
+inline size_t meta_bytes(int ctas) { return ((size_t)ctas * (sizeof(int2) + sizeof(Meta)) + 255) / 256 * 256; }
+inline void lay_out(Args &a, void *space, int ctas)
+{
+    a.note = static_cast<int2 *>(space);
+    a.meta = reinterpret_cast<Meta *>(a.note + ctas);
+    a.part = reinterpret_cast<float *>(static_cast<char *>(space) + meta_bytes(ctas));
+}
 inline size_t part_bytes(int ctas, int rows, int dp) { return (size_t)ctas * 2 * rows * (dp + 2) * sizeof(float); }
 inline int padded_dim(int d) { return d <= 64 ? 64 : 128; }
 

@@ -24,26 +24,27 @@ namespace {
 
 using namespace kv;
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps;
-
-// CTAs of an SM, keys of a warp's tile, and the stages of its ring (keys then values): 192
-// KB of rings per SM, 8 KB (fp32: 8 or 16 KB) a stage, so that two or more stages per warp
-// are in flight, which covers the memory's latency, while one is computed.  Two CTAs overlap
-// one's unit ends with the other's tiles; wide groups (registers) and fp32 rows of 128
-// leave room for one.
+// CTAs of an SM, warps of a CTA, keys of a warp's tile, and the stages of its ring (keys
+// then values): 192 KB of rings and eight warps per SM, three stages of 8 KB a warp, so
+// that two are in flight while one is computed.  16-bit: two CTAs of four warps overlap
+// one's unit ends with the other's tiles (wide groups, for their registers, leave room for
+// one, with longer rings); fp32: one of eight, as the FMA units need the warps at once.
+// A unit has H query heads at most: 8 NG, or 4 for NG = 0 (fp32 alone).
 template <typename T, int DP, int NG>
 struct Ring {
     static constexpr bool kF32 = sizeof(T) == 4;
-    static constexpr int kKeys = DP == 64 && !kF32 ? 32 : 16, kTile = kWarps * kKeys;
+    static constexpr int kWarps = kF32 ? 8 : 4, kThreads = 32 * kWarps;
+    static constexpr int kH = NG ? 8 * NG : 4, kHB = 4;  // heads; heads met at a time (the join's blocks find room beside two CTAs)
+    static constexpr int kKeys = (kF32 ? 1024 : 2048) / DP, kTile = kWarps * kKeys;
     static constexpr int kHalf = kKeys * DP * (int)sizeof(T), kStage = 2 * kHalf;
-    static constexpr int kCtas = NG > 1 || (kF32 && DP == 128) ? 1 : 2;
+    static constexpr int kCtas = kF32 || NG > 1 ? 1 : 2;
     static constexpr int kStages = 192 * 1024 / kCtas / kWarps / kStage;
     static constexpr int kRings = kWarps * kStages * kStage;
     static constexpr int kPad = DP + 4;  // floats of a head's row in the merge buffers
-    static constexpr int kMerge = kWarps * 8 * kPad * 4;
-    static constexpr int kStat = kWarps * 8 * NG * 8;              // (m, l)
-    static constexpr int kQ = kF32 ? 8 * DP * 4 : 0;               // fp32: the unit's queries,
-    static constexpr int kW = kF32 ? kWarps * 8 * kKeys * 4 : 0;  // and a tile's weights
+    static constexpr int kMerge = kWarps * kHB * kPad * 4;
+    static constexpr int kStat = kWarps * kH * 8;                   // (m, l)
+    static constexpr int kQ = kF32 ? kH * DP * 4 : 0;              // fp32: the unit's queries,
+    static constexpr int kW = kF32 ? kWarps * kH * kKeys * 4 : 0;  // and a tile's weights
     static constexpr int kTotal = kRings + kMerge + kStat + kQ + kW;
 };
 
@@ -156,12 +157,13 @@ MB_DEV uint32_t pack2(float x, float y)
 
 // The share of this CTA: its first tile as (sequence, tile within the sequence) in *s_seq
 // and *s_rem, and [start, end) in tiles of the whole call.
-template <int TILE>
+template <int TILE, int kWarps>
 MB_DEV bool find_share(const Work &w, int hh_n, long long *s_warp, int *s_seq, long long *s_rem, long long *start,
                        long long *end, long long *per)
 {
     const Args &a = w.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int kThreads = 32 * kWarps;
     const int chunk = (a.seqs + kThreads - 1) / kThreads, b0 = min(tid * chunk, a.seqs), b1 = min(b0 + chunk, a.seqs);
     Walk<TILE> k;
     long long sum = 0;
@@ -202,16 +204,17 @@ MB_DEV bool find_share(const Work &w, int hh_n, long long *s_warp, int *s_seq, l
 }
 
 template <typename T, int DP, int NG>
-__global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(const __grid_constant__ Work w)
+__global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kCtas) k_decode(const __grid_constant__ Work w)
 {
     using R = Ring<T, DP, NG>;
     constexpr bool F32 = R::kF32;
-    constexpr int KEYS = R::kKeys, H = 8 * NG;
+    constexpr int KEYS = R::kKeys, H = R::kH, HB = R::kHB, kWarps = R::kWarps, kThreads = R::kThreads;
     constexpr int CH = DP * (int)sizeof(T) / 16;     // 16-byte pieces of a row
     constexpr int RPI = 32 / CH;                     // rows of a warp's copy
     constexpr int GROUPS = KEYS / 8;                 // of 8 keys, which lie in one page
     constexpr int ROW = DP * (int)sizeof(T);
-    constexpr int NM = F32 ? 8 : 2 * NG, NACC = F32 ? 8 : NG * DP / 16;
+    constexpr int NM = F32 ? H : 2 * NG, NACC = F32 ? H : NG * DP / 16;
+    constexpr int PARTS = 32 / KEYS;                 // fp32: lanes that share a key's products
     extern __shared__ __align__(128) unsigned char smem[];
     float *merge = reinterpret_cast<float *>(smem + R::kRings);
     float2 *stat = reinterpret_cast<float2 *>(smem + R::kRings + R::kMerge);
@@ -224,8 +227,8 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
     const int hh_n = a.kv_heads * w.hgroups;
     mb::as::griddep_launch();
     long long start, end, per;
-    if (!find_share<R::kTile>(w, hh_n, s_warp, &s_seq, &s_rem, &start, &end, &per)) {
-        if (tid == 0) a.meta[blockIdx.x].c_end = -1;
+    if (!find_share<R::kTile, kWarps>(w, hh_n, s_warp, &s_seq, &s_rem, &start, &end, &per)) {
+        if (tid == 0) a.note[blockIdx.x].x = -1;
         return;
     }
     Walk<R::kTile> in;  // the next tile to load
@@ -346,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
         if (fresh) {
             if constexpr (F32) {
                 // the last unit's queries are no longer read: its end was met
-                for (int e = tid; e < 8 * CH; e += kThreads) {
+                for (int e = tid; e < H * CH; e += kThreads) {
                     const int h = e / CH, cc = e % CH;
                     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (h < ng && cc * 4 < a.d) y = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + it.seq * a.q_row + (head0 + h) * a.q_head + cc * 4);
@@ -367,6 +370,22 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
         __syncwarp();
         if (x + R::kStages - 1 < tiles) {
             issue(slot_in);
+            // the tile after that on its way into L2: what is in flight in shared memory alone
+            // does not cover the latency of loaded memory (128 sequences: 441 -> 405 us)
+            if (in.i + 1 < in.t.n) {
+                constexpr int LINES = ROW / 128;
+                const int kvh = w.hgroups == 1 ? in.hh : in.hh / w.hgroups;
+                const int jp = in.t.key(in.i + 1) + warp * KEYS + lane / LINES, pl = lane % LINES * 128;
+                if (in.sees(jp) && pl < a.d * (int)sizeof(T)) {
+                    const uint32_t sl = div(a.page, jp);
+                    const int id = __ldg(a.table + in.seq * a.table_stride + sl);
+                    if ((unsigned)id < (unsigned)a.pages) {
+                        const char *at = a.k + (id * a.ps + kvh * a.hs + (jp - (int)(sl * a.page.d)) * a.ts) * (long long)sizeof(T) + pl;
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(at + v_off));
+                    }
+                }
+            }
             in.next(a, hh_n);
             look_up();
         }
@@ -475,18 +494,19 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
                     for (int n = 0; n < NG; n++) mma<T>(acc[n * (DP / 16) + d], vf, pt[t][n][0], pt[t][n][1]);
                 }
         } else {
-            // scores: lane = key (16) x half of the dims, 8 heads each
-            const int r = lane & 15, half = lane >> 4;
-            float s[8];
+            // scores: lane = key x part of the dims (32 of them), all heads.  The parts start
+            // two pieces apart, so that their queries lie in different banks.
+            const int r = lane % KEYS, pt = lane / KEYS;
+            float s[H];
 #pragma unroll
-            for (int h = 0; h < 8; h++) s[h] = 0.f;
+            for (int h = 0; h < H; h++) s[h] = 0.f;
             const float *kr = reinterpret_cast<const float *>(smem + warp * R::kStages * R::kStage + slot);
 #pragma unroll 4
-            for (int i = 0; i < CH / 2; i++) {
-                const int cc = half * (CH / 2) + i;
+            for (int i = 0; i < 8; i++) {
+                const int cc = pt * 8 + ((i + 2 * pt) & 7);
                 const float4 kx = *reinterpret_cast<const float4 *>(kr + r * DP + ((cc ^ (r & 7)) * 4));
 #pragma unroll
-                for (int h = 0; h < 8; h++) {
+                for (int h = 0; h < H; h++) {
                     const float4 qx = *reinterpret_cast<const float4 *>(sq + h * DP + cc * 4);
                     s[h] = fmaf(kx.x, qx.x, s[h]);
                     s[h] = fmaf(kx.y, qx.y, s[h]);
@@ -495,18 +515,19 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
                 }
             }
             const bool see = full || it.sees(j + r);
-            float *wt = sw + warp * 8 * KEYS;
+            float *wt = sw + warp * H * KEYS;
             bool past = false;
 #pragma unroll
-            for (int h = 0; h < 8; h++) {
-                s[h] += __shfl_xor_sync(0xffffffffu, s[h], 16);
+            for (int h = 0; h < H; h++) {
+#pragma unroll
+                for (int o = KEYS; o < 32; o <<= 1) s[h] += __shfl_xor_sync(0xffffffffu, s[h], o);
                 const float slope = a.slopes && h < ng ? __ldg(a.slopes + head0 + h) : 0.f;
                 s[h] = !see ? -INFINITY : extra ? score2(a, s[h], slope, p, j + r) : s[h] * k2;
                 past |= s[h] > m[h] + 8.f;
             }
             if (__any_sync(0xffffffffu, past)) {
 #pragma unroll
-                for (int h = 0; h < 8; h++) {
+                for (int h = 0; h < H; h++) {
                     const float mx = fmaxf(m[h], mb::warp_max(s[h])), f = mx == -INFINITY ? 1.f : exp2f(m[h] - mx);
                     m[h] = mx;
                     l[h] *= f;
@@ -515,26 +536,22 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
                 }
             }
 #pragma unroll
-            for (int h = 0; h < 8; h++) {
+            for (int h = 0; h < H; h++) {
                 const float e = exp2f(s[h] - (m[h] == -INFINITY ? 0.f : m[h]));
-                l[h] += e;  // every key counts in two lanes
-                if (!half) wt[h * KEYS + r] = e;
+                l[h] += e;  // every key counts in PARTS lanes
+                if (pt == 0) wt[h * KEYS + r] = e;
             }
             __syncwarp();
             // outputs: a lane holds 4 dims; with 64 dims the half-warps take 8 keys each
             const float *vr = kr + R::kHalf / 4;
-            constexpr int KK = DP == 128 ? KEYS : KEYS / 2;
-            const int cv = DP == 128 ? lane : lane & 15, k0 = DP == 128 ? 0 : half * KK;
+            const int cv = lane % CH, k0 = lane / CH * 8;
 #pragma unroll
-            for (int g = 0; g < KK / 4; g++) {
+            for (int g = 0; g < 2; g++) {
                 float4 v[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int row = k0 + 4 * g + i;
-                    v[i] = *reinterpret_cast<const float4 *>(vr + row * DP + ((cv ^ (row & 7)) * 4));
-                }
+                for (int i = 0; i < 4; i++) v[i] = *reinterpret_cast<const float4 *>(vr + (k0 + 4 * g + i) * DP + ((cv ^ (4 * g + i)) * 4));
 #pragma unroll
-                for (int h = 0; h < 8; h++) {
+                for (int h = 0; h < H; h++) {
                     const float4 e = *reinterpret_cast<const float4 *>(wt + h * KEYS + k0 + 4 * g);
                     const float ew[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
@@ -568,8 +585,8 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
                 }
             } else {
 #pragma unroll
-                for (int h = 0; h < 8; h++) {
-                    l[h] = mb::warp_sum(l[h]) * 0.5f;
+                for (int h = 0; h < H; h++) {
+                    l[h] = mb::warp_sum(l[h]) * (1.f / PARTS);
                     if (DP == 64) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) acc[h][i] += __shfl_xor_sync(0xffffffffu, acc[h][i], 16);
@@ -578,23 +595,28 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
                 }
             }
             float *part = a.part + ((size_t)blockIdx.x * 2 + (began ? 1 : 0)) * ((size_t)H * (DP + 2));
-            float *mine = merge + warp * 8 * R::kPad;
+            float *mine = merge + warp * HB * R::kPad;
 #pragma unroll
-            for (int n = 0; n < NG; n++) {
+            for (int n = 0; n < H / HB; n++) {
                 if constexpr (!F32) {
+                    // a lane has heads 2 (lane % 4) and the next of each eight
+                    if ((lane & 3) / 2 == n % 2) {
 #pragma unroll
-                    for (int d = 0; d < DP / 16; d++)
+                        for (int d = 0; d < DP / 16; d++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            mine[(2 * (lane & 3) + (e & 1)) * R::kPad + d * 16 + (lane >> 2) + (e >> 1) * 8] = acc[n * (DP / 16) + d][e];
+                            for (int e = 0; e < 4; e++)
+                                mine[(2 * (lane & 1) + (e & 1)) * R::kPad + d * 16 + (lane >> 2) + (e >> 1) * 8] = acc[n / 2 * (DP / 16) + d][e];
+                    }
                 } else if (lane * 4 < DP) {
 #pragma unroll
-                    for (int h = 0; h < 8; h++)
-                        *reinterpret_cast<float4 *>(mine + h * R::kPad + lane * 4) = make_float4(acc[h][0], acc[h][1], acc[h][2], acc[h][3]);
+                    for (int h = 0; h < HB; h++) {
+                        const float(&y)[4] = acc[n * HB + h];
+                        *reinterpret_cast<float4 *>(mine + h * R::kPad + lane * 4) = make_float4(y[0], y[1], y[2], y[3]);
+                    }
                 }
                 __syncthreads();
-                for (int e = tid; e < 8 * (DP / 4); e += kThreads) {
-                    const int hl = e / (DP / 4), cc = e % (DP / 4), h = n * 8 + hl;
+                for (int e = tid; e < HB * (DP / 4); e += kThreads) {
+                    const int hl = e / (DP / 4), cc = e % (DP / 4), h = n * HB + hl;
                     if (h >= hn) break;
                     float M = -INFINITY, L = 0.f;
                     float2 ml[kWarps];
@@ -608,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
 #pragma unroll
                     for (int i = 0; i < kWarps; i++) {
                         const float f = exp2f(ml[i].x - ms);
-                        const float4 z = *reinterpret_cast<const float4 *>(merge + (i * 8 + hl) * R::kPad + cc * 4);
+                        const float4 z = *reinterpret_cast<const float4 *>(merge + (i * HB + hl) * R::kPad + cc * 4);
                         L = fmaf(ml[i].y, f, L);
                         y.x = fmaf(z.x, f, y.x);
                         y.y = fmaf(z.y, f, y.y);
@@ -629,18 +651,8 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
                 __syncthreads();  // the buffers are written again
             }
             if (x == tiles - 1 && tid == 0) {
-                Meta mt{};
-                mt.c_end = -1;
-                if (noted) {
-                    mt.c_end = (int)div64(end - 1 + rest, per);
-                    mt.row0 = seq;
-                    mt.ntok = 1;
-                    mt.head0 = h0;
-                    mt.ng = hn;
-                    mt.seq = seq;
-                    mt.pos0 = p;
-                }
-                a.meta[blockIdx.x] = mt;
+                a.note[blockIdx.x] = make_int2(noted ? (int)div64(end - 1 + rest, per) : -1, hn);
+                a.meta[blockIdx.x] = Meta{seq, h0, hn, seq, p};
             }
             began = true;
             fresh = true;
@@ -651,37 +663,42 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DP, NG>::kCtas) k_decode(con
 }
 
 template <typename T, int DP, int NG>
-int run(Work &w, int ctas, cudaStream_t s)
-{
-    const char *who = "mocha_kv_decode";
-    if (launch(who, k_decode<T, DP, NG>, dim3(ctas), kThreads, Ring<T, DP, NG>::kTotal, s, false, w)) return 1;
-    return launch(who, k_join<T, false>, dim3(2 * mb::kSMs), 32 * kJoinWarps, 0, s, true, w.a, ctas, 8 * NG, DP);
-}
+struct Plan {
+    using R = Ring<T, DP, NG>;
+    static constexpr int kCtas = mb::kSMs * R::kCtas;
+    static size_t workspace() { return meta_bytes(kCtas) + part_bytes(kCtas, R::kH, DP); }
+    static int run(Work &w, int page_size, char *space, int device, cudaStream_t s)
+    {
+        const char *who = "mocha_kv_decode";
+        w.unit_heads = R::kH;
+        w.hgroups = (w.a.group + R::kH - 1) / R::kH;
+        w.min_tiles = 1;
+        w.one_page = page_size % R::kKeys == 0;
+        lay_out(w.a, space, kCtas);
+        static std::atomic<unsigned long long> allowed{0};
+        if (allow_smem(who, k_decode<T, DP, NG>, R::kTotal, device, allowed) ||
+            launch(who, k_decode<T, DP, NG>, dim3(kCtas), R::kThreads, R::kTotal, s, false, w))
+            return 1;
+        return launch(who, k_join<T, false>, dim3(kJoinBlocks), 32 * kJoinWarps, 0, s, true, w.a, kCtas, R::kH, DP);
+    }
+};
 
-template <typename T, int DP>
-int run_ng(Work &w, int ng, int ctas, cudaStream_t s)
+// Calls f with the plan for a type, group and dim: units of all heads of a group up to 32
+// (16-bit), of 4 or 8 (fp32, where a wider group's heads read the keys again, from L2).
+template <typename F>
+auto with_plan(int type, int group, int d, F f)
 {
-    if constexpr (sizeof(T) == 4) return run<T, DP, 1>(w, ctas, s);
-    else return ng == 1 ? run<T, DP, 1>(w, ctas, s) : ng == 2 ? run<T, DP, 2>(w, ctas, s) : run<T, DP, 4>(w, ctas, s);
-}
-
-template <typename T>
-int run_dp(Work &w, int dp, int ng, int ctas, cudaStream_t s)
-{
-    return dp == 64 ? run_ng<T, 64>(w, ng, ctas, s) : run_ng<T, 128>(w, ng, ctas, s);
-}
-
-// Heads of a unit in eights: all of a group up to 32 (16-bit), 8 (fp32, where a group's
-// further heads read the keys again, from L2).
-int head_groups(int type, int group)
-{
-    if (type == MOCHA_KV_F32 || group <= 8) return 1;
-    return group <= 16 ? 2 : 4;
-}
-
-int cta_count(int type, int ng, int dp)
-{
-    return mb::kSMs * ((type == MOCHA_KV_F32 && dp == 128) || ng > 1 ? 1 : 2);
+    const bool wide = padded_dim(d) == 128;
+    auto half = [&](auto t) {
+        using T = decltype(t);
+        if (group <= 8) return wide ? f(Plan<T, 128, 1>{}) : f(Plan<T, 64, 1>{});
+        if (group <= 16) return wide ? f(Plan<T, 128, 2>{}) : f(Plan<T, 64, 2>{});
+        return wide ? f(Plan<T, 128, 4>{}) : f(Plan<T, 64, 4>{});
+    };
+    if (type == MOCHA_KV_F16) return half(__half{});
+    if (type == MOCHA_KV_BF16) return half(__nv_bfloat16{});
+    if (group <= 4) return wide ? f(Plan<float, 128, 0>{}) : f(Plan<float, 64, 0>{});
+    return wide ? f(Plan<float, 128, 1>{}) : f(Plan<float, 64, 1>{});
 }
 
 }  // namespace
@@ -689,8 +706,7 @@ int cta_count(int type, int ng, int dp)
 namespace kv {
 size_t decode_workspace(int type, int group, int d)
 {
-    const int ng = head_groups(type, group), dp = padded_dim(d), ctas = cta_count(type, ng, dp);
-    return meta_bytes(ctas) + part_bytes(ctas, 8 * ng, dp);
+    return with_plan(type, group, d, [](auto plan) { return plan.workspace(); });
 }
 }  // namespace kv
 
@@ -710,15 +726,7 @@ extern "C" int mocha_kv_decode(const mocha_kv_pages *pages, const mocha_kv_seqs 
     w.a = make_args(pages, seqs, scores, q, out, lse);
     if (!workspace || !aligned(workspace) || workspace_bytes < decode_workspace(pages->type, w.a.group, d))
         return fail(who, "workspace missing, not 16-byte aligned or smaller than mocha_kv_workspace says");
-    const int ng = head_groups(pages->type, w.a.group), dp = padded_dim(d), ctas = cta_count(pages->type, ng, dp);
-    w.unit_heads = 8 * ng;
-    w.hgroups = (w.a.group + w.unit_heads - 1) / w.unit_heads;
-    w.min_tiles = 2;
-    w.one_page = pages->page_size % (b == 2 && dp == 64 ? 32 : 16) == 0;
-    w.a.meta = static_cast<Meta *>(workspace);
-    w.a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + meta_bytes(ctas));
-    const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return pages->type == MOCHA_KV_F32   ? run_dp<float>(w, dp, ng, ctas, s)
-           : pages->type == MOCHA_KV_F16 ? run_dp<__half>(w, dp, ng, ctas, s)
-                                         : run_dp<__nv_bfloat16>(w, dp, ng, ctas, s);
+    return with_plan(pages->type, w.a.group, d, [&](auto plan) {
+        return plan.run(w, pages->page_size, static_cast<char *>(workspace), guard.device(), static_cast<cudaStream_t>(stream));
+    });
 }

@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kThreads) k_prefill(const __grid_constant__ Ar
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, warp = tid >> 5;
     mb::as::griddep_launch();
     if (!find_share<kKeys, kThreads>(a, tokens, min_tiles, share)) {
-        if (tid == 0) a.meta[blockIdx.x].c_end = -1;
+        if (tid == 0) a.note[blockIdx.x].x = -1;
         return;
     }
     const Share h = share.out;
@@ -351,18 +351,8 @@ __global__ void __launch_bounds__(kThreads) k_prefill(const __grid_constant__ Ar
                 }
         }
         if (left <= 0 && tid == 0) {
-            Meta mt{};
-            mt.c_end = -1;
-            if (first == 0 && !whole) {
-                mt.c_end = (int)div64(h.end - 1 + (u.t.n - stop), h.per);
-                mt.row0 = u.p.q0 + tok0;
-                mt.ntok = ntok;
-                mt.head0 = u.kvh * a.group;
-                mt.ng = a.group;
-                mt.seq = u.seq;
-                mt.pos0 = pa;
-            }
-            a.meta[blockIdx.x] = mt;
+            a.note[blockIdx.x] = make_int2(first == 0 && !whole ? (int)div64(h.end - 1 + (u.t.n - stop), h.per) : -1, nrow);
+            a.meta[blockIdx.x] = Meta{u.p.q0 + tok0, u.kvh * a.group, a.group, u.seq, pa};
         }
         if (left > 0) u.next(a, tokens);
         i = 0;
@@ -617,7 +607,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const bool any = find_share<kTcKeys, kTcThreads>(a, tokens, min_tiles, share), placed = (smem_u32(smem) & 1023) == 0;
     if (!any || !placed) {
         if (!placed && tid == 0 && a.status) *a.status = 2;
-        if (tid == 0) a.meta[blockIdx.x].c_end = -1;
+        if (tid == 0) a.note[blockIdx.x].x = -1;
         return;
     }
     if (tid == 0) bar.share = share.out;
@@ -959,18 +949,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             if (tid == 0) {
                 // the share's last unit leaves the last note
-                Meta mt{};
-                mt.c_end = -1;
-                if (d.first == 0 && d.stop < d.n) {
-                    mt.c_end = (int)div64(bar.share.end - 1 + (d.n - d.stop), bar.share.per);
-                    mt.row0 = d.row0;
-                    mt.ntok = d.ntok;
-                    mt.head0 = d.kvh * a.group;
-                    mt.ng = a.group;
-                    mt.seq = d.seq;
-                    mt.pos0 = d.pos0;
-                }
-                a.meta[blockIdx.x] = mt;
+                const bool cut = d.first == 0 && d.stop < d.n;
+                a.note[blockIdx.x] = make_int2(cut ? (int)div64(bar.share.end - 1 + (d.n - d.stop), bar.share.per) : -1, d.ntok * a.group);
+                a.meta[blockIdx.x] = Meta{d.row0, d.kvh * a.group, a.group, d.seq, d.pos0};
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.unit_empty[units % kTcUnits]);
@@ -981,7 +962,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (bar.abort) {
         // a wait ran out: no notes for the join, and the copies in flight land first
         if (tid == 0) {
-            a.meta[blockIdx.x].c_end = -1;
+            a.note[blockIdx.x].x = -1;
             if (a.status) *a.status = 2;
             const long long t0 = clock64();
             while (clock64() - t0 < kWaitCycles / 64) {
@@ -1014,12 +995,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 template <typename T, int DP>
-int run(Args &a, int ctas, cudaStream_t s)
+int run(Args &a, int ctas, int device, cudaStream_t s)
 {
     const char *who = "mocha_kv_prefill";
     const int tokens = kRows / a.group;
-    if (launch(who, k_prefill<T, DP>, dim3(ctas), kThreads, Smem32<DP>::kTotal, s, false, a, tokens, 2)) return 1;
-    return launch(who, k_join<T, true>, dim3(4 * mb::kSMs), 32 * kJoinWarps, 0, s, true, a, ctas, kRows, DP);
+    static std::atomic<unsigned long long> allowed{0};
+    if (allow_smem(who, k_prefill<T, DP>, Smem32<DP>::kTotal, device, allowed) ||
+        launch(who, k_prefill<T, DP>, dim3(ctas), kThreads, Smem32<DP>::kTotal, s, false, a, tokens, 2))
+        return 1;
+    return launch(who, k_join<T, true>, dim3(kJoinBlocks), 32 * kJoinWarps, 0, s, true, a, ctas, kRows, DP);
 }
 
 // ---- tensor maps -----------------------------------------------------------------------
@@ -1054,7 +1038,7 @@ int encode(CUtensorMap *map, int type, const void *base, const long long (&n)[4]
 }
 
 template <typename T, int DP>
-int run_tc(Args &a, const mocha_kv_pages *p, cudaStream_t s)
+int run_tc(Args &a, const mocha_kv_pages *p, int device, cudaStream_t s)
 {
     const char *who = "mocha_kv_prefill";
     const int tok = 128 / a.group, d = a.d;
@@ -1065,12 +1049,14 @@ int run_tc(Args &a, const mocha_kv_pages *p, cudaStream_t s)
         !encode(&maps.k, p->type, a.k, {d, p->page_size, a.kv_heads, a.pages}, {a.ts * 2, a.hs * 2, a.ps * 2}, box, 1) ||
         !encode(&maps.v, p->type, a.v, {d, p->page_size, a.kv_heads, a.pages}, {a.ts * 2, a.hs * 2, a.ps * 2}, box, 1))
         return fail(who, "the tensor maps cannot be encoded");
-    const bool extra = a.cap > 0.f || a.slopes || !(a.scale > 0.f);
     const int ctas = mb::kSMs;
-    if (extra ? launch(who, k_prefill_tc<T, DP, true>, dim3(ctas), kTcThreads, SmemTc<DP>::kTiles + sizeof(TcBars), s, false, a, maps, tok, box, 4)
-              : launch(who, k_prefill_tc<T, DP, false>, dim3(ctas), kTcThreads, SmemTc<DP>::kTiles + sizeof(TcBars), s, false, a, maps, tok, box, 4))
-        return 1;
-    return launch(who, k_join<T, true>, dim3(4 * mb::kSMs), 32 * kJoinWarps, 0, s, true, a, ctas, 256, DP);
+    const auto go = [&](auto kernel, std::atomic<unsigned long long> &allowed) {
+        constexpr size_t smem = SmemTc<DP>::kTiles + sizeof(TcBars);
+        return allow_smem(who, kernel, smem, device, allowed) || launch(who, kernel, dim3(ctas), kTcThreads, smem, s, false, a, maps, tok, box, 2);
+    };
+    static std::atomic<unsigned long long> allowed[2] = {};
+    if (a.cap > 0.f || a.slopes || !(a.scale > 0.f) ? go(k_prefill_tc<T, DP, true>, allowed[1]) : go(k_prefill_tc<T, DP, false>, allowed[0])) return 1;
+    return launch(who, k_join<T, true>, dim3(kJoinBlocks), 32 * kJoinWarps, 0, s, true, a, ctas, 256, DP);
 }
 
 }  // namespace
@@ -1117,13 +1103,13 @@ extern "C" int mocha_kv_prefill(const mocha_kv_pages *pages, const mocha_kv_seqs
     if (!workspace || !aligned(workspace) || workspace_bytes < kv::prefill_workspace(pages->type, d))
         return fail(who, "workspace missing, not 16-byte aligned or smaller than mocha_kv_workspace says");
     const int ctas = kv::prefill_ctas(pages->type);
-    a.meta = static_cast<Meta *>(workspace);
-    a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + meta_bytes(ctas));
+    lay_out(a, workspace, ctas);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int dev = guard.device();
     const bool narrow = padded_dim(d) == 64;
     switch (pages->type) {
-    case MOCHA_KV_F32: return narrow ? run<float, 64>(a, ctas, s) : run<float, 128>(a, ctas, s);
-    case MOCHA_KV_F16: return narrow ? run_tc<__half, 64>(a, pages, s) : run_tc<__half, 128>(a, pages, s);
-    default: return narrow ? run_tc<__nv_bfloat16, 64>(a, pages, s) : run_tc<__nv_bfloat16, 128>(a, pages, s);
+    case MOCHA_KV_F32: return narrow ? run<float, 64>(a, ctas, dev, s) : run<float, 128>(a, ctas, dev, s);
+    case MOCHA_KV_F16: return narrow ? run_tc<__half, 64>(a, pages, dev, s) : run_tc<__half, 128>(a, pages, dev, s);
+    default: return narrow ? run_tc<__nv_bfloat16, 64>(a, pages, dev, s) : run_tc<__nv_bfloat16, 128>(a, pages, dev, s);
     }
 }

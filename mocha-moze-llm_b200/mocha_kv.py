@@ -71,9 +71,8 @@ def _load() -> C.CDLL:
     return _lib
 
 
-def _need(ok: bool, what: str):
-    if not ok:
-        raise ValueError(what)
+def _stream(device: int) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 class KvPages:
@@ -81,46 +80,55 @@ class KvPages:
     views) of one type, fp32, fp16 or bf16, with the same strides."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
-        _need(k.dim() == 4 and k.shape == v.shape, "k and v must be [pages, kv_heads, page_size, head_dim]")
-        _need(k.dtype in _TYPES and k.dtype == v.dtype, "k and v must be float32, float16 or bfloat16, of one type")
-        _need(k.stride() == v.stride() and k.stride(3) == 1, "k and v must have the same strides, the last one 1")
-        _need(k.device.type == "cuda" and k.device == v.device, "k and v must be on one CUDA device")
+        if k.dim() != 4 or k.shape != v.shape:
+            raise ValueError("k and v must be [pages, kv_heads, page_size, head_dim]")
+        if k.dtype not in _TYPES or k.dtype != v.dtype:
+            raise ValueError("k and v must be float32, float16 or bfloat16, of one type")
+        if k.stride() != v.stride() or k.stride(3) != 1:
+            raise ValueError("k and v must have the same strides, the last one 1")
+        if k.device.type != "cuda" or k.device != v.device:
+            raise ValueError("k and v must be on one CUDA device")
         self.k, self.v = k, v
         self.device, self.dtype = k.device, k.dtype
         self.kv_heads, self.page_size, self.head_dim = k.shape[1:]
-        self._p = _Pages(k.device.index, _TYPES[k.dtype], k.shape[0], k.shape[2], k.shape[1], k.shape[3], k.stride(0),
+        self._index = k.get_device()
+        self._p = _Pages(self._index, _TYPES[k.dtype], k.shape[0], k.shape[2], k.shape[1], k.shape[3], k.stride(0),
                          k.stride(1), k.stride(2), k.data_ptr(), v.data_ptr())
         self._pages = C.addressof(self._p)
         self._bytes = {}
 
-    # -- argument views -----------------------------------------------------------------
+    # -- argument views (messages are put together only when a check fails) --------------
 
-    def _int(self, t, name, n=None):
-        _need(t.dtype == torch.int32 and t.device == self.device and t.dim() == 1 and t.is_contiguous() and
-              (n is None or t.shape[0] == n),
-              f"{name} must be a contiguous int32 vector on the pages' device" + (f" of {n}" if n is not None else ""))
+    def _int(self, t, name, n):
+        if t.dtype is not torch.int32 or t.get_device() != self._index or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 vector of {n} on the pages' device")
         return t.data_ptr()
 
     def _seqs(self, table, kv_len, status):
-        _need(table.dim() == 2 and table.dtype == torch.int32 and table.device == self.device and
-              (table.shape[1] < 2 or table.stride(1) == 1),
-              "table must be an int32 matrix [seqs, pages of a sequence] on the pages' device")
-        n, width = table.shape
-        return _Seqs(n, width, max(table.stride(0), width) if n < 2 else table.stride(0), table.data_ptr(),
+        shape = table.shape
+        if (len(shape) != 2 or table.dtype is not torch.int32 or table.get_device() != self._index or
+                (shape[1] > 1 and table.stride(1) != 1)):
+            raise ValueError("table must be an int32 matrix [seqs, pages of a sequence] on the pages' device")
+        n, width = shape
+        return _Seqs(n, width, table.stride(0) if n > 1 else width, table.data_ptr(),
                      None if kv_len is None else self._int(kv_len, "kv_len", n),
                      None if status is None else self._int(status, "status", 1))
 
     def _rows(self, t, name, dtype, rows, heads=None):
-        _need(t.dim() == 3 and t.dtype == dtype and t.device == self.device and t.shape[0] == rows and
-              t.shape[2] == self.head_dim and t.stride(2) == 1 and (heads is None or t.shape[1] == heads),
-              f"{name} must be [{rows}, {heads or 'heads'}, {self.head_dim}] of {dtype} on the pages' device, "
-              "a head's values contiguous")
-        return _Rows(t.data_ptr(), t.stride(0) if rows > 1 else 0, t.stride(1) if t.shape[1] > 1 else self.head_dim)
+        shape = t.shape
+        if (len(shape) != 3 or t.dtype is not dtype or t.get_device() != self._index or shape[0] != rows or
+                shape[2] != self.head_dim or (heads is not None and shape[1] != heads)):
+            raise ValueError(f"{name} must be [{rows}, {heads or 'heads'}, {self.head_dim}] of {dtype} on the pages' device")
+        row, head, one = t.stride()
+        if one != 1:
+            raise ValueError(f"{name}: a head's values must be contiguous")
+        return _Rows(t.data_ptr(), row if rows > 1 else 0, head if shape[1] > 1 else self.head_dim)
 
     def _scores(self, heads, n, scale, window, prefix, cap, slopes):
         if slopes is not None:
-            _need(slopes.dtype == torch.float32 and slopes.device == self.device and slopes.is_contiguous() and
-                  slopes.shape == (heads,), f"slopes must be a contiguous float32 vector of {heads} on the pages' device")
+            if (slopes.dtype is not torch.float32 or slopes.get_device() != self._index or slopes.shape != (heads,) or
+                    not slopes.is_contiguous()):
+                raise ValueError(f"slopes must be a contiguous float32 vector of {heads} on the pages' device")
             slopes = slopes.data_ptr()
         return _Scores(heads, window, self.head_dim ** -0.5 if scale is None else scale, cap,
                        None if prefix is None else self._int(prefix, "prefix", n), slopes)
@@ -128,8 +136,9 @@ class KvPages:
     def _lse(self, lse, rows, heads):
         if lse is None:
             return None
-        _need(lse.dtype == torch.float32 and lse.device == self.device and lse.is_contiguous() and
-              lse.shape == (rows, heads), f"lse must be a contiguous float32 [{rows}, {heads}] on the pages' device")
+        if (lse.dtype is not torch.float32 or lse.get_device() != self._index or lse.shape != (rows, heads) or
+                not lse.is_contiguous()):
+            raise ValueError(f"lse must be a contiguous float32 [{rows}, {heads}] on the pages' device")
         return lse.data_ptr()
 
     def _space(self, lib, heads, prefill):
@@ -139,7 +148,7 @@ class KvPages:
             if lib.mocha_kv_workspace(self._pages, heads, prefill, C.byref(got)):
                 raise RuntimeError("mocha_kv_workspace failed")
             n = self._bytes[heads, prefill] = got.value
-        return torch.empty(n, dtype=torch.uint8, device=self.device)
+        return n, torch.empty(n, dtype=torch.uint8, device=self.device)
 
     # -- operators ----------------------------------------------------------------------
 
@@ -147,9 +156,10 @@ class KvPages:
         """Rotary positions on q [rows, heads, dim] (or None) and k [rows, kv_heads, dim], and k
         and v into the pages of (seq[i], pos[i]); rows with a negative seq are skipped.  cos and
         sin: [positions, rotated dims / 2] float32, or None for no rotation.  Returns q_out."""
-        lib = _load()
+        lib = _lib or _load()
         rows = k.shape[0]
-        _need(k.dtype in _TYPES, "k must be float32, float16 or bfloat16")
+        if k.dtype not in _TYPES:
+            raise ValueError("k must be float32, float16 or bfloat16")
         kr = self._rows(k, "k", k.dtype, rows, self.kv_heads)
         vr = self._rows(v, "v", k.dtype, rows, self.kv_heads)
         qr = orr = None
@@ -160,23 +170,25 @@ class KvPages:
             if q_out is None:
                 q_out = torch.empty(rows, heads, self.head_dim, dtype=self.dtype, device=self.device)
             orr = self._rows(q_out, "q_out", self.dtype, rows, heads)
-        else:
-            _need(q_out is None, "q_out without q")
-        _need((cos is None) == (sin is None), "cos and sin go together")
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        if (cos is None) != (sin is None):
+            raise ValueError("cos and sin go together")
         if cos is None:
             rope = _Rope(None, None, 0, 0, 0, 0)
         else:
-            _need(cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.dim() == 2 and
-                  cos.shape == sin.shape and cos.device == self.device and sin.device == self.device and
-                  cos.stride(1) == 1 and cos.stride() == sin.stride(),
-                  "cos and sin must be float32 [positions, rotated dims / 2] with the same strides on the pages' device")
+            if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.dim() != 2 or
+                    cos.shape != sin.shape or cos.get_device() != self._index or sin.get_device() != self._index or
+                    cos.stride() != sin.stride() or cos.stride(1) != 1):
+                raise ValueError("cos and sin must be float32 [positions, rotated dims / 2] with the same strides on "
+                                 "the pages' device")
             rope = _Rope(cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0], 2 * cos.shape[1],
                          int(bool(interleaved)))
         seqs = self._seqs(table, None, status)
         if lib.mocha_kv_append(self._pages, C.addressof(seqs), rows, self._int(seq, "seq", rows),
                                self._int(pos, "pos", rows), _TYPES[k.dtype], heads, qr and C.addressof(qr),
                                C.addressof(kr), C.addressof(vr), orr and C.addressof(orr), C.addressof(rope),
-                               torch.cuda.current_stream(self.device).cuda_stream):
+                               _stream(self._index)):
             raise RuntimeError("mocha_kv_append failed")
         return q_out
 
@@ -184,7 +196,7 @@ class KvPages:
                status=None):
         """Attention of q [seqs, heads, dim], the sequences' last positions; scale defaults to
         dim ** -0.5.  Returns out."""
-        lib = _load()
+        lib = _lib or _load()
         n = table.shape[0]
         qr = self._rows(q, "q", self.dtype, n)
         heads = q.shape[1]
@@ -193,10 +205,10 @@ class KvPages:
         orr = self._rows(out, "out", self.dtype, n, heads)
         seqs = self._seqs(table, kv_len, status)
         scores = self._scores(heads, n, scale, window, prefix, cap, slopes)
-        space = self._space(lib, heads, 0)
+        size, space = self._space(lib, heads, 0)
         if lib.mocha_kv_decode(self._pages, C.addressof(seqs), C.addressof(scores), C.addressof(qr), C.addressof(orr),
-                               self._lse(lse, n, heads), space.data_ptr(), space.numel(),
-                               torch.cuda.current_stream(self.device).cuda_stream):
+                               self._lse(lse, n, heads), space.data_ptr(), size,
+                               _stream(self._index)):
             raise RuntimeError("mocha_kv_decode failed")
         return out
 
@@ -204,7 +216,7 @@ class KvPages:
                 lse=None, status=None):
         """Attention of q [rows, heads, dim], rows q_start[s] .. q_start[s + 1] - 1 being the last
         positions of sequence s.  Rows outside every range are left as they were.  Returns out."""
-        lib = _load()
+        lib = _lib or _load()
         rows, n = q.shape[0], table.shape[0]
         qr = self._rows(q, "q", self.dtype, rows)
         heads = q.shape[1]
@@ -213,10 +225,10 @@ class KvPages:
         orr = self._rows(out, "out", self.dtype, rows, heads)
         seqs = self._seqs(table, kv_len, status)
         scores = self._scores(heads, n, scale, window, prefix, cap, slopes)
-        space = self._space(lib, heads, 1)
+        size, space = self._space(lib, heads, 1)
         if lib.mocha_kv_prefill(self._pages, C.addressof(seqs), C.addressof(scores), rows,
                                 self._int(q_start, "q_start", n + 1), C.addressof(qr), C.addressof(orr),
-                                self._lse(lse, rows, heads), space.data_ptr(), space.numel(),
-                                torch.cuda.current_stream(self.device).cuda_stream):
+                                self._lse(lse, rows, heads), space.data_ptr(), size,
+                                _stream(self._index)):
             raise RuntimeError("mocha_kv_prefill failed")
         return out
