@@ -143,6 +143,24 @@ typedef struct mocha_q8b mocha_q8b;
 int mocha_q8b_open(int device, const void *file, unsigned long long bytes, int max_rows, int slots, mocha_q8b **out);
 int mocha_q8b_close(mocha_q8b *h);
 
+/* mocha_q8b_open with a paged KV cache (mocha_kv.h) in place of the slots' fixed 1024
+ * positions: `pages` pages of `page_size` positions (a multiple of 8), shared by all slots,
+ * of kv_type MOCHA_KV_F32, MOCHA_KV_F16 or MOCHA_KV_BF16 (queries and keys are rounded to
+ * it after their rotation, attention outputs too).  A page holds a position's keys and
+ * values of every layer: 2 * 24 * 2 * 64 values, 12,288 bytes a position in bf16 against
+ * the fixed cache's 49,152 with its shadows.  Every function of the handle works as on a
+ * fixed cache.  mocha_q8b_forward and mocha_q8b_prefill take pages as positions need them
+ * and fail when none are left; position 0 of a slot starts the slot's pages anew.
+ * mocha_q8b_generate* begin with all pages free, admit a sequence when the pages for its
+ * prompt and its token budget are free and return them when it ends; they fail when one
+ * sequence alone needs more than there are. */
+int mocha_q8b_open_paged(int device, const void *file, unsigned long long bytes, int max_rows, int slots, int kv_type,
+                         int page_size, int pages, mocha_q8b **out);
+/* Pages that no slot holds; -1 on a handle with a fixed cache. */
+int mocha_q8b_free_pages(mocha_q8b *h);
+/* Returns a slot's pages.  On a fixed cache it does nothing. */
+int mocha_q8b_release(mocha_q8b *h, int slot);
+
 /* One forward over n rows: row i runs tokens[i] at position pos[i] of KV slot
  * slots[i] (keys 0..pos[i] of that slot must already hold earlier positions; rows of
  * one slot run in increasing position order within the call).  Logits of the

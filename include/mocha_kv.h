@@ -40,8 +40,9 @@ typedef struct {
 /* The sequences.  table[s * table_stride + i], i < table_width, is the page of positions
  * [i * page_size, (i + 1) * page_size) of sequence s; entries of positions that no call
  * needs are not used.  A needed page id outside [0, pages) reads as a page of zeros and is
- * not written.  Where `status` is not NULL, *status becomes 1 when such a page, or an
- * append position that the table or the angles do not hold, was met (it is never reset). */
+ * not written.  Where `status` is not NULL, *status becomes at least 1 when such a page, or
+ * an append position that the table or the angles do not hold, was met, and 2 when a
+ * bounded wait inside a kernel ran out, which leaves outputs unwritten (it is never reset). */
 typedef struct {
     int seqs, table_width;
     long long table_stride;

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256) k_append(const __grid_constant__ Append a
     const int s = __ldg(a.seq + row), p = __ldg(a.pos + row);
     if (s < 0 || s >= a.seqs || p < 0) return;
     if (p >= a.max_len || (a.rot_chunks && p >= a.positions)) {
-        if (a.status) *a.status = 1;
+        if (a.status) atomicMax(a.status, 1);
         return;
     }
     int head = div(a.chunk_div, item);
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(256) k_append(const __grid_constant__ Append a
         const uint32_t slot = div(a.page, p);
         const int page = __ldg(a.table + s * a.table_stride + slot);
         if ((unsigned)page >= (unsigned)a.pages) {
-            if (a.status) *a.status = 1;
+            if (a.status) atomicMax(a.status, 1);
             return;
         }
         src = key ? reinterpret_cast<const TI *>(a.k) + row * a.k_row + head * a.k_head

@@ -115,7 +115,7 @@ MB_DEV int page_of(const Args &a, int seq, int j)
 {
     const int id = __ldg(a.table + (long long)seq * a.table_stride + div(a.page, (uint32_t)j));
     if ((unsigned)id < (unsigned)a.pages) return id;
-    if (a.status) *a.status = 1;
+    if (a.status) atomicMax(a.status, 1);
     return -1;
 }
 

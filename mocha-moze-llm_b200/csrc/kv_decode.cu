@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
                     cp_async16(group + to_lane[y] + R::kHalf, from + v_off);
                 }
             } else {
-                if (!good && jg < in.len && a.status && (in.sees(jg) || in.sees(min(jg + 7, in.len - 1)))) *a.status = 1;
+                if (!good && jg < in.len && a.status && (in.sees(jg) || in.sees(min(jg + 7, in.len - 1)))) atomicMax(a.status, 1);
 #pragma unroll
                 for (int y = 0; y < 8 / RPI; y++, from += row_step) {
                     const bool use = good && dims && in.sees(jg + r0 + RPI * y);

@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // swizzled tiles are laid out by address: their base has to be a multiple of 1024
     const bool any = find_share<kTcKeys, kTcThreads>(a, tokens, min_tiles, share), placed = (smem_u32(smem) & 1023) == 0;
     if (!any || !placed) {
-        if (!placed && tid == 0 && a.status) *a.status = 2;
+        if (!placed && tid == 0 && a.status) atomicMax(a.status, 2);
         if (tid == 0) a.note[blockIdx.x].x = -1;
         return;
     }
@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             bool seen = false;
                             for (int y = 0; y < box && j + y < u.p.len; y++)
                                 seen |= (j + y <= pb && (a.window == 0 || pa - (j + y) < a.window)) || j + y < u.p.pre;
-                            if (seen) *a.status = 1;
+                            if (seen) atomicMax(a.status, 1);
                         }
                         for (int c = 0; c < DP / 64; c++)
                             tma_load_4d(dst + c * (128 * 128) + b * box * 128, v ? &maps.v : &maps.k, 64 * c, j - (int)(slot * a.page.d), u.kvh, id, full);
@@ -963,7 +963,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // a wait ran out: no notes for the join, and the copies in flight land first
         if (tid == 0) {
             a.note[blockIdx.x].x = -1;
-            if (a.status) *a.status = 2;
+            if (a.status) atomicMax(a.status, 2);
             const long long t0 = clock64();
             while (clock64() - t0 < kWaitCycles / 64) {
             }

@@ -32,6 +32,7 @@
 
 #include "mb_common.cuh"
 #include "mocha_b200.h"
+#include "mocha_kv.h"
 #include "q8_decode.cuh"
 #include "q8_layout.h"
 #include "sampling.cuh"
@@ -1064,6 +1065,39 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_bs_stage2(const unsigned lon
     }
 }
 
+// ---- paged KV cache -------------------------------------------------------------------
+
+// q | k | v of a row: sum of the GEMM's partials + bias, for mocha_kv_append.
+__global__ void __launch_bounds__(QKV_ROWS / 4) k_qkv_sum(const float *__restrict__ part, int splits, long long sstride,
+                                                          const float *__restrict__ bias, float *out)
+{
+    pdl_enter();
+    const int i0 = threadIdx.x * 4;
+    const float4 v = sum_splits4<8>(part + (size_t)blockIdx.x * QKV_ROWS + i0, splits, sstride);
+    const float4 b = __ldg(reinterpret_cast<const float4 *>(bias + i0));
+    *reinterpret_cast<float4 *>(out + (size_t)blockIdx.x * QKV_ROWS + i0) = f4add(v, b);
+}
+
+// Attention outputs as limbs for the O GEMM (16 lanes hold one head, one 64-group).
+template <typename T>
+__global__ void __launch_bounds__(NT) k_attn_limbs(const T *__restrict__ att, Limbs out)
+{
+    pdl_enter();
+    const int t = blockIdx.x, i0 = threadIdx.x * 4;
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = (float)att[(size_t)t * DIM + i0 + j];
+    mb::tq::store_limbs<4, 16>(v, out.q + (size_t)t * 3 * DIM, DIM, i0, out.s + (size_t)t * (DIM / GROUP) + i0 / GROUP,
+                               threadIdx.x & 15);
+}
+
+// A decode step's lengths: row i holds position pos[i].
+__global__ void k_lengths(const int *__restrict__ pos, int n, int *kv_len)
+{
+    pdl_enter();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) kv_len[i] = pos[i] + 1;
+}
+
 // ---- engine -------------------------------------------------------------------------
 
 // A grouped-Q8 matrix for the int8 GEMM: int8 [rows][cols] and fp32 scales [rows][cols/64].
@@ -1080,8 +1114,45 @@ struct PlanSet {
 
 }  // namespace qb
 
+// The paged cache of a handle: pools of all layers, the slots' pages (one id names a page
+// of every layer's pool), and one call's rows as the paged operators take them.  A call's
+// sequences are its runs of rows of one slot at consecutive positions.
+struct Paged {
+    int type = 0, page_size = 0, pages = 0, width = 0;  // width: pages of a slot's 1024 positions
+    size_t item = 0;
+    unsigned char *k = nullptr, *v = nullptr;           // [LAYERS][pages][KV_HEADS][page_size][64]
+    float *qkv = nullptr;                               // [max_rows][1152]
+    unsigned char *q = nullptr, *att = nullptr;         // [max_rows][896]
+    int *seq = nullptr, *start = nullptr, *len = nullptr, *table = nullptr;  // prompt calls: [max_rows], + 1, , [max_rows][width]
+    int *dec_len = nullptr, *dec_table = nullptr;       // decode steps: [slots], [slots][width]; row = sequence = slot
+    int *status = nullptr;
+    void *space[2] = {nullptr, nullptr};                // of decode and prefill
+    unsigned long long space_bytes[2] = {0, 0};
+    int seqs = 0;                                       // of the prompt call; single: each has one row
+    bool single = false;
+    std::vector<int> free;
+    std::vector<std::vector<int>> held;                 // [slots]
+
+    void release(int slot)
+    {
+        free.insert(free.end(), held[slot].rbegin(), held[slot].rend());
+        held[slot].clear();
+    }
+    bool reserve(int slot, int positions)  // pages for the slot's first `positions`
+    {
+        const int need = (positions + page_size - 1) / page_size;
+        if ((int)held[slot].size() + (int)free.size() < need) return false;
+        while ((int)held[slot].size() < need) {
+            held[slot].push_back(free.back());
+            free.pop_back();
+        }
+        return true;
+    }
+};
+
 struct mocha_q8b {
     int device = 0, max_rows = 0, slots = 0;
+    Paged *paged = nullptr;
     cudaStream_t stream = nullptr;
     unsigned char *d_file = nullptr;
     q8::Model m{};
@@ -1142,6 +1213,14 @@ int check_err(mocha_q8b *h)
     if (e) {
         fprintf(stderr, "mocha_q8b: device-side wait gave up (code %d)\n", e);
         return 1;
+    }
+    if (h->paged) {
+        // 1, a position without a page, is ordinary: a finished sequence's row runs on until it is harvested
+        QB_TRY(cudaMemcpy(&e, h->paged->status, sizeof(int), cudaMemcpyDeviceToHost));
+        if (e > 1) {
+            fprintf(stderr, "mocha_q8b: a wait of the paged attention gave up\n");
+            return 1;
+        }
     }
     return 0;
 }
@@ -1251,6 +1330,82 @@ int enqueue_attention(mocha_q8b *h, Rows rows, int n, int layer, int block, int 
                layer, h->la);
 }
 
+// The paged path from the QKV sums to the O GEMM's input: rotation and page writes, then
+// single-token attention when every sequence of the call has one row, prompt attention
+// else.  graph_step: rows 0..n-1 are the slots' decode rows, sequence = row.
+int enqueue_paged_attention(mocha_q8b *h, Rows rows, int n, int layer, bool graph_step)
+{
+    Paged &g = *h->paged;
+    const size_t at = (size_t)layer * g.pages * KV_HEADS * g.page_size * HEAD_DIM * g.item;
+    const mocha_kv_pages pages{h->device, g.type, g.pages, g.page_size, KV_HEADS, HEAD_DIM,
+                               (long long)KV_HEADS * g.page_size * HEAD_DIM, (long long)g.page_size * HEAD_DIM, HEAD_DIM,
+                               g.k + at, g.v + at};
+    const mocha_kv_seqs seqs{graph_step ? n : g.seqs, g.width, g.width, graph_step ? g.dec_table : g.table,
+                             graph_step ? g.dec_len : g.len, g.status};
+    const mocha_kv_rope rope{h->rope_cos, h->rope_sin, HEAD_DIM / 2, CONTEXT, HEAD_DIM, 0};
+    const mocha_kv_rows q{g.qkv, QKV_ROWS, HEAD_DIM}, k{g.qkv + DIM, QKV_ROWS, HEAD_DIM}, v{g.qkv + DIM + KV, QKV_ROWS, HEAD_DIM};
+    const mocha_kv_rows qr{g.q, DIM, HEAD_DIM}, att{g.att, DIM, HEAD_DIM};
+    const mocha_kv_scores scores{HEADS, 0, 0.125f, 0.f, nullptr, nullptr};
+    if (mocha_kv_append(&pages, &seqs, n, graph_step ? h->ident : g.seq, rows.pos, MOCHA_KV_F32, HEADS, &q, &k, &v, &qr, &rope,
+                        h->stream))
+        return 1;
+    if (graph_step || g.single
+            ? mocha_kv_decode(&pages, &seqs, &scores, &qr, &att, nullptr, g.space[0], g.space_bytes[0], h->stream)
+            : mocha_kv_prefill(&pages, &seqs, &scores, n, g.start, &qr, &att, nullptr, g.space[1], g.space_bytes[1], h->stream))
+        return 1;
+    return g.type == MOCHA_KV_F32   ? pdl(k_attn_limbs<float>, n, NT, 0, h->stream, (const float *)g.att, h->la)
+           : g.type == MOCHA_KV_F16 ? pdl(k_attn_limbs<__half>, n, NT, 0, h->stream, (const __half *)g.att, h->la)
+                                    : pdl(k_attn_limbs<bf16>, n, NT, 0, h->stream, (const bf16 *)g.att, h->la);
+}
+
+// Takes the pages that rows (host arrays) need and hands the rows' sequences to the device.
+// A no-op on a fixed cache.
+int paged_rows(mocha_q8b *h, int n, const int *pos, const int *slots, bool reserved = false)
+{
+    if (!h->paged) return 0;
+    Paged &g = *h->paged;
+    for (int i = 0; i < n && !reserved; i++)
+        if (pos[i] == 0) g.release(slots[i]);
+    for (int i = 0; i < n; i++)
+        if (!g.reserve(slots[i], pos[i] + 1)) {
+            fprintf(stderr, "mocha_q8b: out of KV pages (%d of %d positions)\n", g.pages, g.page_size);
+            return 1;
+        }
+    std::vector<int> seq(n), start, len, table;
+    for (int i = 0; i < n; i++) {
+        if (i == 0 || slots[i] != slots[i - 1] || pos[i] != pos[i - 1] + 1) {
+            start.push_back(i);
+            len.push_back(0);
+            std::vector<int> row(g.held[slots[i]]);
+            row.resize(g.width, -1);
+            table.insert(table.end(), row.begin(), row.end());
+        }
+        seq[i] = (int)start.size() - 1;
+        len.back() = pos[i] + 1;
+    }
+    g.seqs = (int)start.size();
+    g.single = g.seqs == n;
+    start.push_back(n);
+    QB_TRY(cudaMemcpyAsync(g.seq, seq.data(), sizeof(int) * n, cudaMemcpyHostToDevice, h->stream));
+    QB_TRY(cudaMemcpyAsync(g.start, start.data(), sizeof(int) * start.size(), cudaMemcpyHostToDevice, h->stream));
+    QB_TRY(cudaMemcpyAsync(g.len, len.data(), sizeof(int) * len.size(), cudaMemcpyHostToDevice, h->stream));
+    QB_TRY(cudaMemcpyAsync(g.table, table.data(), sizeof(int) * table.size(), cudaMemcpyHostToDevice, h->stream));
+    QB_TRY(cudaStreamSynchronize(h->stream));  // the vectors end here
+    return 0;
+}
+
+// The slots' page tables for decode steps.
+int paged_tables(mocha_q8b *h)
+{
+    if (!h->paged) return 0;
+    Paged &g = *h->paged;
+    std::vector<int> table((size_t)h->slots * g.width, -1);
+    for (int i = 0; i < h->slots; i++) std::copy(g.held[i].begin(), g.held[i].end(), table.begin() + (size_t)i * g.width);
+    QB_TRY(cudaMemcpyAsync(g.dec_table, table.data(), sizeof(int) * table.size(), cudaMemcpyHostToDevice, h->stream));
+    QB_TRY(cudaStreamSynchronize(h->stream));
+    return 0;
+}
+
 // Attention kernel for rows (host arrays): 2 when every block of 128 rows is one slot
 // at consecutive positions from a multiple of 128 (tensor cores), 1 for blocks of 64
 // (CUDA cores), else one CTA per (KV head, row): ATTN_ROWS_POST (QKV post-processing
@@ -1280,16 +1435,22 @@ int block_kind(int n, const int *pos, const int *slots)
 // The whole transformer for rows [0, n) plus the head for `np` projected rows
 // (proj_dst maps row -> head row or -1; the head reads rows 0..np-1 of the head limbs).
 int enqueue_forward(mocha_q8b *h, Rows rows, int n, bool decode_set, const int *proj_dst, int np,
-                    int block_attention, int max_pos)
+                    int block_attention, int max_pos, bool graph_step = false)
 {
     const PlanSet &ps = decode_set ? h->dec : h->pre;
     cudaStream_t s = h->stream;
+    if (h->paged && graph_step && pdl(k_lengths, 1, 256, 0, s, rows.pos, n, h->paged->dec_len)) return 1;
     if (pdl(k_embed_norm, n, NT, 0, s, h->m.embed, rows, h->m.layer[0].attn_norm, h->x, h->lx)) return 1;
     mb::tc::Split sp;
     for (int l = 0; l < LAYERS; l++) {
         const Layer &L = h->m.layer[l];
         if (mb::tq::launch(ps.qkv[l], n, s, &sp)) return 1;
-        if (block_attention == ATTN_ROWS_POST) {
+        if (h->paged) {
+            if (pdl(k_qkv_sum, n, QKV_ROWS / 4, 0, s, h->part, sp.splits, sp.split_stride, h->bqkv + (size_t)l * QKV_ROWS,
+                    h->paged->qkv) ||
+                enqueue_paged_attention(h, rows, n, l, graph_step))
+                return 1;
+        } else if (block_attention == ATTN_ROWS_POST) {
             // rows of distinct slots: QKV post-processing fused into the row attention
             const QkvPost pp{h->part, sp.splits, sp.split_stride, h->bqkv + (size_t)l * QKV_ROWS, h->rope_cos,
                              h->rope_sin, h->kvs};
@@ -1381,7 +1542,7 @@ int capture_step(mocha_q8b *h, int n)
     cudaGraph_t g;
     QB_TRY(cudaStreamBeginCapture(h->stream, cudaStreamCaptureModeThreadLocal));
     const Rows r{h->ntok, h->npos, h->nslot};
-    int rc = enqueue_forward(h, r, n, true, h->ident, n, ATTN_ROWS_POST, CONTEXT - 1);  // one row per slot
+    int rc = enqueue_forward(h, r, n, true, h->ident, n, ATTN_ROWS_POST, CONTEXT - 1, true);  // one row per slot
     if (!rc) rc = enqueue_sample(h, r, n, h->ident);
     const cudaError_t e = cudaStreamEndCapture(h->stream, &g);
     if (rc || e != cudaSuccess) {
@@ -1399,8 +1560,11 @@ int capture_step(mocha_q8b *h, int n)
 
 using namespace qb;
 
-extern "C" int mocha_q8b_open(int device, const void *file, unsigned long long bytes, int max_rows, int slots,
-                              mocha_q8b **out)
+namespace {
+
+// kv_type < 0: the fixed cache.
+int open_engine(int device, const void *file, unsigned long long bytes, int max_rows, int slots, int kv_type, int page_size,
+                int pages, mocha_q8b **out)
 {
     if (!out || !q8::valid_file(file, (size_t)bytes, false) || max_rows < 1 || max_rows > 16384 || slots < 1 ||
         slots > 256) {
@@ -1474,7 +1638,7 @@ extern "C" int mocha_q8b_open(int device, const void *file, unsigned long long b
     if (dalloc(&h->x, R * DIM) || dalloc(&h->q, R * DIM) || dalloc(&h->lx.q, 3 * R * DIM) ||
         dalloc(&h->lx.s, R * (DIM / GROUP)) || dalloc(&h->la.q, 3 * R * DIM) || dalloc(&h->la.s, R * (DIM / GROUP)) ||
         dalloc(&h->lhq, 3 * R * HIDDEN) || dalloc(&h->lhs, R * (HIDDEN / GROUP)) ||
-        dalloc(&h->apart, R * HEADS * NCHUNK * PART) || dalloc(&h->lhead.q, 3 * (size_t)slots * DIM) ||
+        dalloc(&h->apart, kv_type >= 0 ? 64 : R * HEADS * NCHUNK * PART) || dalloc(&h->lhead.q, 3 * (size_t)slots * DIM) ||
         dalloc(&h->lhead.s, (size_t)slots * (DIM / GROUP)) ||
         dalloc(&h->logits, (size_t)slots * VOCAB) || dalloc(&h->tok, R) || dalloc(&h->pos, R) ||
         dalloc(&h->slot, R) || dalloc(&h->ntok, slots) || dalloc(&h->npos, slots) || dalloc(&h->nslot, slots) ||
@@ -1482,18 +1646,39 @@ extern "C" int mocha_q8b_open(int device, const void *file, unsigned long long b
         dalloc(&h->keys, (size_t)slots * NSLICE * sampling::kMaxK) || dalloc(&h->st, slots) ||
         dalloc(&h->params, 1) || dalloc(&h->out_count, slots))
         return fail();
-    const size_t kv = kv_off(slots, 0, 0, 0);
+    if (kv_type >= 0) {
+        Paged &g = *(h->paged = new Paged());
+        g.type = kv_type;
+        g.item = kv_type == MOCHA_KV_F32 ? 4 : 2;
+        g.page_size = page_size;
+        g.pages = pages;
+        g.width = (CONTEXT + page_size - 1) / page_size;
+        g.held.resize(slots);
+        const size_t pool = (size_t)LAYERS * pages * KV_HEADS * page_size * HEAD_DIM * g.item;
+        const mocha_kv_pages one{device, kv_type, pages, page_size, KV_HEADS, HEAD_DIM, (long long)KV_HEADS * page_size * HEAD_DIM,
+                                 (long long)page_size * HEAD_DIM, HEAD_DIM, (void *)256, (void *)256};
+        if (mocha_kv_workspace(&one, HEADS, 0, &g.space_bytes[0]) || mocha_kv_workspace(&one, HEADS, 1, &g.space_bytes[1]) ||
+            dalloc(&g.k, pool) || dalloc(&g.v, pool) || dalloc(&g.qkv, R * QKV_ROWS) || dalloc(&g.q, R * DIM * g.item) ||
+            dalloc(&g.att, R * DIM * g.item) || dalloc(&g.seq, R) || dalloc(&g.start, R + 1) || dalloc(&g.len, R) ||
+            dalloc(&g.table, R * g.width) || dalloc(&g.dec_len, slots) || dalloc(&g.dec_table, (size_t)slots * g.width) ||
+            dalloc(&g.status, 1) || dalloc((unsigned char **)&g.space[0], g.space_bytes[0]) ||
+            dalloc((unsigned char **)&g.space[1], g.space_bytes[1]) || cudaMemset(g.status, 0, sizeof(int)))
+            return fail();
+        for (int i = pages - 1; i >= 0; i--) g.free.push_back(i);
+    }
+    const size_t kv = h->paged ? 64 : kv_off(slots, 0, 0, 0);
     if (dalloc(&h->kc, kv) || dalloc(&h->vc, kv) || dalloc(&h->kvs.k_hi, kv) || dalloc(&h->kvs.k_lo, kv) ||
         dalloc(&h->kvs.vt_hi, kv) || dalloc(&h->kvs.vt_lo, kv))
         return fail();
-    if (mb::tc::make_map_bf16(&h->amaps.k_hi, h->kvs.k_hi, (long long)slots * LAYERS * KV_HEADS * CONTEXT, HEAD_DIM,
+    if (!h->paged &&
+        (mb::tc::make_map_bf16(&h->amaps.k_hi, h->kvs.k_hi, (long long)slots * LAYERS * KV_HEADS * CONTEXT, HEAD_DIM,
                               TK) ||
         mb::tc::make_map_bf16(&h->amaps.k_lo, h->kvs.k_lo, (long long)slots * LAYERS * KV_HEADS * CONTEXT, HEAD_DIM,
                               TK) ||
         mb::tc::make_map_bf16(&h->amaps.vt_hi, h->kvs.vt_hi, (long long)slots * LAYERS * KV_HEADS * HEAD_DIM, CONTEXT,
                               HEAD_DIM) ||
         mb::tc::make_map_bf16(&h->amaps.vt_lo, h->kvs.vt_lo, (long long)slots * LAYERS * KV_HEADS * HEAD_DIM, CONTEXT,
-                              HEAD_DIM))
+                              HEAD_DIM)))
         return fail();
     if (cudaMemset(h->kc, 0, sizeof(float) * kv) || cudaMemset(h->vc, 0, sizeof(float) * kv) ||
         cudaMemset(h->err, 0, sizeof(int)) || cudaMemset(h->out_count, 0, sizeof(int) * slots) ||
@@ -1532,6 +1717,37 @@ extern "C" int mocha_q8b_open(int device, const void *file, unsigned long long b
     return 0;
 }
 
+}  // namespace
+
+extern "C" int mocha_q8b_open(int device, const void *file, unsigned long long bytes, int max_rows, int slots,
+                              mocha_q8b **out)
+{
+    return open_engine(device, file, bytes, max_rows, slots, -1, 0, 0, out);
+}
+
+extern "C" int mocha_q8b_open_paged(int device, const void *file, unsigned long long bytes, int max_rows, int slots,
+                                    int kv_type, int page_size, int pages, mocha_q8b **out)
+{
+    if ((kv_type != MOCHA_KV_F32 && kv_type != MOCHA_KV_F16 && kv_type != MOCHA_KV_BF16) || page_size < 8 || page_size % 8 ||
+        page_size > CONTEXT || pages < 1 || (long long)pages * page_size > 1ll << 30) {
+        fprintf(stderr, "mocha_q8b_open_paged: kv_type must be a MOCHA_KV_* type, page_size a multiple of 8 up to %d, pages positive\n", CONTEXT);
+        return 1;
+    }
+    return open_engine(device, file, bytes, max_rows, slots, kv_type, page_size, pages, out);
+}
+
+extern "C" int mocha_q8b_free_pages(mocha_q8b *h) { return h && h->paged ? (int)h->paged->free.size() : -1; }
+
+extern "C" int mocha_q8b_release(mocha_q8b *h, int slot)
+{
+    if (!h || slot < 0 || slot >= h->slots) {
+        fprintf(stderr, "mocha_q8b_release: bad arguments\n");
+        return 1;
+    }
+    if (h->paged) h->paged->release(slot);
+    return 0;
+}
+
 extern "C" int mocha_q8b_close(mocha_q8b *h)
 {
     if (!h) return 1;
@@ -1545,6 +1761,13 @@ extern "C" int mocha_q8b_close(mocha_q8b *h)
                     h->err, h->keys, h->st, h->params, h->out_tokens, h->out_count};
     for (void *p : ptrs)
         if (p) cudaFree(p);
+    if (h->paged) {
+        Paged &g = *h->paged;
+        void *own[] = {g.k, g.v, g.qkv, g.q, g.att, g.seq, g.start, g.len, g.table, g.dec_len, g.dec_table, g.status, g.space[0], g.space[1]};
+        for (void *p : own)
+            if (p) cudaFree(p);
+        delete h->paged;
+    }
     for (int l = 0; l < LAYERS; l++)
         for (Weights *w : {&h->w_qkv[l], &h->w_o[l], &h->w_gu[l], &h->w_down[l]}) {
             if (w->own_q) cudaFree(w->own_q);
@@ -1571,7 +1794,8 @@ extern "C" int mocha_q8b_forward(mocha_q8b *h, int n, const int *tokens, const i
             return 1;
         }
     QB_TRY(cudaSetDevice(h->device));
-    if (upload_rows(h, n, tokens, pos, slots) || set_projection(h, n, n_project, project_rows)) return 1;
+    if (paged_rows(h, n, pos, slots) || upload_rows(h, n, tokens, pos, slots) || set_projection(h, n, n_project, project_rows))
+        return 1;
     const Rows r{h->tok, h->pos, h->slot};
     int max_pos = 0;
     for (int i = 0; i < n; i++) max_pos = std::max(max_pos, pos[i]);
@@ -1614,6 +1838,13 @@ namespace {
 // prompt tokens, seed seed_base + sequence index (src/minimind.cpp:160-179).
 constexpr int kCheckEvery = 32;
 
+// Rows of sequences that have just been admitted with their pages.
+int paged_admitted(mocha_q8b *h, int n, const int *pos, const int *slots)
+{
+    if (!h->paged) return 0;
+    return paged_rows(h, n, pos, slots, true) || paged_tables(h);
+}
+
 int generate_impl(mocha_q8b *h, int nseq, const int *prompts, int prompt_len, const int *n_new, int max_new,
                   const mocha_sampling *sp, unsigned seed_base, int *out_tokens, int *out_counts, mocha_timing *timing)
 {
@@ -1635,6 +1866,13 @@ int generate_impl(mocha_q8b *h, int nseq, const int *prompts, int prompt_len, co
     sampling::Params prm{sp->repeat_penalty, sp->temperature, sp->top_k, sp->top_p, EOS, CONTROL_FIRST, VOCAB};
     QB_TRY(cudaMemcpyAsync(h->params, &prm, sizeof(prm), cudaMemcpyHostToDevice, h->stream));
     const int b = std::min(wave, nseq);        // slots stepped together
+    if (h->paged) {
+        for (int i = 0; i < h->slots; i++) h->paged->release(i);
+        // rows of slots that wait for pages run on token 0 at position 0 without any
+        QB_TRY(cudaMemsetAsync(h->ntok, 0, sizeof(int) * b, h->stream));
+        QB_TRY(cudaMemsetAsync(h->npos, 0, sizeof(int) * b, h->stream));
+        QB_TRY(cudaMemcpyAsync(h->nslot, h->ident, sizeof(int) * b, cudaMemcpyDeviceToDevice, h->stream));
+    }
     std::vector<int> seq_of(b, -1);             // sequence in each slot, -1 free
     std::vector<sampling::SeqState> st(b);
     std::vector<int> counts(b), row;
@@ -1647,6 +1885,7 @@ int generate_impl(mocha_q8b *h, int nseq, const int *prompts, int prompt_len, co
         std::vector<int> tok, pos, sl, src, idx;
         for (int i = 0; i < b && next < nseq; i++) {
             if (seq_of[i] >= 0) continue;
+            if (h->paged && !h->paged->reserve(i, prompt_len + n_new[next])) break;  // waits for pages
             const int q = next++;
             seq_of[i] = q;
             sampling::SeqState x;
@@ -1669,7 +1908,9 @@ int generate_impl(mocha_q8b *h, int nseq, const int *prompts, int prompt_len, co
         }
         if (src.empty()) return 0;
         const int n = (int)tok.size(), np = (int)src.size();
-        if (upload_rows(h, n, tok.data(), pos.data(), sl.data()) || set_projection(h, n, np, src.data())) return 1;
+        if (paged_admitted(h, n, pos.data(), sl.data()) || upload_rows(h, n, tok.data(), pos.data(), sl.data()) ||
+            set_projection(h, n, np, src.data()))
+            return 1;
         QB_TRY(cudaMemcpyAsync(h->next_index, idx.data(), sizeof(int) * np, cudaMemcpyHostToDevice, h->stream));
         QB_TRY(cudaEventRecord(h->ev[0], h->stream));
         const Rows pr{h->tok, h->pos, h->slot};
@@ -1690,6 +1931,7 @@ int generate_impl(mocha_q8b *h, int nseq, const int *prompts, int prompt_len, co
         QB_TRY(cudaMemcpy(st.data(), h->st, sizeof(sampling::SeqState) * b, cudaMemcpyDeviceToHost));
         if (check_err(h)) return 1;
         int run = kCheckEvery, active = 0;
+        bool harvested = false;
         for (int i = 0; i < b; i++) {
             const int q = seq_of[i];
             if (q < 0) continue;
@@ -1705,6 +1947,8 @@ int generate_impl(mocha_q8b *h, int nseq, const int *prompts, int prompt_len, co
                 out_counts[q] = kept;
                 generated += kept;
                 seq_of[i] = -1;
+                if (h->paged) h->paged->release(i);
+                harvested = true;
             } else {
                 active++;
                 run = std::min(run, n_new[q] - counts[i]);
@@ -1716,7 +1960,14 @@ int generate_impl(mocha_q8b *h, int nseq, const int *prompts, int prompt_len, co
             active += next - before;
             if (next > before) run = 1;  // look again once the new sequences have a token
         }
-        if (!active) break;
+        if (!active) {
+            if (next < nseq) {
+                fprintf(stderr, "mocha_q8b: a sequence needs more KV pages than there are\n");
+                return 1;
+            }
+            break;
+        }
+        if (harvested && paged_tables(h)) return 1;  // a harvested slot's row must not write to pages given on
         QB_TRY(cudaEventRecord(h->ev[2], h->stream));
         for (int k = 0; k < std::max(run, 1); k++) QB_TRY(cudaGraphLaunch(h->g_step, h->stream));
         QB_TRY(cudaEventRecord(h->ev[3], h->stream));
@@ -1774,6 +2025,7 @@ extern "C" int mocha_q8b_generate_each(mocha_q8b *h, int nseq, const int *prompt
 extern "C" int mocha_q8b_launches_per_step(mocha_q8b *h)
 {
     if (!h) return -1;
+    if (h->paged) return 2 + LAYERS * 12 + 1 + 2;  // lengths; attention is sums, append, two of the attention, limbs
     return 1 + LAYERS * 8 + 1 + 2;  // embed+norm, 8 per layer, head GEMM, two sampler kernels
 }
 
@@ -1838,7 +2090,9 @@ extern "C" int mocha_q8b_bench_prefill(mocha_q8b *h, int n, unsigned seed, int w
         pos[i] = i;
     }
     const int last = n - 1;
-    if (upload_rows(h, n, tok.data(), pos.data(), sl.data()) || set_projection(h, n, 1, &last)) return 1;
+    if (paged_rows(h, n, pos.data(), sl.data()) || upload_rows(h, n, tok.data(), pos.data(), sl.data()) ||
+        set_projection(h, n, 1, &last))
+        return 1;
     const Rows r{h->tok, h->pos, h->slot};
     const int block = n % TQ == 0 ? 2 : (n % QB == 0 ? 1 : 0);
     for (int i = 0; i < warmup; i++)

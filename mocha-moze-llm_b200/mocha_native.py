@@ -73,6 +73,10 @@ _SIGS = {
     "mocha_gguf_launches_per_step": (C.c_int, [C.c_void_p]),
     "mocha_q8_counters": (C.c_int, [C.c_void_p, C.POINTER(C.c_ulonglong), C.POINTER(C.c_ulonglong)]),
     "mocha_q8b_open": (C.c_int, [C.c_int, C.c_void_p, C.c_ulonglong, C.c_int, C.c_int, C.POINTER(C.c_void_p)]),
+    "mocha_q8b_open_paged": (C.c_int, [C.c_int, C.c_void_p, C.c_ulonglong, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                       C.POINTER(C.c_void_p)]),
+    "mocha_q8b_free_pages": (C.c_int, [C.c_void_p]),
+    "mocha_q8b_release": (C.c_int, [C.c_void_p, C.c_int]),
     "mocha_q8b_close": (C.c_int, [C.c_void_p]),
     "mocha_q8b_forward": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
                                     C.c_void_p]),
@@ -254,17 +258,26 @@ def _addr(buf):
 
 class Q8BatchHandle:
     """The batched grouped-Q8 engine on one device (mocha_q8b handle): tcgen05 GEMMs
-    over rows of (token, position, KV slot)."""
+    over rows of (token, position, KV slot).  With kv_type ("f32", "f16" or "bf16") the
+    slots share `pages` pages of page_size positions (default: enough for all slots)."""
 
     VOCAB = 151936
+    KV_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
 
-    def __init__(self, device: int, file_bytes, max_rows: int = 1024, slots: int = 64, lib: C.CDLL | None = None):
+    def __init__(self, device: int, file_bytes, max_rows: int = 1024, slots: int = 64, lib: C.CDLL | None = None,
+                 kv_type: str | None = None, page_size: int = 16, pages: int | None = None):
         import numpy as np
         self.lib = lib or load()
         self._file = np.ascontiguousarray(file_bytes, dtype=np.uint8)
         h = C.c_void_p()
-        if self.lib.mocha_q8b_open(device, self._file.ctypes.data, self._file.nbytes, max_rows, slots, C.byref(h)):
-            raise RuntimeError("mocha_q8b_open failed")
+        if kv_type is None:
+            if self.lib.mocha_q8b_open(device, self._file.ctypes.data, self._file.nbytes, max_rows, slots, C.byref(h)):
+                raise RuntimeError("mocha_q8b_open failed")
+        elif self.lib.mocha_q8b_open_paged(device, self._file.ctypes.data, self._file.nbytes, max_rows, slots,
+                                           self.KV_TYPES[kv_type], page_size,
+                                           -(-1024 // max(page_size, 1)) * slots if pages is None else pages,
+                                           C.byref(h)):
+            raise RuntimeError("mocha_q8b_open_paged failed")
         self.h = h
         self.slots = slots
         self.max_rows = max_rows
@@ -338,6 +351,14 @@ class Q8BatchHandle:
 
     def launches_per_step(self) -> int:
         return self.lib.mocha_q8b_launches_per_step(self.h)
+
+    def free_pages(self) -> int:
+        """Pages that no slot holds; -1 with a fixed cache."""
+        return self.lib.mocha_q8b_free_pages(self.h)
+
+    def release(self, slot: int):
+        if self.lib.mocha_q8b_release(self.h, slot):
+            raise RuntimeError("mocha_q8b_release failed")
 
     def sample(self, logits, histories, temperature, top_k, top_p, penalty, seeds):
         import numpy as np

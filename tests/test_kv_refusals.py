@@ -131,3 +131,11 @@ def test_workspace(kv):
                 p = pages(kv, type=t, head_dim=d, token_stride=128, head_stride=2048, page_stride=4096)
                 assert lib.mocha_kv_workspace(*refs(p), 28, prefill, C.byref(got)) == 0
                 assert 0 < got.value < 64 << 20 and got.value % 8 == 0
+
+
+@pytest.mark.parametrize("kv_type,page_size,pages", [(3, 16, 10), (-1, 16, 10), (2, 12, 10), (2, 0, 10), (2, 2048, 10), (2, 16, 0),
+                                                    (2, 16, 2 ** 31 - 1)])
+def test_open_paged(native, capfd, kv_type, page_size, pages):
+    out = C.c_void_p()
+    assert native.load().mocha_q8b_open_paged(0, None, 0, 64, 2, kv_type, page_size, pages, C.byref(out)) == 1
+    assert "mocha_q8b_open_paged" in capfd.readouterr().err
