@@ -219,6 +219,23 @@ __device__ __forceinline__ void lone_row(const Args &a, int seq, int p, int head
     if (a.lse && lane == 0) a.lse[(long long)row * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
+// ---- asynchronous copies ----------------------------------------------------------------
+
+MB_DEV void cp_async16(uint32_t dst, const void *src, bool ok)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+MB_DEV void cp_async16(uint32_t dst, const void *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+MB_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+MB_DEV void cp_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // ---- join of the parts of cut units --------------------------------------------------
 // The rows of all cut units are dealt to the blocks: a warp takes a row whose parts are
 // few, a block one whose parts are many (more than kJoinSerial), lanes the dims.  Bound by

@@ -94,21 +94,6 @@ struct Walk {
     MB_DEV bool sees(int k) const { return k < len && (k >= lo || k < pre); }
 };
 
-MB_DEV void cp_async16(uint32_t dst, const void *src, bool ok)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
-MB_DEV void cp_async16(uint32_t dst, const void *src)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-MB_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-MB_DEV void cp_wait()
-{
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 MB_DEV void ldsm4(uint32_t addr, uint32_t (&r)[4])
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"

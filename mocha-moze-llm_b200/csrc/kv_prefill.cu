@@ -161,22 +161,15 @@ struct Smem32 {
     static constexpr int kRow = DP + 4;  // floats; 16 bytes on from line to line: no bank conflicts down a column
     static constexpr int kPRow = kKeys + 4;
     static constexpr int kTotal = (kRows + 2 * kKeys) * kRow * 4 + kRows * kPRow * 4;
+    static constexpr int kCtas = DP == 64 ? 2 : 1;  // of an SM
 };
 
-template <typename T>
-MB_DEV float4 load4(const T *p)
-{
-    if constexpr (sizeof(T) == 4) return *reinterpret_cast<const float4 *>(p);
-    const uint2 u = *reinterpret_cast<const uint2 *>(p);
-    const T *t = reinterpret_cast<const T *>(&u);
-    return make_float4(to_f32(t[0]), to_f32(t[1]), to_f32(t[2]), to_f32(t[3]));
-}
-
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) k_prefill(const __grid_constant__ Args a, int tokens, int min_tiles)
+template <int DP>
+__global__ void __launch_bounds__(kThreads, Smem32<DP>::kCtas) k_prefill(const __grid_constant__ Args a, int tokens, int min_tiles)
 {
     using S = Smem32<DP>;
     extern __shared__ __align__(16) float sm[];
+    constexpr int kCopies = kKeys * (DP / 4) / kThreads;  // 16-byte copies of a thread for a tile
     float *sq = sm, *sk = sq + kRows * S::kRow, *sv = sk + kKeys * S::kRow, *sp = sv + kKeys * S::kRow;
     __shared__ ShareSmem share;
     __shared__ unsigned char s_bad[kRows];
@@ -195,13 +188,12 @@ __global__ void __launch_bounds__(kThreads) k_prefill(const __grid_constant__ Ar
         const int pa = u.p.pos(tok0), pb = pa + ntok - 1;
         const int first = i, stop = (int)min((long long)u.t.n, i + left);
         const int low = a.window ? pa - a.window + 1 : 0;
-        __syncthreads();  // the last unit's tiles have been read
         for (int e = tid; e < kRows * (DP / 4); e += kThreads) {
             const int r = e / (DP / 4), c = e % (DP / 4);
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
             if (r < nrow && c * 4 < a.d) {
                 const int t = div(a.group_div, r), head = u.kvh * a.group + r - t * a.group;
-                x = load4(reinterpret_cast<const T *>(a.q) + (u.p.q0 + tok0 + t) * a.q_row + head * a.q_head + c * 4);
+                x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + (u.p.q0 + tok0 + t) * a.q_row + head * a.q_head + c * 4);
             }
             *reinterpret_cast<float4 *>(sq + r * S::kRow + c * 4) = x;
         }
@@ -217,24 +209,37 @@ __global__ void __launch_bounds__(kThreads) k_prefill(const __grid_constant__ Ar
 #pragma unroll
             for (int c = 0; c < DP / 16; c++) acc[y][c] = 0.f;
         }
+        // keys and values on their way by asynchronous copies: the next keys while the weights
+        // and outputs of a tile are made, its values while the next scores are
+        auto offsets = [&](int j0, long long (&at)[kCopies]) {
+#pragma unroll
+            for (int y = 0; y < kCopies; y++) {
+                const int j = j0 + (tid + kThreads * y) / (DP / 4);
+                at[y] = -1;
+                if (j < u.p.len && (j < u.p.pre || (j >= low && j <= pb))) {
+                    const int id = page_of(a, u.seq, j);
+                    if (id >= 0) at[y] = (id * a.ps + u.kvh * a.hs + (long long)(j - div(a.page, j) * a.page.d) * a.ts) * 4;
+                }
+            }
+        };
+        auto copy = [&](float *to, const char *from, const long long (&at)[kCopies]) {
+#pragma unroll
+            for (int y = 0; y < kCopies; y++) {
+                const int e = tid + kThreads * y, r = e / (DP / 4), c = e % (DP / 4);
+                const bool use = at[y] >= 0 && c * 4 < a.d;
+                cp_async16(mb::as::smem_u32(to + r * S::kRow + c * 4), use ? from + at[y] + c * 16 : from, use);
+            }
+            cp_commit();
+        };
+        long long at[kCopies], at_next[kCopies];
+        offsets(u.t.key(i), at);
+        copy(sk, a.k, at);
+        copy(sv, a.v, at);
         for (; i < stop; i++) {
             const int j0 = u.t.key(i);
-            __syncthreads();  // the tile before has been used, the queries are there
-            for (int e = tid; e < kKeys * (DP / 4); e += kThreads) {
-                const int r = e / (DP / 4), c = e % (DP / 4), j = j0 + r;
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-                if (c * 4 < a.d && j < u.p.len && (j < u.p.pre || (j >= low && j <= pb))) {
-                    const int id = page_of(a, u.seq, j);
-                    if (id >= 0) {
-                        const long long at = id * a.ps + u.kvh * a.hs + (long long)(j - div(a.page, j) * a.page.d) * a.ts + c * 4;
-                        x = load4(reinterpret_cast<const T *>(a.k) + at);
-                        y = load4(reinterpret_cast<const T *>(a.v) + at);
-                    }
-                }
-                *reinterpret_cast<float4 *>(sk + r * S::kRow + c * 4) = x;
-                *reinterpret_cast<float4 *>(sv + r * S::kRow + c * 4) = y;
-            }
-            __syncthreads();
+            const bool more = i + 1 < stop;
+            cp_wait<1>();
+            __syncthreads();  // the keys and the queries are there
             float s[4][4];
 #pragma unroll
             for (int y = 0; y < 4; y++)
@@ -257,6 +262,10 @@ __global__ void __launch_bounds__(kThreads) k_prefill(const __grid_constant__ Ar
                         s[y][x] = fmaf(q[y].w, k[x].w, s[y][x]);
                     }
             }
+            if (more) offsets(u.t.key(i + 1), at_next);
+            __syncthreads();  // the keys have been read
+            if (more) copy(sk, a.k, at_next);
+            else cp_commit();
 #pragma unroll
             for (int y = 0; y < 4; y++) {
                 float mx = -INFINITY;
@@ -280,7 +289,8 @@ __global__ void __launch_bounds__(kThreads) k_prefill(const __grid_constant__ Ar
 #pragma unroll
                 for (int c = 0; c < DP / 16; c++) acc[y][c] *= f;
             }
-            __syncwarp();  // a warp reads the rows that it wrote
+            cp_wait<1>();
+            __syncthreads();  // the values are there, and the weights
 #pragma unroll 4
             for (int k = 0; k < kKeys; k += 4) {
                 float4 e[4];
@@ -301,6 +311,9 @@ __global__ void __launch_bounds__(kThreads) k_prefill(const __grid_constant__ Ar
                         }
                     }
             }
+            __syncthreads();  // the values have been read
+            if (more) copy(sv, a.v, at_next);
+            else cp_commit();
         }
         left -= stop - first;
         const bool whole = first == 0 && stop == u.t.n;
@@ -332,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) k_prefill(const __grid_constant__ Ar
                 const int at = tx * 4 + 64 * c;
                 const float4 x = make_float4(acc[y][4 * c], acc[y][4 * c + 1], acc[y][4 * c + 2], acc[y][4 * c + 3]);
                 if (!whole) *reinterpret_cast<float4 *>(part + (size_t)r * DP + at) = x;
-                else if (at < a.d) store4(reinterpret_cast<T *>(a.out) + row * a.o_row + head * a.o_head + at, x);
+                else if (at < a.d) store4(reinterpret_cast<float *>(a.out) + row * a.o_row + head * a.o_head + at, x);
             }
             if (tx == 0) {
                 if (!whole) {
@@ -347,7 +360,7 @@ __global__ void __launch_bounds__(kThreads) k_prefill(const __grid_constant__ Ar
             for (int r = warp; r < nrow; r += kThreads / 32)
                 if (s_bad[r]) {
                     const int t = div(a.group_div, r);
-                    lone_row<T>(a, u.seq, pa + t, u.kvh * a.group + r - t * a.group, u.p.q0 + tok0 + t);
+                    lone_row<float>(a, u.seq, pa + t, u.kvh * a.group + r - t * a.group, u.p.q0 + tok0 + t);
                 }
         }
         if (left <= 0 && tid == 0) {
@@ -534,6 +547,34 @@ MB_DEV void exp2_fma(float &x0, float &x1)
     }
     x0 = __int_as_float(__float_as_int(y0) + (__float_as_int(r0) << 23));
     x1 = __int_as_float(__float_as_int(y1) + (__float_as_int(r1) << 23));
+}
+
+// tanh(k s) of a row of scores.  Where all of a warp's arguments are within 0.6, as those of
+// ordinary scores under an ordinary cap are, x times a polynomial in x^2 (least largest
+// relative error on [0, 0.36]: 2^-23.7), on the FMA units alone; else 1 - 2 / (1 + e^2x).
+MB_DEV void cap_scores(float (&s)[128], float k)
+{
+    float big = 0.f;
+#pragma unroll
+    for (int c = 0; c < 128; c += 2) {
+        fma2(s[c], s[c + 1], s[c], s[c + 1], k, k, 0.f, 0.f);
+        big = fmaxf(big, fmaxf(fabsf(s[c]), fabsf(s[c + 1])));
+    }
+    if (__any_sync(0xffffffffu, big > 0.6f)) {
+#pragma unroll
+        for (int c = 0; c < 128; c++) s[c] = 1.f - __fdividef(2.f, 1.f + ex2(s[c] * (2.f * kLog2e)));
+    } else {
+#pragma unroll
+        for (int c = 0; c < 128; c += 2) {
+            float t0, t1, y0 = 0.015475427731871605f, y1 = y0;
+            fma2(t0, t1, s[c], s[c + 1], s[c], s[c + 1], 0.f, 0.f);
+            fma2(y0, y1, y0, y1, t0, t1, -0.05210148170590401f, -0.05210148170590401f);
+            fma2(y0, y1, y0, y1, t0, t1, 0.13310173153877258f, 0.13310173153877258f);
+            fma2(y0, y1, y0, y1, t0, t1, -0.33332309126853943f, -0.33332309126853943f);
+            fma2(y0, y1, y0, y1, t0, t1, 0.9999999403953552f, 0.9999999403953552f);
+            fma2(s[c], s[c + 1], s[c], s[c + 1], y0, y1, 0.f, 0.f);
+        }
+    }
 }
 
 // Pairs of exponentials on the FMA units: kOnFma of every kMixed.
@@ -806,11 +847,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const int hi = min(p + 1, d.len), lo = a.window ? max(p - a.window + 1, 0) : 0;
                     const int full_hi = min(p0 + 1, d.len) - kTcKeys, full_lo = a.window ? p1 - a.window + 1 : 0;
                     const int first = d.first, stop = d.stop;
-                    float slope = 0.f, kcap = 0.f;
-                    if (EXTRA) {
-                        if (a.slopes && t < tok) slope = __ldg(a.slopes + d.kvh * a.group + r - t * a.group);
-                        if (a.cap > 0.f) kcap = 2.f * kLog2e / a.cap;
-                    }
+                    const float slope = EXTRA && a.slopes && t < tok ? -kLog2e * __ldg(a.slopes + d.kvh * a.group + r - t * a.group) : 0.f;
                     for (int i = first; i < stop; i++, step++) {
                         const int j0 = d.key(i);
                         const bool full = (j0 <= full_hi && j0 >= full_lo) || j0 + kTcKeys <= pre;
@@ -822,11 +859,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         tmem_ld32<96>(ts + 96, s);
                         tmem_wait_ld();
                         if (EXTRA) {
+                            float kc = a.scale * kLog2e;
+                            if (a.cap > 0.f) {
+                                cap_scores(s, a.scale / a.cap);
+                                kc = a.cap * kLog2e;
+                            }
+                            // the bias by distance, and to powers of two; no key after the row but in a prefix
+                            if (a.slopes && j0 < pre && j0 + kTcKeys > p0 + 1) {
 #pragma unroll
-                            for (int c = 0; c < 128; c++) {
-                                float z = s[c] * a.scale;
-                                if (a.cap > 0.f) z = capped(z, a.cap, kcap);
-                                s[c] = fmaf(-slope, fabsf((float)(p - (j0 + c))), z) * kLog2e;
+                                for (int c = 0; c < 128; c++) s[c] = fmaf(s[c], kc, slope * fabsf((float)(p - j0) - c));
+                            } else {
+                                const float base = slope * (float)(p - j0);
+#pragma unroll
+                                for (int c = 0; c < 128; c += 2) {
+                                    float b0, b1;
+                                    fma2(b0, b1, -slope, -slope, (float)c, (float)(c + 1), base, base);
+                                    fma2(s[c], s[c + 1], s[c], s[c + 1], kc, kc, b0, b1);
+                                }
                             }
                         }
                         if (!full) {
@@ -994,16 +1043,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
 }
 
-template <typename T, int DP>
-int run(Args &a, int ctas, int device, cudaStream_t s)
+template <int DP>
+int run(Args &a, void *space, int device, cudaStream_t s)
 {
     const char *who = "mocha_kv_prefill";
-    const int tokens = kRows / a.group;
+    const int tokens = kRows / a.group, ctas = mb::kSMs * Smem32<DP>::kCtas;
+    lay_out(a, space, ctas);
     static std::atomic<unsigned long long> allowed{0};
-    if (allow_smem(who, k_prefill<T, DP>, Smem32<DP>::kTotal, device, allowed) ||
-        launch(who, k_prefill<T, DP>, dim3(ctas), kThreads, Smem32<DP>::kTotal, s, false, a, tokens, 2))
+    if (allow_smem(who, k_prefill<DP>, Smem32<DP>::kTotal, device, allowed) ||
+        launch(who, k_prefill<DP>, dim3(ctas), kThreads, Smem32<DP>::kTotal, s, false, a, tokens, 2))
         return 1;
-    return launch(who, k_join<T, true>, dim3(kJoinBlocks), 32 * kJoinWarps, 0, s, true, a, ctas, kRows, DP);
+    return launch(who, k_join<float, true>, dim3(kJoinBlocks), 32 * kJoinWarps, 0, s, true, a, ctas, kRows, DP);
 }
 
 // ---- tensor maps -----------------------------------------------------------------------
@@ -1038,7 +1088,7 @@ int encode(CUtensorMap *map, int type, const void *base, const long long (&n)[4]
 }
 
 template <typename T, int DP>
-int run_tc(Args &a, const mocha_kv_pages *p, int device, cudaStream_t s)
+int run_tc(Args &a, const mocha_kv_pages *p, void *space, int device, cudaStream_t s)
 {
     const char *who = "mocha_kv_prefill";
     const int tok = 128 / a.group, d = a.d;
@@ -1049,7 +1099,8 @@ int run_tc(Args &a, const mocha_kv_pages *p, int device, cudaStream_t s)
         !encode(&maps.k, p->type, a.k, {d, p->page_size, a.kv_heads, a.pages}, {a.ts * 2, a.hs * 2, a.ps * 2}, box, 1) ||
         !encode(&maps.v, p->type, a.v, {d, p->page_size, a.kv_heads, a.pages}, {a.ts * 2, a.hs * 2, a.ps * 2}, box, 1))
         return fail(who, "the tensor maps cannot be encoded");
-    const int ctas = mb::kSMs;
+    constexpr int ctas = mb::kSMs;
+    lay_out(a, space, ctas);
     const auto go = [&](auto kernel, std::atomic<unsigned long long> &allowed) {
         constexpr size_t smem = SmemTc<DP>::kTiles + sizeof(TcBars);
         return allow_smem(who, kernel, smem, device, allowed) || launch(who, kernel, dim3(ctas), kTcThreads, smem, s, false, a, maps, tok, box, 2);
@@ -1064,11 +1115,10 @@ int run_tc(Args &a, const mocha_kv_pages *p, int device, cudaStream_t s)
 namespace kv {
 size_t decode_workspace(int type, int group, int d);
 
-static int prefill_ctas(int type) { return type == MOCHA_KV_F32 ? 2 * mb::kSMs : mb::kSMs; }
 static size_t prefill_workspace(int type, int d)
 {
-    const int n = prefill_ctas(type);
-    return meta_bytes(n) + part_bytes(n, type == MOCHA_KV_F32 ? kRows : 256, padded_dim(d));
+    const int dp = padded_dim(d), f32 = type == MOCHA_KV_F32, n = mb::kSMs * (!f32 ? 1 : dp == 64 ? Smem32<64>::kCtas : Smem32<128>::kCtas);
+    return meta_bytes(n) + part_bytes(n, f32 ? kRows : 256, dp);
 }
 }  // namespace kv
 
@@ -1102,14 +1152,12 @@ extern "C" int mocha_kv_prefill(const mocha_kv_pages *pages, const mocha_kv_seqs
     a.rows = rows;
     if (!workspace || !aligned(workspace) || workspace_bytes < kv::prefill_workspace(pages->type, d))
         return fail(who, "workspace missing, not 16-byte aligned or smaller than mocha_kv_workspace says");
-    const int ctas = kv::prefill_ctas(pages->type);
-    lay_out(a, workspace, ctas);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int dev = guard.device();
     const bool narrow = padded_dim(d) == 64;
     switch (pages->type) {
-    case MOCHA_KV_F32: return narrow ? run<float, 64>(a, ctas, dev, s) : run<float, 128>(a, ctas, dev, s);
-    case MOCHA_KV_F16: return narrow ? run_tc<__half, 64>(a, pages, dev, s) : run_tc<__half, 128>(a, pages, dev, s);
-    default: return narrow ? run_tc<__nv_bfloat16, 64>(a, pages, dev, s) : run_tc<__nv_bfloat16, 128>(a, pages, dev, s);
+    case MOCHA_KV_F32: return narrow ? run<64>(a, workspace, dev, s) : run<128>(a, workspace, dev, s);
+    case MOCHA_KV_F16: return narrow ? run_tc<__half, 64>(a, pages, workspace, dev, s) : run_tc<__half, 128>(a, pages, workspace, dev, s);
+    default: return narrow ? run_tc<__nv_bfloat16, 64>(a, pages, workspace, dev, s) : run_tc<__nv_bfloat16, 128>(a, pages, workspace, dev, s);
     }
 }
