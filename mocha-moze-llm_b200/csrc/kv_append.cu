@@ -67,6 +67,8 @@ MB_DEV void store8(T *p, const float (&x)[8])
 template <typename TI, typename TO, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) k_append(const __grid_constant__ Append a)
 {
+    mb::as::griddep_launch();
+    mb::as::griddep_wait();
     const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
     if (id >= a.total) return;
     const long long row = a.total <= INT_MAX ? (long long)div(a.items, (uint32_t)id) : id / a.items.d;
@@ -130,8 +132,8 @@ template <typename TI, typename TO>
 int run(const Append &a, bool interleaved, cudaStream_t s)
 {
     const dim3 grid((unsigned)((a.total + 255) / 256));
-    return interleaved ? launch("mocha_kv_append", k_append<TI, TO, true>, grid, 256, 0, s, false, a)
-                       : launch("mocha_kv_append", k_append<TI, TO, false>, grid, 256, 0, s, false, a);
+    return interleaved ? launch("mocha_kv_append", k_append<TI, TO, true>, grid, 256, 0, s, a)
+                       : launch("mocha_kv_append", k_append<TI, TO, false>, grid, 256, 0, s, a);
 }
 
 template <typename TI>

@@ -269,13 +269,15 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 2) k_join(const __grid_consta
 {
     __shared__ Joined s_part[kJoinWarps][32];
     __shared__ int s_items[kJoinMetas], s_warp[kJoinWarps], s_total;
+    __shared__ int2 s_note[kJoinMetas];
+    mb::as::griddep_launch();
     mb::as::griddep_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     // items (a block's work) before each unit's end, in the order of the CTAs
     static_assert(kJoinMetas <= 32 * kJoinWarps, "a thread per note");
     int n = 0;
     if (tid < metas) {
-        const int2 note = __ldcg(a.note + tid);
+        const int2 note = s_note[tid] = __ldcg(a.note + tid);
         if (note.x >= 0) n = note.x - tid < kJoinSerial ? (note.y + kJoinWarps - 1) / kJoinWarps : note.y;
     }
     int incl = n;
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 2) k_join(const __grid_consta
         int c = 0;  // the first unit that ends after `item`
         for (int step = 256; step; step >>= 1)
             if (c + step <= metas && s_items[c + step - 1] <= item) c += step;
-        const int2 note = __ldcg(a.note + c);
+        const int2 note = s_note[c];
         const Meta mt = a.meta[c];
         const int first = c ? s_items[c - 1] : 0, c_end = note.x;
         const bool serial = c_end - c < kJoinSerial;
@@ -513,10 +515,10 @@ inline Args make_args(const mocha_kv_pages *p, const mocha_kv_seqs *s, const moc
     return a;
 }
 
-// Launch on the current device with an error message; `after`: the kernel may start while
-// the one before it in the stream ends, and waits for it itself.
+// Launch on the current device with an error message.  The kernel may start while the one
+// before it in the stream ends, and waits for it itself before it reads or writes anything.
 template <typename... K, typename... A>
-int launch(const char *who, void (*kernel)(K...), dim3 grid, int threads, size_t smem, cudaStream_t s, bool after, A &&...args)
+int launch(const char *who, void (*kernel)(K...), dim3 grid, int threads, size_t smem, cudaStream_t s, A &&...args)
 {
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at{};
@@ -527,7 +529,7 @@ int launch(const char *who, void (*kernel)(K...), dim3 grid, int threads, size_t
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = &at;
-    cfg.numAttrs = after ? 1 : 0;
+    cfg.numAttrs = 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
     if (e != cudaSuccess) return (void)cudaGetLastError(), fail(who, cudaGetErrorString(e));
     return 0;

@@ -34,7 +34,7 @@ template <typename T, int DP, int NG>
 struct Ring {
     static constexpr bool kF32 = sizeof(T) == 4;
     static constexpr int kWarps = kF32 ? 8 : 4, kThreads = 32 * kWarps;
-    static constexpr int kH = NG ? 8 * NG : 4, kHB = 4;  // heads; heads met at a time (the join's blocks find room beside two CTAs)
+    static constexpr int kH = NG ? 8 * NG : 4, kHB = kF32 ? 4 : 8;  // heads; heads met at a time
     static constexpr int kKeys = (kF32 ? 1024 : 2048) / DP, kTile = kWarps * kKeys;
     static constexpr int kHalf = kKeys * DP * (int)sizeof(T), kStage = 2 * kHalf;
     static constexpr int kCtas = kF32 || NG > 1 ? 1 : 2;
@@ -54,6 +54,11 @@ struct Work {
     int min_tiles;            // of a share
     bool one_page;            // a warp's keys of a tile lie in one page
 };
+
+// What a unit's end counts for in a share, in tiles: the warps' meeting and the next unit's
+// start.  Without it the CTAs with the shortest sequences were last (64 sequences up to
+// 2047: the slowest 41 us, half of them 32).
+constexpr int kUnitEnd = 1;
 
 // A walk along a CTA's tiles; j is the tile's first key.
 template <int TILE>
@@ -76,11 +81,12 @@ struct Walk {
         i = tile;
         j = t.key(tile);
     }
-    MB_DEV void next(const Args &a, int hh_n)
+    // On to the next tile; returns what the tile left behind counts for in a share.
+    MB_DEV int next(const Args &a, int hh_n)
     {
         if (++i < t.n) {
             j = i == t.pre_t ? t.lo_t * TILE : j + TILE;
-            return;
+            return 1;
         }
         if (++hh == hh_n) {
             hh = 0;
@@ -88,6 +94,7 @@ struct Walk {
             load(a);
         }
         at(0);
+        return 1 + kUnitEnd;
     }
     // whether all of n keys from k on are visible; whether key k is
     MB_DEV bool all_visible(int k, int n) const { return k + n <= len && (k >= lo || k + n <= pre); }
@@ -154,7 +161,7 @@ MB_DEV bool find_share(const Work &w, int hh_n, long long *s_warp, int *s_seq, l
     long long sum = 0;
     for (k.seq = b0; k.seq < b1; k.seq++) {
         k.load(a);
-        sum += (long long)k.t.n * hh_n;
+        sum += (long long)(k.t.n + kUnitEnd) * hh_n;
     }
     long long incl = sum;
 #pragma unroll
@@ -177,7 +184,7 @@ MB_DEV bool find_share(const Work &w, int hh_n, long long *s_warp, int *s_seq, l
     if (*start < total && at <= *start && *start < incl) {
         for (k.seq = b0;; k.seq++) {
             k.load(a);
-            const long long n = (long long)k.t.n * hh_n;
+            const long long n = (long long)(k.t.n + kUnitEnd) * hh_n;
             if (*start < at + n) break;
             at += n;
         }
@@ -211,6 +218,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int hh_n = a.kv_heads * w.hgroups;
     mb::as::griddep_launch();
+    mb::as::griddep_wait();
     long long start, end, per;
     if (!find_share<R::kTile, kWarps>(w, hh_n, s_warp, &s_seq, &s_rem, &start, &end, &per)) {
         if (tid == 0) a.note[blockIdx.x].x = -1;
@@ -219,8 +227,19 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
     Walk<R::kTile> in;  // the next tile to load
     in.seq = s_seq;
     in.load(a);
-    in.hh = (int)div64(s_rem, in.t.n);
-    in.at((int)(s_rem - (long long)in.hh * in.t.n));
+    in.hh = (int)div64(s_rem, in.t.n + kUnitEnd);
+    in.at((int)(s_rem - (long long)in.hh * (in.t.n + kUnitEnd)));
+    int left = (int)(end - start);  // of the share, from tile `it` on
+    if (in.i >= in.t.n) {           // within a unit's end: the next unit is the first
+        left -= in.t.n + kUnitEnd - in.i;
+        in.i = in.t.n - 1;
+        in.next(a, hh_n);
+    }
+    if (left <= 0) {
+        if (tid == 0) a.note[blockIdx.x].x = -1;
+        return;
+    }
+    int left_in = left;  // from tile `in` on
     Walk<R::kTile> it = in;  // the tile to compute
     const uint32_t wring = mb::as::smem_u32(smem) + warp * R::kStages * R::kStage;
 
@@ -236,12 +255,12 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
 
     // pages of the groups of this warp's keys of tile `in`; one when pages hold whole tiles
     int pages[GROUPS];
-    auto look_up = [&]() {
-        const int j = in.j + warp * KEYS;
-        const int *row = a.table + in.seq * a.table_stride;
+    auto look_up = [&](const Walk<R::kTile> &at, int (&to)[GROUPS]) {
+        const int j = at.j + warp * KEYS;
+        const int *row = a.table + at.seq * a.table_stride;
 #pragma unroll
         for (int g = 0; g < GROUPS; g++)
-            if (g == 0 || !w.one_page) pages[g] = j + 8 * g < in.len ? __ldg(row + div(a.page, j + 8 * g)) : 0;
+            if (g == 0 || !w.one_page) to[g] = j + 8 * g < at.len ? __ldg(row + div(a.page, j + 8 * g)) : 0;
     };
     auto issue = [&](uint32_t slot) {
         const int j = in.j + warp * KEYS;
@@ -279,16 +298,27 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
         }
     };
 
-    const int tiles = (int)(end - start);
-    look_up();
+    {
+        // the first tiles' pages are asked for together
+        int first[R::kStages][GROUPS], left_at = left;
+        Walk<R::kTile> at = in;
 #pragma unroll
-    for (int x = 0; x < R::kStages - 1; x++) {
-        if (x < tiles) {
-            issue(x * R::kStage);
-            in.next(a, hh_n);
-            look_up();
+        for (int x = 0; x < R::kStages; x++)
+            if (left_at > 0) {
+                look_up(at, first[x]);
+                left_at -= at.next(a, hh_n);
+            }
+#pragma unroll
+        for (int x = 0; x < R::kStages; x++) {
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) pages[g] = first[x][g];
+            if (x == R::kStages - 1) break;
+            if (left_in > 0) {
+                issue(x * R::kStage);
+                left_in -= in.next(a, hh_n);
+            }
+            cp_commit();
         }
-        cp_commit();
     }
 
     // the unit's heads and queries: 16-bit, the products' narrow operand in registers
@@ -330,7 +360,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
     float m[NM], l[NM];  // value that weights are taken from (log2), sums of this lane's weights
     uint32_t seen = 0;   // heads that have such a value
     float acc[NACC][4];
-    for (int x = 0; x < tiles; x++) {
+    while (left > 0) {
         if (fresh) {
             if constexpr (F32) {
                 // the last unit's queries are no longer read: its end was met
@@ -353,7 +383,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
         }
         cp_wait<R::kStages - 2>();
         __syncwarp();
-        if (x + R::kStages - 1 < tiles) {
+        if (left_in > 0) {
             issue(slot_in);
             // the tile after that on its way into L2: what is in flight in shared memory alone
             // does not cover the latency of loaded memory (128 sequences: 441 -> 405 us)
@@ -371,8 +401,8 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
                     }
                 }
             }
-            in.next(a, hh_n);
-            look_up();
+            left_in -= in.next(a, hh_n);
+            look_up(in, pages);
         }
         cp_commit();
         const int j = it.j + warp * KEYS, p = it.len - 1;
@@ -554,11 +584,11 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
         slot = slot == (R::kStages - 1) * R::kStage ? 0 : slot + R::kStage;
         slot_in = slot_in == (R::kStages - 1) * R::kStage ? 0 : slot_in + R::kStage;
         const bool last = it.i == it.t.n - 1;
-        if (last || x == tiles - 1) {
+        if (last || left == 1) {
             const int seq = it.seq, h0 = head0, hn = ng, rest = it.t.n - 1 - it.i;
             const bool whole = began && last, noted = began && !last;
-            it.next(a, hh_n);
-            if (x + 1 < tiles) queries();  // the next unit's, on their way while this one ends
+            left -= it.next(a, hh_n);
+            if (left > 0) queries();  // the next unit's, on their way while this one ends
             // the four warps' (m, l, output) into one, in the order of the warps
             if constexpr (!F32) {
 #pragma unroll
@@ -584,14 +614,11 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
 #pragma unroll
             for (int n = 0; n < H / HB; n++) {
                 if constexpr (!F32) {
-                    // a lane has heads 2 (lane % 4) and the next of each eight
-                    if ((lane & 3) / 2 == n % 2) {
 #pragma unroll
-                        for (int d = 0; d < DP / 16; d++)
+                    for (int d = 0; d < DP / 16; d++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                mine[(2 * (lane & 1) + (e & 1)) * R::kPad + d * 16 + (lane >> 2) + (e >> 1) * 8] = acc[n / 2 * (DP / 16) + d][e];
-                    }
+                        for (int e = 0; e < 4; e++)
+                            mine[(2 * (lane & 3) + (e & 1)) * R::kPad + d * 16 + (lane >> 2) + (e >> 1) * 8] = acc[n * (DP / 16) + d][e];
                 } else if (lane * 4 < DP) {
 #pragma unroll
                     for (int h = 0; h < HB; h++) {
@@ -635,14 +662,14 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
                 }
                 __syncthreads();  // the buffers are written again
             }
-            if (x == tiles - 1 && tid == 0) {
+            if (left <= 0 && tid == 0) {
                 a.note[blockIdx.x] = make_int2(noted ? (int)div64(end - 1 + rest, per) : -1, hn);
                 a.meta[blockIdx.x] = Meta{seq, h0, hn, seq, p};
             }
             began = true;
             fresh = true;
         } else
-            it.next(a, hh_n);
+            left -= it.next(a, hh_n);
     }
     cp_wait<0>();
 }
@@ -662,9 +689,9 @@ struct Plan {
         lay_out(w.a, space, kCtas);
         static std::atomic<unsigned long long> allowed{0};
         if (allow_smem(who, k_decode<T, DP, NG>, R::kTotal, device, allowed) ||
-            launch(who, k_decode<T, DP, NG>, dim3(kCtas), R::kThreads, R::kTotal, s, false, w))
+            launch(who, k_decode<T, DP, NG>, dim3(kCtas), R::kThreads, R::kTotal, s, w))
             return 1;
-        return launch(who, k_join<T, false>, dim3(kJoinBlocks), 32 * kJoinWarps, 0, s, true, w.a, kCtas, R::kH, DP);
+        return launch(who, k_join<T, false>, dim3(kJoinBlocks), 32 * kJoinWarps, 0, s, w.a, kCtas, R::kH, DP);
     }
 };
 

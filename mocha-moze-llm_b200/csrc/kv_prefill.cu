@@ -48,18 +48,51 @@ struct ShareSmem {
     Share out;
 };
 
-// Tiles of sequence s per kv head, by a warp.
+// What a unit's end counts for in a share, in tiles: outputs, and the next unit's start.
+constexpr int kUnitEnd = 2;
+
+// Tiles of sequence s per kv head with its units' ends, by a warp.
 template <int T>
 MB_DEV long long seq_tiles(const Args &a, int s, int tokens)
 {
     Piece p;
     p.load(a, s, tokens);
     long long n = 0;
-    for (int b = threadIdx.x & 31; b < p.blocks; b += 32) n += block_tiles<T>(a, p, b, tokens).n;
+    for (int b = threadIdx.x & 31; b < p.blocks; b += 32) n += block_tiles<T>(a, p, b, tokens).n + kUnitEnd;
 #pragma unroll
     for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     return n;
 }
+
+// A walk along the units of a CTA's share.
+template <int T>
+struct Units {
+    int seq, kvh, block;
+    Piece p;
+    Tiles<T> t;
+    MB_DEV void start(const Args &a, const Share &h, int tokens)
+    {
+        seq = h.seq;
+        kvh = h.kvh;
+        block = h.block;
+        p.load(a, seq, tokens);
+        t = block_tiles<T>(a, p, block, tokens);
+    }
+    MB_DEV void next(const Args &a, int tokens)
+    {
+        if (++block == p.blocks) {
+            block = 0;
+            if (++kvh == a.kv_heads) {
+                kvh = 0;
+                do {
+                    seq++;
+                    p.load(a, seq, tokens);
+                } while (p.blocks == 0);
+            }
+        }
+        t = block_tiles<T>(a, p, block, tokens);
+    }
+};
 
 // This CTA's share; false when it has none.  Called by all threads.
 template <int T, int THREADS>
@@ -98,7 +131,7 @@ MB_DEV bool find_share(const Args &a, int tokens, int min_tiles, ShareSmem &sm)
             Piece p;
             p.load(a, s, tokens);
             for (int b = 0;; b += 32) {
-                const int x = b + lane < p.blocks ? block_tiles<T>(a, p, b + lane, tokens).n : 0;
+                const int x = b + lane < p.blocks ? block_tiles<T>(a, p, b + lane, tokens).n + kUnitEnd : 0;
                 int incl = x;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -114,42 +147,24 @@ MB_DEV bool find_share(const Args &a, int tokens, int min_tiles, ShareSmem &sm)
                 }
                 rem -= __shfl_sync(0xffffffffu, incl, 31);
             }
+            Units<T> u;
+            u.start(a, h, tokens);
+            if (h.i >= u.t.n) {  // within a unit's end: the next unit is the first
+                h.start += u.t.n + kUnitEnd - h.i;
+                if (h.start < h.end) {
+                    u.next(a, tokens);
+                    h.seq = u.seq;
+                    h.kvh = u.kvh;
+                    h.block = u.block;
+                    h.i = 0;
+                }
+            }
         }
         if (lane == 0) sm.out = h;
     }
     __syncthreads();
     return sm.out.start < sm.out.end;
 }
-
-// A walk along the units of a CTA's share.
-template <int T>
-struct Units {
-    int seq, kvh, block;
-    Piece p;
-    Tiles<T> t;
-    MB_DEV void start(const Args &a, const Share &h, int tokens)
-    {
-        seq = h.seq;
-        kvh = h.kvh;
-        block = h.block;
-        p.load(a, seq, tokens);
-        t = block_tiles<T>(a, p, block, tokens);
-    }
-    MB_DEV void next(const Args &a, int tokens)
-    {
-        if (++block == p.blocks) {
-            block = 0;
-            if (++kvh == a.kv_heads) {
-                kvh = 0;
-                do {
-                    seq++;
-                    p.load(a, seq, tokens);
-                } while (p.blocks == 0);
-            }
-        }
-        t = block_tiles<T>(a, p, block, tokens);
-    }
-};
 
 // ---- fp32 ------------------------------------------------------------------------------
 // Products on the FMA units: 64 rows x 64 keys, 256 threads of 4 x 4 scores and 4 rows x
@@ -175,11 +190,13 @@ __global__ void __launch_bounds__(kThreads, Smem32<DP>::kCtas) k_prefill(const _
     __shared__ unsigned char s_bad[kRows];
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, warp = tid >> 5;
     mb::as::griddep_launch();
+    mb::as::griddep_wait();
     if (!find_share<kKeys, kThreads>(a, tokens, min_tiles, share)) {
         if (tid == 0) a.note[blockIdx.x].x = -1;
         return;
     }
     const Share h = share.out;
+    const bool extra = a.cap > 0.f || a.slopes;
     Units<kKeys> u;
     u.start(a, h, tokens);
     int i = h.i;
@@ -266,13 +283,15 @@ __global__ void __launch_bounds__(kThreads, Smem32<DP>::kCtas) k_prefill(const _
             __syncthreads();  // the keys have been read
             if (more) copy(sk, a.k, at_next);
             else cp_commit();
+            const bool full = (j0 + kKeys <= min(pa + 1, u.p.len) && (a.window == 0 || pb - j0 < a.window)) || j0 + kKeys <= u.p.pre;
 #pragma unroll
             for (int y = 0; y < 4; y++) {
                 float mx = -INFINITY;
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
                     const int j = j0 + tx + 16 * x;
-                    s[y][x] = visible(j, rp[y], u.p.len, u.p.pre, a.window) ? score2(a, s[y][x], slope[y], rp[y], j) : -INFINITY;
+                    s[y][x] = extra ? score2(a, s[y][x], slope[y], rp[y], j) : s[y][x] * a.scale * kLog2e;
+                    if (!full && !visible(j, rp[y], u.p.len, u.p.pre, a.window)) s[y][x] = -INFINITY;
                     mx = fmaxf(mx, s[y][x]);
                 }
 #pragma unroll
@@ -315,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, Smem32<DP>::kCtas) k_prefill(const _
             if (more) copy(sv, a.v, at_next);
             else cp_commit();
         }
-        left -= stop - first;
+        left -= stop - first + (stop == u.t.n ? kUnitEnd : 0);
         const bool whole = first == 0 && stop == u.t.n;
         float *part = a.part + ((size_t)blockIdx.x * 2 + (first == 0 ? 1 : 0)) * ((size_t)kRows * (DP + 2));
         if (tid < kRows) s_bad[tid] = 0;
@@ -644,6 +663,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         bar.abort = bar.bad = 0;
         fence_barrier_init();
     }
+    griddep_wait();
     // swizzled tiles are laid out by address: their base has to be a multiple of 1024
     const bool any = find_share<kTcKeys, kTcThreads>(a, tokens, min_tiles, share), placed = (smem_u32(smem) & 1023) == 0;
     if (!any || !placed) {
@@ -692,7 +712,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 mbar_arrive(&bar.unit_full[units % kTcUnits]);
             }
             if (!more) break;
-            left -= stop - i;
+            left -= stop - i + (stop == u.t.n ? kUnitEnd : 0);
             for (; i < stop && ok; i++) {
                 const int j0 = u.t.key(i);
                 const int keys = min(kTcKeys, u.p.len - j0);           // keys there are (not positive: none)
@@ -1038,7 +1058,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int e = lane; e < a.d; e += 32) bad |= !isfinite(to_f32(o[e]));
                 if (__any_sync(0xffffffffu, bad)) lone_row<T>(a, u.seq, u.p.pos(tok0 + t), head, row);
             }
-        left -= u.t.n - i;
+        left -= u.t.n - i + kUnitEnd;
         if (left > 0) u.next(a, tokens);
     }
 }
@@ -1051,9 +1071,9 @@ int run(Args &a, void *space, int device, cudaStream_t s)
     lay_out(a, space, ctas);
     static std::atomic<unsigned long long> allowed{0};
     if (allow_smem(who, k_prefill<DP>, Smem32<DP>::kTotal, device, allowed) ||
-        launch(who, k_prefill<DP>, dim3(ctas), kThreads, Smem32<DP>::kTotal, s, false, a, tokens, 2))
+        launch(who, k_prefill<DP>, dim3(ctas), kThreads, Smem32<DP>::kTotal, s, a, tokens, 1))
         return 1;
-    return launch(who, k_join<float, true>, dim3(kJoinBlocks), 32 * kJoinWarps, 0, s, true, a, ctas, kRows, DP);
+    return launch(who, k_join<float, true>, dim3(kJoinBlocks), 32 * kJoinWarps, 0, s, a, ctas, kRows, DP);
 }
 
 // ---- tensor maps -----------------------------------------------------------------------
@@ -1103,11 +1123,11 @@ int run_tc(Args &a, const mocha_kv_pages *p, void *space, int device, cudaStream
     lay_out(a, space, ctas);
     const auto go = [&](auto kernel, std::atomic<unsigned long long> &allowed) {
         constexpr size_t smem = SmemTc<DP>::kTiles + sizeof(TcBars);
-        return allow_smem(who, kernel, smem, device, allowed) || launch(who, kernel, dim3(ctas), kTcThreads, smem, s, false, a, maps, tok, box, 2);
+        return allow_smem(who, kernel, smem, device, allowed) || launch(who, kernel, dim3(ctas), kTcThreads, smem, s, a, maps, tok, box, 2);
     };
     static std::atomic<unsigned long long> allowed[2] = {};
     if (a.cap > 0.f || a.slopes || !(a.scale > 0.f) ? go(k_prefill_tc<T, DP, true>, allowed[1]) : go(k_prefill_tc<T, DP, false>, allowed[0])) return 1;
-    return launch(who, k_join<T, true>, dim3(kJoinBlocks), 32 * kJoinWarps, 0, s, true, a, ctas, 256, DP);
+    return launch(who, k_join<T, true>, dim3(kJoinBlocks), 32 * kJoinWarps, 0, s, a, ctas, 256, DP);
 }
 
 }  // namespace
