@@ -393,7 +393,9 @@ __global__ void __launch_bounds__(kThreads, Smem32<DP>::kCtas) k_prefill(const _
 
 
 // ---- 16-bit types: the tensor cores ----------------------------------------------------
-// One CTA per SM with two tiles of 128 query rows.  A producer warp copies queries, keys and
+// One CTA per SM with two tiles of 128 query rows (a unit of one tile, as of a few tokens
+// over a long cache, has its keys dealt to both in turn and the outputs added at its end:
+// 4 tokens of 32 sequences over up to 4000 keys: 71 -> 62 us).  A producer warp copies queries, keys and
 // values into shared memory by TMA (a page or a part of one per copy, 128-byte swizzle), one
 // thread issues the products, and four warps per tile, a row per thread, turn scores into
 // weights.  Scores S = Q K^T and outputs O += P V are accumulated in TMEM; P goes back to
@@ -429,13 +431,16 @@ struct TcUnit {
     int first, stop, n; // tiles of this share, and of the unit
     MB_DEV int key(int i) const { return (i < pre_t ? i : i - pre_t + lo_t) * kTcKeys; }
     MB_DEV bool whole() const { return first == 0 && stop == n; }
+    // one tile of rows: the tiles' warps take its key tiles in turn
+    MB_DEV bool lone(int tok) const { return ntok <= tok; }
 };
 
 struct TcBars {
     uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], o_full[2], kv_full[10], kv_empty[10], unit_full[kTcUnits],
-        unit_empty[kTcUnits], edge, drain;
+        unit_empty[kTcUnits], pair_full, pair_done, edge, drain;
     TcUnit unit[kTcUnits];
     Share share;
+    float2 pair[128];         // of a lone unit: the second tile's (m, l)
     uint32_t tmem;
     volatile int abort, bad;  // a wait ran out; an output is not finite
 };
@@ -536,38 +541,6 @@ MB_DEV void add2(float &d0, float &d1, float a0, float a1)
         : "f"(a0), "f"(a1));
 }
 
-// 2^x of a pair on the FMA units, for x <= 127: with n the integer nearest to x and
-// f = x - n in [-1/2, 1/2], a polynomial for 2^f (least largest relative error: 2^-13.7 of
-// degree 3 where weights are rounded to 2^-9, 2^-18.5 of degree 4 where to 2^-12) and n
-// added to its exponent.  Results below 2^-126 become 2^-126; of NaN something that is not
-// finite once rounded to 16 bits.
-template <typename T>
-MB_DEV void exp2_fma(float &x0, float &x1)
-{
-    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x0));
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x1));
-    float r0 = kRound, r1 = kRound, f0, f1, y0, y1;
-    add2(r0, r1, x0, x1);
-    float t0 = r0, t1 = r1;
-    add2(t0, t1, -kRound, -kRound);
-    fma2(f0, f1, t0, t1, -1.f, -1.f, x0, x1);
-    if constexpr (std::is_same<T, __half>::value) {
-        y0 = y1 = 0.009570102207362652f;
-        fma2(y0, y1, y0, y1, f0, f1, 0.05591785907745361f, 0.05591785907745361f);
-        fma2(y0, y1, y0, y1, f0, f1, 0.240247443318367f, 0.240247443318367f);
-        fma2(y0, y1, y0, y1, f0, f1, 0.6931217908859253f, 0.6931217908859253f);
-        fma2(y0, y1, y0, y1, f0, f1, 0.9999992847442627f, 0.9999992847442627f);
-    } else {
-        y0 = y1 = 0.0551716685295105f;
-        fma2(y0, y1, y0, y1, f0, f1, 0.2426111251115799f, 0.2426111251115799f);
-        fma2(y0, y1, y0, y1, f0, f1, 0.6932609677314758f, 0.6932609677314758f);
-        fma2(y0, y1, y0, y1, f0, f1, 0.9999280571937561f, 0.9999280571937561f);
-    }
-    x0 = __int_as_float(__float_as_int(y0) + (__float_as_int(r0) << 23));
-    x1 = __int_as_float(__float_as_int(y1) + (__float_as_int(r1) << 23));
-}
-
 // tanh(k s) of a row of scores.  Where all of a warp's arguments are within 0.6, as those of
 // ordinary scores under an ordinary cap are, x times a polynomial in x^2 (least largest
 // relative error on [0, 0.36]: 2^-23.7), on the FMA units alone; else 1 - 2 / (1 + e^2x).
@@ -595,9 +568,6 @@ MB_DEV void cap_scores(float (&s)[128], float k)
         }
     }
 }
-
-// Pairs of exponentials on the FMA units: kOnFma of every kMixed.
-constexpr int kMixed = 4, kOnFma = 1;
 
 // The n lowest bits.
 MB_DEV uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; }
@@ -658,6 +628,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&bar.unit_full[i], 1);
             mbar_init(&bar.unit_empty[i], 9);  // eight warps of weights and the thread of products
         }
+        mbar_init(&bar.pair_full, 128);
+        mbar_init(&bar.pair_done, 128);
         mbar_init(&bar.edge, 1);
         mbar_init(&bar.drain, 1);
         bar.abort = bar.bad = 0;
@@ -713,11 +685,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             if (!more) break;
             left -= stop - i + (stop == u.t.n ? kUnitEnd : 0);
+            // lane b has the page of the tile's keys b * box ..; the next tile's is asked for a tile ahead
+            auto page_at = [&](int tile) {
+                const int j = u.t.key(tile) + lane * box;
+                return tile < stop && lane * box < kTcKeys && j < u.p.len ? __ldg(a.table + u.seq * a.table_stride + div(a.page, j)) : 0;
+            };
+            int id = page_at(i);
             for (; i < stop && ok; i++) {
-                const int j0 = u.t.key(i);
+                const int j0 = u.t.key(i), j = j0 + lane * box;
                 const int keys = min(kTcKeys, u.p.len - j0);           // keys there are (not positive: none)
                 const int boxes = keys > 0 ? (keys + box - 1) / box : 0;
                 const bool edge = keys < kTcKeys;
+                const int row = lane < boxes ? j - (int)(div(a.page, j) * a.page.d) : 0;
+                const int id_next = page_at(i + 1);
+                if (lane < boxes && (unsigned)id >= (unsigned)a.pages && a.status) {
+                    bool seen = false;
+                    for (int y = 0; y < box && j + y < u.p.len; y++)
+                        seen |= (j + y <= pb && (a.window == 0 || pa - (j + y) < a.window)) || j + y < u.p.pre;
+                    if (seen) atomicMax(a.status, 1);
+                }
                 for (int v = 0; v < 2 && ok; v++, it++) {
                     const int st = it % S::kStages;
                     ok = mbar_wait(&bar.kv_empty[st], ((it / S::kStages) & 1) ^ 1, &bar.abort);
@@ -726,19 +712,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     uint64_t *full = v && edge ? &bar.edge : &bar.kv_full[st];
                     if (lane == 0) mbar_expect_tx(full, (uint32_t)(boxes * box * DP * 2));
                     __syncwarp();
-                    for (int b = lane; b < boxes; b += 32) {
-                        const int j = j0 + b * box;
-                        const uint32_t slot = div(a.page, j);
-                        const int id = __ldg(a.table + u.seq * a.table_stride + slot);
-                        if ((unsigned)id >= (unsigned)a.pages && a.status) {
-                            bool seen = false;
-                            for (int y = 0; y < box && j + y < u.p.len; y++)
-                                seen |= (j + y <= pb && (a.window == 0 || pa - (j + y) < a.window)) || j + y < u.p.pre;
-                            if (seen) atomicMax(a.status, 1);
-                        }
+                    if (lane < boxes)
                         for (int c = 0; c < DP / 64; c++)
-                            tma_load_4d(dst + c * (128 * 128) + b * box * 128, v ? &maps.v : &maps.k, 64 * c, j - (int)(slot * a.page.d), u.kvh, id, full);
-                    }
+                            tma_load_4d(dst + c * (128 * 128) + lane * box * 128, v ? &maps.v : &maps.k, 64 * c, row, u.kvh, id, full);
                     if (!v && i == begin) {
                         // the queries, behind the first keys: once the unit before no longer reads its own
                         for (int x = 0; x < 2 && x * tok < ntok; x++) {
@@ -764,6 +740,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         if (lane == 0) mbar_arrive(&bar.kv_full[st]);
                     }
                 }
+                id = id_next;
             }
             if (!ok) break;
             if (left > 0) u.next(a, tokens);
@@ -782,8 +759,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             return ok;
         };
         auto full = [&](int n) { return wait(&bar.kv_full[n % S::kStages], (n / S::kStages) & 1); };
-        auto qk = [&](int x, int st, bool last) {
-            const uint64_t q = sw128_desc(sq + x * S::kTile), k = sw128_desc(skv + st * S::kTile);
+        // keys of stage st; last: the unit's last keys for these queries; both: the stage is done with
+        auto qk = [&](int x, int st, bool lone, bool last, bool both) {
+            const uint64_t q = sw128_desc(sq + (lone ? 0 : x * S::kTile)), k = sw128_desc(skv + st * S::kTile);
             if (elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; kk++) {
@@ -791,9 +769,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     mma_bf16(tmem + x * 128, q + off, k + off, id_qk, kk > 0);
                 }
                 mma_commit(&bar.s_full[x]);
-                if (last) mma_commit(&bar.q_empty[x]);
+                if (last) mma_commit(&bar.q_empty[lone ? 0 : x]);
+                if (both) mma_commit(&bar.kv_empty[st]);
             }
             __syncwarp();
+        };
+        // weights of tile x with the values of stage st; the first 64 keys' are used while the others' are made
+        auto pv = [&](int x, int st, bool accumulate, bool both) {
+            const uint64_t v = mn_desc(skv + st * S::kTile, 128 * 128);
+            const uint32_t step = steps[x]++ & 1;
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                if (!wait(&bar.p_full[x][hf], step)) return false;
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 4 * hf; kk < 4 * hf + 4; kk++)
+                        mma_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, v + (kk * 2048 >> 4), id_pv, accumulate || kk > 0);
+                    if (hf) mma_commit(&bar.o_full[x]);
+                    if (hf && both) mma_commit(&bar.kv_empty[st]);
+                }
+                __syncwarp();
+            }
+            return true;
         };
         for (int units = 0; wait(&bar.unit_full[units % kTcUnits], (units / kTcUnits) & 1); units++) {
             const TcUnit &d = bar.unit[units % kTcUnits];
@@ -802,40 +799,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.unit_empty[units % kTcUnits]);
             if (done || !full(it)) break;
-            for (int x = 0; x < tiles && wait(&bar.q_full[x], asked[x]++ & 1); x++) qk(x, it % S::kStages, n == 1);
-            if (elect_one()) mma_commit(&bar.kv_empty[it % S::kStages]);
+            if (tiles == 1) {
+                // key tile j is tile j % 2's: K 0, K 1, then V j and K j + 2 in turn
+                if (!wait(&bar.q_full[0], asked[0]++ & 1)) break;
+                qk(0, it % S::kStages, true, n == 1, true);
+                if (n > 1) {
+                    if (!full(it + 2)) break;
+                    qk(1, (it + 2) % S::kStages, true, n == 2, true);
+                }
+                for (int j = 0; j < n; j++, it += 2) {
+                    if (!full(it + 1) || !pv(j & 1, (it + 1) % S::kStages, j > 1, true)) break;
+                    if (j + 2 < n) {
+                        if (!full(it + 4)) break;
+                        qk(j & 1, (it + 4) % S::kStages, true, j + 3 == n, true);
+                    }
+                }
+                continue;
+            }
+            for (int x = 0; x < 2 && wait(&bar.q_full[x], asked[x]++ & 1); x++) qk(x, it % S::kStages, false, n == 1, x == 1);
             for (int j = 0; j < n && ok; j++, it += 2) {
-                const int vt = (it + 1) % S::kStages, kt = (it + 2) % S::kStages;
+                // copies are ahead: asked for before the weights, they hold nothing up after
+                if (!full(it + 1) || (j + 1 < n && !full(it + 2))) break;
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    if (x == tiles) break;
-                    // the first 64 keys' weights are used while the others' are made
-                    const uint64_t v = mn_desc(skv + vt * S::kTile, 128 * 128);
-                    const uint32_t step = steps[x]++ & 1;
-                    if (x == 0 && !full(it + 1)) break;
-#pragma unroll
-                    for (int hf = 0; hf < 2; hf++) {
-                        if (!wait(&bar.p_full[x][hf], step)) break;
-                        if (elect_one()) {
-#pragma unroll
-                            for (int kk = 4 * hf; kk < 4 * hf + 4; kk++)
-                                mma_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, v + (kk * 2048 >> 4), id_pv, j > 0 || kk > 0);
-                            if (hf) mma_commit(&bar.o_full[x]);
-                        }
-                        __syncwarp();
-                    }
-                    if (!ok) break;
-                    if (j + 1 < n) {
-                        if (x == 0 && !full(it + 2)) break;
-                        qk(x, kt, j + 2 == n);
-                    }
+                    if (!pv(x, (it + 1) % S::kStages, j > 0, x == 1)) break;
+                    if (j + 1 < n) qk(x, (it + 2) % S::kStages, false, j + 2 == n, x == 1);
                 }
-                if (!ok) break;
-                if (elect_one()) {
-                    mma_commit(&bar.kv_empty[vt]);
-                    if (j + 1 < n) mma_commit(&bar.kv_empty[kt]);
-                }
-                __syncwarp();
             }
         }
         if (!ok) bar.abort = 1;
@@ -849,7 +838,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int x = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t ts = tmem + x * 128 + ((uint32_t)((warp & 3) * 32) << 16), to = ts + 256;
         const float k2 = EXTRA ? 1.f : a.scale * kLog2e;
-        uint32_t step = 0;
+        uint32_t step = 0, pairs = 0;
         // false when a wait has run out, here or elsewhere in the CTA
         auto wait = [&](uint64_t *b, uint32_t parity) {
             ok = __all_sync(0xffffffffu, mbar_wait(b, parity, &bar.abort));
@@ -859,16 +848,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int units = 0; wait(&bar.unit_full[units % kTcUnits], (units / kTcUnits) & 1); units++) {
             const TcUnit &d = bar.unit[units % kTcUnits];
             if (d.ntok == 0) break;
-            if (x * tok < d.ntok) {
+            const bool lone = d.lone(tok);
+            const int xt = lone ? 0 : x * tok;  // first token of this tile's rows
+            if (lone ? x < d.stop - d.first : xt < d.ntok) {
                 const int t = div(a.group_div, r);
                 float m = -INFINITY, l = 0.f;
                 {
-                    const int p0 = d.pos0 + x * tok, p1 = p0 + min(tok, d.ntok - x * tok) - 1, p = p0 + t, pre = d.pre;
+                    const int p0 = d.pos0 + xt, p1 = p0 + min(tok, d.ntok - xt) - 1, p = p0 + t, pre = d.pre;
                     const int hi = min(p + 1, d.len), lo = a.window ? max(p - a.window + 1, 0) : 0;
                     const int full_hi = min(p0 + 1, d.len) - kTcKeys, full_lo = a.window ? p1 - a.window + 1 : 0;
-                    const int first = d.first, stop = d.stop;
+                    const int first = d.first + (lone ? x : 0), stop = d.stop, stride = lone ? 2 : 1;
                     const float slope = EXTRA && a.slopes && t < tok ? -kLog2e * __ldg(a.slopes + d.kvh * a.group + r - t * a.group) : 0.f;
-                    for (int i = first; i < stop; i++, step++) {
+                    for (int i = first; i < stop; i += stride, step++) {
                         const int j0 = d.key(i);
                         const bool full = (j0 <= full_hi && j0 >= full_lo) || j0 + kTcKeys <= pre;
                         if (!wait(&bar.s_full[x], step & 1)) break;
@@ -913,21 +904,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         for (int c = 0; c < 128; c += 2) mx[(c / 2) & 3] = fmaxf(mx[(c / 2) & 3], fmaxf(s[c], s[c + 1]));
                         const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                         // a new maximum, and the output so far to its scale
-                        float f = 1.f;
-                        if ((mn - m) * k2 > 8.f) {
-                            f = ex2((m - mn) * k2);
-                            m = mn;
-                        }
-                        if (i > first && __any_sync(0xffffffffu, f != 1.f)) {
-                            if (!wait(&bar.o_full[x], (step & 1) ^ 1)) break;
+                        const bool grown = (mn - m) * k2 > 8.f;
+                        if (__any_sync(0xffffffffu, grown)) {
+                            const float f = grown ? ex2((m - mn) * k2) : 1.f;
+                            if (grown) m = mn;
+                            l *= f;
+                            if (i > first) {
+                                if (!wait(&bar.o_full[x], (step & 1) ^ 1)) break;
 #pragma unroll
-                            for (int c = 0; c < DP; c += 16) {
-                                float o[16];
-                                tmem_ld16f(to + c, o);
-                                tmem_wait_ld();
+                                for (int c = 0; c < DP; c += 16) {
+                                    float o[16];
+                                    tmem_ld16f(to + c, o);
+                                    tmem_wait_ld();
 #pragma unroll
-                                for (int e = 0; e < 16; e++) o[e] *= f;
-                                tmem_st16f(to + c, o);
+                                    for (int e = 0; e < 16; e++) o[e] *= f;
+                                    tmem_st16f(to + c, o);
+                                }
                             }
                         }
                         const float sub = m == -INFINITY ? 0.f : -m * k2;
@@ -939,12 +931,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             for (int e = 0; e < 16; e++) {
                                 float e0, e1;
                                 fma2(e0, e1, s[32 * b + 2 * e], s[32 * b + 2 * e + 1], k2, k2, sub, sub);
-                                if (e % kMixed < kOnFma) {
-                                    exp2_fma<T>(e0, e1);
-                                } else {
-                                    e0 = ex2(e0);
-                                    e1 = ex2(e1);
-                                }
+                                e0 = ex2(e0);
+                                e1 = ex2(e1);
                                 add2(sum[(2 * e) & 3], sum[(2 * e + 1) & 3], e0, e1);
                                 w[e] = pack16<T>(e0, e1);
                             }
@@ -955,16 +943,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                 mbar_arrive(&bar.p_full[x][b / 2]);
                             }
                         }
-                        l = fmaf(l, f, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     }
                 }
                 if (!ok || !wait(&bar.o_full[x], (step & 1) ^ 1)) break;
-                const bool mine = t < tok && x * tok + t < d.ntok, whole = d.whole();
+                // a lone unit's outputs: both tiles' rows are the same, the first's warps add them
+                float fa = 1.f, fb = 0.f;
+                const bool two = lone && d.stop - d.first > 1;
+                if (two) {
+                    if (x == 1) {
+                        bar.pair[r] = make_float2(m, l);
+                        tc_fence_before();
+                        mbar_arrive(&bar.pair_full);
+                        if (!wait(&bar.pair_done, pairs++ & 1)) break;  // the outputs have been read
+                    } else {
+                        if (!wait(&bar.pair_full, pairs++ & 1)) break;
+                        const float2 other = bar.pair[r];
+                        const float mm = fmaxf(m, other.x), ms = mm == -INFINITY ? 0.f : mm;
+                        fa = ex2((m - ms) * k2);
+                        fb = ex2((other.x - ms) * k2);
+                        l = l * fa + other.y * fb;
+                        m = mm;
+                    }
+                }
+                const bool mine = t < tok && xt + t < d.ntok && !(lone && x), whole = d.whole();
                 const int g = r - t * a.group, head = d.kvh * a.group + g;
-                const int at = (x * tok + t) * a.group + g;
-                const long long row = d.row0 + x * tok + t;
+                const int at = (xt + t) * a.group + g;
+                const long long row = d.row0 + xt + t;
                 float *part = a.part + ((size_t)blockIdx.x * 2 + (d.first == 0 ? 1 : 0)) * ((size_t)256 * (DP + 2));
-                // a row whose maximum is still -infinity has seen nothing (its weights are 2^-126)
+                // a row whose maximum is still -infinity has seen nothing
                 const float inv = !whole ? 1.f : m == -INFINITY ? 0.f : 1.f / l;
                 bool bad = false;
                 // 128 bytes of a row at a time; the four lanes of a quad write their rows' lines together
@@ -972,13 +979,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                             : reinterpret_cast<unsigned char *>(part + (size_t)at * DP);
                 const unsigned ours = __ballot_sync(0xffffffffu, mine);
 #pragma unroll 1
-                for (int line = 0; line < (whole ? DP / 64 : DP / 32); line++) {
+                for (int line = 0; line < (lone && x ? 0 : whole ? DP / 64 : DP / 32); line++) {
                     uint32_t w[32];
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         float o[32];
-                        tmem_ld32<0>(to + (whole ? 64 * line + 32 * c : 32 * line), o);
+                        const int col = whole ? 64 * line + 32 * c : 32 * line;
+                        tmem_ld32<0>(to + col, o);
                         tmem_wait_ld();
+                        if (two) {
+                            float o2[32];
+                            tmem_ld32<0>(to + 128 + col, o2);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] = fmaf(o2[e], fb, o[e] * fa);
+                        }
 #pragma unroll
                         for (int e = 0; e < 32; e++) {
                             o[e] *= inv;
@@ -1015,6 +1030,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
                 tc_fence_before();
+                if (two && x == 0) mbar_arrive(&bar.pair_done);
             }
             if (tid == 0) {
                 // the share's last unit leaves the last note
