@@ -3,11 +3,12 @@
 //
 // Every value is read once and written once; nothing else is to be done, so the kernel is
 // bound by memory: (heads + 2 kv heads) * dim values in and out per token, and 2 * dim / 2
-// angles.  A thread takes 16 values of one head, as 16-byte vectors: the two ends of eight
-// pairs (i, i + dims/2), or sixteen neighbours when pairs are interleaved or the values
-// are only copied.  Threads go along a token's heads, so a warp reads and writes whole
-// lines in every layout, and the token's angles, slot and page are L1 hits after the
-// first thread's.
+// angles.  A thread takes two 16-byte vectors of a head (four of fp32) that lie half the
+// rotated values apart: the two ends of eight pairs (i, i + dims/2), or twice four
+// interleaved pairs, or values that are only copied, likewise far apart.  Threads go along a
+// token's heads, so each of a warp's accesses covers whole lines in every layout, and the
+// token's slot, page and angles are L1 hits after the first thread's.  16381 rows of 32 + 16
+// heads of 128, bf16: 63.6 us, 5.1 TB/s; one row of 14 + 4 heads of 64: 2 us, a launch.
 #include "kv_common.cuh"
 
 namespace {
@@ -32,21 +33,20 @@ struct Append {
     const float *cos, *sin;
     long long rope_stride;
     int positions, rot_chunks, half;
+    int per_thread;
     long long total;
 };
 
-template <typename T>
-MB_DEV void load8(const T *p, float (&x)[8])
+// Heads of a thread, which share its angles and addresses, once half as many threads still
+// fill half the card: 32 + 16 heads of 128 take 3.26 us (512 rows), 5.26 (1024) and 79.7
+// (16384) with two heads, 3.65, 5.51 and 83.4 with one; at 256 rows both take 3.1, and one
+// row 2.6 against 2.35.  Four and eight heads measured 3 to 20 % worse up to 4096 rows.
+constexpr int kHeads = 2;
+
+MB_DEV void load4(const float *p, float *x)
 {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-        uint4 u = *reinterpret_cast<const uint4 *>(p);
-        const T *t = reinterpret_cast<const T *>(&u);
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = to_f32(t[i]);
-    }
+    const float4 a = *reinterpret_cast<const float4 *>(p);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
 }
 
 template <typename T>
@@ -64,7 +64,27 @@ MB_DEV void store8(T *p, const float (&x)[8])
     }
 }
 
-template <typename TI, typename TO, bool INTERLEAVED>
+// 16 values as they are stored.
+template <typename T>
+struct Raw {
+    uint4 v[sizeof(T)];  // 8 values take sizeof(T) / 2 vectors
+    MB_DEV void load(const T *first, const T *second)
+    {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+            v[i] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(first) + 16 * i);
+            v[sizeof(T) / 2 + i] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(second) + 16 * i);
+        }
+    }
+    MB_DEV void values(float (&x)[8], float (&y)[8]) const
+    {
+        const T *t = reinterpret_cast<const T *>(v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = to_f32(t[i]), y[i] = to_f32(t[8 + i]);
+    }
+};
+
+template <typename TI, typename TO, bool INTERLEAVED, int HEADS>
 __global__ void __launch_bounds__(256) k_append(const __grid_constant__ Append a)
 {
     mb::as::griddep_launch();
@@ -79,61 +99,76 @@ __global__ void __launch_bounds__(256) k_append(const __grid_constant__ Append a
         if (a.status) atomicMax(a.status, 1);
         return;
     }
-    int head = div(a.chunk_div, item);
-    const int c = item - head * a.chunks;
-    const TI *src;
-    TO *dst;
-    bool turn = c < a.rot_chunks;
-    if (head < a.heads) {
-        src = reinterpret_cast<const TI *>(a.q) + row * a.q_row + head * a.q_head;
-        dst = reinterpret_cast<TO *>(a.q_out) + row * a.o_row + head * a.o_head;
-    } else {
-        head -= a.heads;
-        const bool key = head < a.kv_heads;
-        if (!key) head -= a.kv_heads;
-        const uint32_t slot = div(a.page, p);
-        const int page = __ldg(a.table + s * a.table_stride + slot);
-        if ((unsigned)page >= (unsigned)a.pages) {
-            if (a.status) atomicMax(a.status, 1);
-            return;
+    const int h0 = div(a.chunk_div, item), c = item - h0 * a.chunks;
+    const int heads = a.heads + 2 * a.kv_heads;
+    const uint32_t slot = div(a.page, p);
+    const int page = __ldg(a.table + s * a.table_stride + slot);
+    const long long at = (p - (int)(slot * a.page.d)) * a.ts;
+    // two vectors of 8 values, half the rotated (or the other) values apart, of heads h0 HEADS ..
+    const bool turned = c < a.rot_chunks;
+    const int first = turned ? 8 * c : 2 * a.half + 8 * (c - a.rot_chunks);
+    const int second = first + (turned ? a.half : 8 * (a.chunks - a.rot_chunks));
+    Raw<TI> raw[HEADS];
+    float cs[8], sn[8];
+    if (turned && h0 * HEADS < a.heads + a.kv_heads) {
+        const float *cos = a.cos + p * a.rope_stride, *sin = a.sin + p * a.rope_stride;
+        if (INTERLEAVED) {
+            load4(cos + first / 2, cs), load4(cos + second / 2, cs + 4);
+            load4(sin + first / 2, sn), load4(sin + second / 2, sn + 4);
+        } else {
+            load4(cos + first, cs), load4(cos + first + 4, cs + 4);
+            load4(sin + first, sn), load4(sin + first + 4, sn + 4);
         }
-        src = key ? reinterpret_cast<const TI *>(a.k) + row * a.k_row + head * a.k_head
-                  : reinterpret_cast<const TI *>(a.v) + row * a.v_row + head * a.v_head;
-        dst = reinterpret_cast<TO *>(key ? a.k_pages : a.v_pages) + page * a.ps + head * a.hs + (p - (int)(slot * a.page.d)) * a.ts;
-        turn = turn && key;
     }
-    const int first = turn && !INTERLEAVED ? 8 * c : 16 * c, second = turn && !INTERLEAVED ? a.half + 8 * c : 16 * c + 8;
-    float x[8], y[8];
-    load8(src + first, x);
-    load8(src + second, y);
-    if (turn) {
-        float cs[8], sn[8];
-        load8(a.cos + p * a.rope_stride + 8 * c, cs);
-        load8(a.sin + p * a.rope_stride + 8 * c, sn);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if (INTERLEAVED) {
-                float &u = i < 4 ? x[2 * i] : y[2 * i - 8], &w = i < 4 ? x[2 * i + 1] : y[2 * i - 7];
+    for (int h = 0; h < HEADS; h++) {
+        const int head = h0 * HEADS + h;
+        if (head >= heads) break;
+        const int kv = head - a.heads;
+        const TI *src = kv < 0 ? reinterpret_cast<const TI *>(a.q) + row * a.q_row + head * a.q_head
+                        : kv < a.kv_heads ? reinterpret_cast<const TI *>(a.k) + row * a.k_row + kv * a.k_head
+                                          : reinterpret_cast<const TI *>(a.v) + row * a.v_row + (kv - a.kv_heads) * a.v_head;
+        raw[h].load(src + first, src + second);
+    }
+#pragma unroll
+    for (int h = 0; h < HEADS; h++) {
+        const int head = h0 * HEADS + h;
+        if (head >= heads) break;
+        const int kv = head - a.heads;
+        TO *dst;
+        if (kv < 0) {
+            dst = reinterpret_cast<TO *>(a.q_out) + row * a.o_row + head * a.o_head;
+        } else {
+            if ((unsigned)page >= (unsigned)a.pages) {
+                if (a.status) atomicMax(a.status, 1);
+                return;  // queries come first
+            }
+            dst = reinterpret_cast<TO *>(kv < a.kv_heads ? a.k_pages : a.v_pages) + page * a.ps + (kv < a.kv_heads ? kv : kv - a.kv_heads) * a.hs + at;
+        }
+        float x[8], y[8];
+        raw[h].values(x, y);
+        if (turned && head < a.heads + a.kv_heads) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                float &u = INTERLEAVED ? (i < 4 ? x[2 * i] : y[2 * i - 8]) : x[i], &w = INTERLEAVED ? (i < 4 ? x[2 * i + 1] : y[2 * i - 7]) : y[i];
                 const float r = u * cs[i] - w * sn[i];
                 w = u * sn[i] + w * cs[i];
                 u = r;
-            } else {
-                const float r = x[i] * cs[i] - y[i] * sn[i];
-                y[i] = x[i] * sn[i] + y[i] * cs[i];
-                x[i] = r;
             }
         }
+        store8(dst + first, x);
+        store8(dst + second, y);
     }
-    store8(dst + first, x);
-    store8(dst + second, y);
 }
 
 template <typename TI, typename TO>
 int run(const Append &a, bool interleaved, cudaStream_t s)
 {
     const dim3 grid((unsigned)((a.total + 255) / 256));
-    return interleaved ? launch("mocha_kv_append", k_append<TI, TO, true>, grid, 256, 0, s, a)
-                       : launch("mocha_kv_append", k_append<TI, TO, false>, grid, 256, 0, s, a);
+    const char *who = "mocha_kv_append";
+    if (a.per_thread == 1)
+        return interleaved ? launch(who, k_append<TI, TO, true, 1>, grid, 256, 0, s, a) : launch(who, k_append<TI, TO, false, 1>, grid, 256, 0, s, a);
+    return interleaved ? launch(who, k_append<TI, TO, true, kHeads>, grid, 256, 0, s, a) : launch(who, k_append<TI, TO, false, kHeads>, grid, 256, 0, s, a);
 }
 
 template <typename TI>
@@ -166,8 +201,10 @@ extern "C" int mocha_kv_append(const mocha_kv_pages *pages, const mocha_kv_seqs 
     if (rope->dims && (!rope->cos || !rope->sin || !aligned(rope->cos) || !aligned(rope->sin) || rope->positions < 1 ||
                        rope->stride < rope->dims / 2 || rope->stride % 4))
         return fail(who, "cos and sin must be 16-byte aligned tables with a stride of at least dims / 2, a multiple of 4");
-    const long long items = (long long)((q ? heads : 0) + 2ll * pages->kv_heads) * (d / 16);
-    if (items > INT_MAX / 2 || items * rows > 256ll * INT_MAX) return fail(who, "too many rows or heads for one call");
+    const long long all_heads = (q ? heads : 0) + 2ll * pages->kv_heads;
+    const int per_thread = all_heads * rows * (d / 16) >= mb::kSMs * 1024ll ? kHeads : 1;
+    const long long items = (all_heads + per_thread - 1) / per_thread * (d / 16);
+    if (all_heads > INT_MAX / 16 || items * rows > 256ll * INT_MAX) return fail(who, "too many rows or heads for one call");
     DeviceGuard guard;
     if (guard.enter(who, pages->device)) return 1;
     if (!rows) return 0;
@@ -211,6 +248,7 @@ extern "C" int mocha_kv_append(const mocha_kv_pages *pages, const mocha_kv_seqs 
     a.positions = rope->positions;
     a.rot_chunks = rope->dims / 16;
     a.half = rope->dims / 2;
+    a.per_thread = per_thread;
     a.total = items * rows;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     return in_type == MOCHA_KV_F32   ? run_to<float>(a, pages->type, rope->interleaved != 0, s)
