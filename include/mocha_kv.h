@@ -73,7 +73,7 @@ typedef struct {
  * z -= slopes[h] * |p - j| when slopes is not NULL.  Key j is visible when
  * j < kv_len and (j <= p and (window == 0 or p - j < window), or j < prefix[s]): a prefix
  * is seen by every query, also by those before its end and past the window.
- * heads / kv_heads is at most 64. */
+ * heads / kv_heads is at most 64, scale within 2^40, a cap from 2^-40 to 2^40. */
 typedef struct {
     int heads, window;
     float scale, cap;

@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
     queries();
 
     const bool extra = a.cap > 0.f || a.slopes || !(a.scale > 0.f);  // scores are more than a positive multiple of products
-    const float k2 = extra && !F32 ? 1.f : a.scale * kLog2e, kcap = a.cap > 0.f ? 2.f * kLog2e / a.cap : 0.f;
+    const float k2 = extra && !F32 ? 1.f : a.scale * kLog2e, kcap = a.cap > 0.f ? a.scale / a.cap : 0.f;
     // where a lane's matrices of the products lie in a stage
     uint32_t k_at[F32 ? 1 : DP / 16], v_at[F32 ? 1 : DP / 16];
     if constexpr (!F32) {
@@ -426,6 +426,22 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
                     for (int n = 0; n < NG; n++) mma<T>(s[t][n], kf, q[n][k][0], q[n][k][1]);
                 }
             // element e of tile t: key 16 t + lane / 4 (+ 8 for e > 1), head 2 (lane % 4) + e % 2
+            if (a.cap > 0.f) {
+                float big = 0.f;
+#pragma unroll
+                for (int t = 0; t < MT; t++)
+#pragma unroll
+                    for (int n = 0; n < NG; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) big = fmaxf(big, fabsf(s[t][n][e] *= kcap));
+                const bool far = __any_sync(0xffffffffu, big > kTanhPart);
+#pragma unroll
+                for (int t = 0; t < MT; t++)
+#pragma unroll
+                    for (int n = 0; n < NG; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[t][n][e] = far ? tanh_of(s[t][n][e]) : tanh_small(s[t][n][e]);
+            }
             if (extra || !full) {
 #pragma unroll
                 for (int t = 0; t < MT; t++)
@@ -437,8 +453,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
                             float z = s[t][n][e];
                             if (extra) {
                                 const int h = n * 8 + 2 * (lane & 3) + (e & 1);
-                                z *= a.scale;
-                                if (a.cap > 0.f) z = capped(z, a.cap, kcap);
+                                z *= a.cap > 0.f ? a.cap : a.scale;
                                 if (a.slopes && h < ng) z -= __ldg(a.slopes + head0 + h) * (float)(p - jj);
                                 z *= kLog2e;
                             }

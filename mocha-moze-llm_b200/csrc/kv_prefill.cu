@@ -541,30 +541,29 @@ MB_DEV void add2(float &d0, float &d1, float a0, float a1)
         : "f"(a0), "f"(a1));
 }
 
-// tanh(k s) of a row of scores.  Where all of a warp's arguments are within 0.6, as those of
-// ordinary scores under an ordinary cap are, x times a polynomial in x^2 (least largest
-// relative error on [0, 0.36]: 2^-23.7), on the FMA units alone; else 1 - 2 / (1 + e^2x).
-MB_DEV void cap_scores(float (&s)[128], float k)
+// cap tanh(k s) + bias of a row of scores, bias = base - slope c for column c, where cap is in
+// log2.  Where all of a warp's |k s| are within tanh_of's polynomial, as those of ordinary
+// scores under an ordinary cap are, on the FMA units alone: its coefficients take up k and cap.
+MB_DEV void cap_scores(float (&s)[128], float cap, float k, float slope, float base)
 {
     float big = 0.f;
 #pragma unroll
-    for (int c = 0; c < 128; c += 2) {
-        fma2(s[c], s[c + 1], s[c], s[c + 1], k, k, 0.f, 0.f);
-        big = fmaxf(big, fmaxf(fabsf(s[c]), fabsf(s[c + 1])));
-    }
-    if (__any_sync(0xffffffffu, big > 0.6f)) {
+    for (int c = 0; c < 128; c += 2) big = fmaxf(big, fmaxf(fabsf(s[c]), fabsf(s[c + 1])));
+    if (fabsf(k) > 256.f || __any_sync(0xffffffffu, big * fabsf(k) > kTanhPart)) {  // k^8 has to be finite
 #pragma unroll
-        for (int c = 0; c < 128; c++) s[c] = 1.f - __fdividef(2.f, 1.f + ex2(s[c] * (2.f * kLog2e)));
+        for (int c = 0; c < 128; c++) s[c] = fmaf(cap, tanh_of(s[c] * k), fmaf(-slope, (float)c, base));
     } else {
+        const float kk = k * k, c0 = kTanh0 * cap * k, c1 = kTanh1 * cap * k * kk, c2 = kTanh2 * cap * k * kk * kk,
+                    c3 = kTanh3 * cap * k * kk * kk * kk, c4 = kTanh4 * cap * k * kk * kk * kk * kk;
 #pragma unroll
         for (int c = 0; c < 128; c += 2) {
-            float t0, t1, y0 = 0.015475427731871605f, y1 = y0;
+            float t0, t1, y0, y1;
             fma2(t0, t1, s[c], s[c + 1], s[c], s[c + 1], 0.f, 0.f);
-            fma2(y0, y1, y0, y1, t0, t1, -0.05210148170590401f, -0.05210148170590401f);
-            fma2(y0, y1, y0, y1, t0, t1, 0.13310173153877258f, 0.13310173153877258f);
-            fma2(y0, y1, y0, y1, t0, t1, -0.33332309126853943f, -0.33332309126853943f);
-            fma2(y0, y1, y0, y1, t0, t1, 0.9999999403953552f, 0.9999999403953552f);
-            fma2(s[c], s[c + 1], s[c], s[c + 1], y0, y1, 0.f, 0.f);
+            fma2(y0, y1, t0, t1, c4, c4, c3, c3);
+            fma2(y0, y1, y0, y1, t0, t1, c2, c2);
+            fma2(y0, y1, y0, y1, t0, t1, c1, c1);
+            fma2(y0, y1, y0, y1, t0, t1, c0, c0);
+            fma2(s[c], s[c + 1], s[c], s[c + 1], y0, y1, fmaf(-slope, (float)c, base), fmaf(-slope, (float)(c + 1), base));
         }
     }
 }
@@ -870,23 +869,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         tmem_ld32<96>(ts + 96, s);
                         tmem_wait_ld();
                         if (EXTRA) {
-                            float kc = a.scale * kLog2e;
+                            // the cap, the bias by distance, and to powers of two.  No key is after
+                            // the row but in a prefix; there the distance changes its sign.
+                            const bool ahead = a.slopes && j0 < pre && j0 + kTcKeys > p0 + 1;
+                            const float by = ahead ? 0.f : slope, base = by * (float)(p - j0);
                             if (a.cap > 0.f) {
-                                cap_scores(s, a.scale / a.cap);
-                                kc = a.cap * kLog2e;
-                            }
-                            // the bias by distance, and to powers of two; no key after the row but in a prefix
-                            if (a.slopes && j0 < pre && j0 + kTcKeys > p0 + 1) {
-#pragma unroll
-                                for (int c = 0; c < 128; c++) s[c] = fmaf(s[c], kc, slope * fabsf((float)(p - j0) - c));
+                                cap_scores(s, a.cap * kLog2e, a.scale / a.cap, by, base);
                             } else {
-                                const float base = slope * (float)(p - j0);
 #pragma unroll
-                                for (int c = 0; c < 128; c += 2) {
-                                    float b0, b1;
-                                    fma2(b0, b1, -slope, -slope, (float)c, (float)(c + 1), base, base);
-                                    fma2(s[c], s[c + 1], s[c], s[c + 1], kc, kc, b0, b1);
-                                }
+                                for (int c = 0; c < 128; c++) s[c] = fmaf(s[c], a.scale * kLog2e, fmaf(-by, (float)c, base));
+                            }
+                            if (ahead) {
+#pragma unroll
+                                for (int c = 0; c < 128; c++) s[c] = fmaf(slope, fabsf((float)(p - j0) - c), s[c]);
                             }
                         }
                         if (!full) {

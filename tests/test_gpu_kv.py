@@ -225,6 +225,45 @@ def test_prefill_scores(kv, dtype, window, prefix, cap, slopes):
           slopes=slopes, scale=0.31)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("scale,cap", [(-0.3, 0.0), (0.0, 0.0), (-2.0, 3.0), (0.7, 0.25), (1e-3, 40.0), (4e4, 100.0), (-1e9, 1e-9)])
+def test_scales_and_caps(kv, dtype, scale, cap):
+    """Scales of any sign, and caps that scores stay far below or pass by far."""
+    check(kv, [150, 9], None, 4, 2, 64, 8, dtype, scale=scale, cap=cap)
+    check(kv, [150, 9], [40, 9], 4, 2, 64, 8, dtype, scale=scale, cap=cap, slopes=True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_zero_scores_under_a_steep_cap(kv, dtype):
+    """Scores of zero stay zero whatever scale and cap are: every key has the same weight."""
+    k, v, table = pool([150], 2, 64, 8, dtype, False, 5)
+    cache = kv.KvPages(k.zero_(), v)
+    q = queries(150, 4, 64, dtype, 6)
+    mean = ref.gather(v, table, 0, 150).mean(1).repeat_interleave(2, 0)
+    for scale, cap in [(2.0**40, 2.0**-40), (1.0, 2.0**-40), (2.0**40, 2.0**40)]:
+        for got in (cache.prefill(q, ints([0, 150]), table, ints([150]), scale=scale, cap=cap)[-1],
+                    cache.decode(q[-1:].contiguous(), table, ints([150]), scale=scale, cap=cap)[0]):
+            # 150 terms and two roundings of values below 5: fp32 150 2^-24 5, bf16 2^-8 of weights and result
+            assert (got.double() - mean).abs().max() <= (5e-5 if dtype == F32 else 2 * 2.0**-8 * 5)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_small_scores_below_a_wide_cap(kv, dtype):
+    """A cap far above most scores leaves them as they are, also beside one that reaches it."""
+    lens = [150]
+    k, v, table = pool(lens, 2, 64, 8, dtype, False, 5)
+    cache = kv.KvPages(k, v)
+    q = queries(150, 4, 64, dtype, 6)
+    q[140] *= 5e3
+    for scale, cap in [(0.125, 1e6), (0.125, 2.0**40), (0.125, 1e3)]:
+        want, wl, tol, tol_l = ref.attend(q, ref.gather(k, table, 0, 150), ref.gather(v, table, 0, 150), range(150), scale,
+                                          cap=cap, dtype=dtype)
+        got = cache.prefill(q, ints([0, 150]), table, ints([150]), scale=scale, cap=cap)
+        ok = torch.arange(150, device=DEV) != 140
+        close(got[ok], want[ok], tol[ok], f"cap {cap}")
+        close(cache.decode(q[-1:].contiguous(), table, ints([150]), scale=scale, cap=cap), want[-1:], tol[-1:], f"decode, cap {cap}")
+
+
 def test_prefill_more_rows_than_keys(kv):
     """Rows at negative positions see at most the prefix; without one they are zeros."""
     for prefix in (None, [2, 0, 9]):

@@ -53,6 +53,9 @@ def test_pages(kv, capfd, more, message):
     (dict(s=(2, 4, 4, 4096, None, None)), "kv_len"), (dict(z=(3, 0, 0.1, 0.0, None, None)), "multiple of kv_heads"),
     (dict(z=(130, 0, 0.1, 0.0, None, None)), "64 times"), (dict(z=(4, -1, 0.1, 0.0, None, None)), "window"),
     (dict(z=(4, 0, float("inf"), 0.0, None, None)), "finite"), (dict(z=(4, 0, 0.1, -1.0, None, None)), "cap"),
+    (dict(z=(4, 0, 2.0**41, 0.0, None, None)), "scale"), (dict(z=(4, 0, float("nan"), 0.0, None, None)), "scale"),
+    (dict(z=(4, 0, 0.1, 2.0**-41, None, None)), "cap"), (dict(z=(4, 0, 0.1, 2.0**41, None, None)), "cap"),
+    (dict(z=(4, 0, 0.1, float("nan"), None, None)), "cap"),
     (dict(q=(None, 256, 64)), "null q"), (dict(q=((1 << 16) + 2, 256, 64)), "q must be"),
     (dict(q=(1 << 16, 257, 64)), "q must be"), (dict(out=(1 << 17, 256, 32)), "out must be"),
     (dict(out=(1 << 17, -256, 64)), "out must be"),
