@@ -28,6 +28,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <new>
 #include <vector>
 
 #include "mb_common.cuh"
@@ -1133,14 +1134,28 @@ struct Paged {
     std::vector<int> free;
     std::vector<std::vector<int>> held;                 // [slots]
 
+    // All the host memory that release and reserve use.
+    bool lists(int slots)
+    {
+        try {
+            free.reserve(pages);
+            held.resize(slots);
+            for (auto &x : held) x.reserve(width);
+        } catch (const std::exception &) {
+            return false;
+        }
+        for (int i = pages - 1; i >= 0; i--) free.push_back(i);
+        return true;
+    }
     void release(int slot)
     {
         free.insert(free.end(), held[slot].rbegin(), held[slot].rend());
         held[slot].clear();
     }
+    int need(int positions) const { return (positions + page_size - 1) / page_size; }
     bool reserve(int slot, int positions)  // pages for the slot's first `positions`
     {
-        const int need = (positions + page_size - 1) / page_size;
+        const int need = this->need(positions);
         if ((int)held[slot].size() + (int)free.size() < need) return false;
         while ((int)held[slot].size() < need) {
             held[slot].push_back(free.back());
@@ -1359,19 +1374,30 @@ int enqueue_paged_attention(mocha_q8b *h, Rows rows, int n, int layer, bool grap
 }
 
 // Takes the pages that rows (host arrays) need and hands the rows' sequences to the device.
-// A no-op on a fixed cache.
+// Where there are too few pages nothing changes.  A no-op on a fixed cache.
 int paged_rows(mocha_q8b *h, int n, const int *pos, const int *slots, bool reserved = false)
-{
+try {
     if (!h->paged) return 0;
     Paged &g = *h->paged;
-    for (int i = 0; i < n && !reserved; i++)
-        if (pos[i] == 0) g.release(slots[i]);
-    for (int i = 0; i < n; i++)
-        if (!g.reserve(slots[i], pos[i] + 1)) {
+    std::vector<int> seq(n), start, len, table;
+    if (!reserved) {
+        std::vector<int> has(h->slots);  // pages of a slot after the rows so far
+        for (int i = 0; i < h->slots; i++) has[i] = (int)g.held[i].size();
+        long long more = 0;
+        for (int i = 0; i < n; i++) {
+            int &x = has[slots[i]];
+            if (pos[i] == 0) more -= x, x = 0;
+            const int need = g.need(pos[i] + 1);
+            if (need > x) more += need - x, x = need;
+        }
+        if (more > (long long)g.free.size()) {
             fprintf(stderr, "mocha_q8b: out of KV pages (%d of %d positions)\n", g.pages, g.page_size);
             return 1;
         }
-    std::vector<int> seq(n), start, len, table;
+        for (int i = 0; i < n; i++)
+            if (pos[i] == 0) g.release(slots[i]);
+        for (int i = 0; i < n; i++) g.reserve(slots[i], pos[i] + 1);
+    }
     for (int i = 0; i < n; i++) {
         if (i == 0 || slots[i] != slots[i - 1] || pos[i] != pos[i - 1] + 1) {
             start.push_back(i);
@@ -1392,11 +1418,14 @@ int paged_rows(mocha_q8b *h, int n, const int *pos, const int *slots, bool reser
     QB_TRY(cudaMemcpyAsync(g.table, table.data(), sizeof(int) * table.size(), cudaMemcpyHostToDevice, h->stream));
     QB_TRY(cudaStreamSynchronize(h->stream));  // the vectors end here
     return 0;
+} catch (const std::exception &e) {
+    fprintf(stderr, "mocha_q8b: %s\n", e.what());
+    return 1;
 }
 
 // The slots' page tables for decode steps.
 int paged_tables(mocha_q8b *h)
-{
+try {
     if (!h->paged) return 0;
     Paged &g = *h->paged;
     std::vector<int> table((size_t)h->slots * g.width, -1);
@@ -1404,6 +1433,9 @@ int paged_tables(mocha_q8b *h)
     QB_TRY(cudaMemcpyAsync(g.dec_table, table.data(), sizeof(int) * table.size(), cudaMemcpyHostToDevice, h->stream));
     QB_TRY(cudaStreamSynchronize(h->stream));
     return 0;
+} catch (const std::exception &e) {
+    fprintf(stderr, "mocha_q8b: %s\n", e.what());
+    return 1;
 }
 
 // Attention kernel for rows (host arrays): 2 when every block of 128 rows is one slot
@@ -1647,24 +1679,23 @@ int open_engine(int device, const void *file, unsigned long long bytes, int max_
         dalloc(&h->params, 1) || dalloc(&h->out_count, slots))
         return fail();
     if (kv_type >= 0) {
-        Paged &g = *(h->paged = new Paged());
+        if (!(h->paged = new (std::nothrow) Paged())) return fail();
+        Paged &g = *h->paged;
         g.type = kv_type;
         g.item = kv_type == MOCHA_KV_F32 ? 4 : 2;
         g.page_size = page_size;
         g.pages = pages;
         g.width = (CONTEXT + page_size - 1) / page_size;
-        g.held.resize(slots);
         const size_t pool = (size_t)LAYERS * pages * KV_HEADS * page_size * HEAD_DIM * g.item;
         const mocha_kv_pages one{device, kv_type, pages, page_size, KV_HEADS, HEAD_DIM, (long long)KV_HEADS * page_size * HEAD_DIM,
                                  (long long)page_size * HEAD_DIM, HEAD_DIM, (void *)256, (void *)256};
-        if (mocha_kv_workspace(&one, HEADS, 0, &g.space_bytes[0]) || mocha_kv_workspace(&one, HEADS, 1, &g.space_bytes[1]) ||
+        if (!g.lists(slots) || mocha_kv_workspace(&one, HEADS, 0, &g.space_bytes[0]) || mocha_kv_workspace(&one, HEADS, 1, &g.space_bytes[1]) ||
             dalloc(&g.k, pool) || dalloc(&g.v, pool) || dalloc(&g.qkv, R * QKV_ROWS) || dalloc(&g.q, R * DIM * g.item) ||
             dalloc(&g.att, R * DIM * g.item) || dalloc(&g.seq, R) || dalloc(&g.start, R + 1) || dalloc(&g.len, R) ||
             dalloc(&g.table, R * g.width) || dalloc(&g.dec_len, slots) || dalloc(&g.dec_table, (size_t)slots * g.width) ||
             dalloc(&g.status, 1) || dalloc((unsigned char **)&g.space[0], g.space_bytes[0]) ||
             dalloc((unsigned char **)&g.space[1], g.space_bytes[1]) || cudaMemset(g.status, 0, sizeof(int)))
             return fail();
-        for (int i = pages - 1; i >= 0; i--) g.free.push_back(i);
     }
     const size_t kv = h->paged ? 64 : kv_off(slots, 0, 0, 0);
     if (dalloc(&h->kc, kv) || dalloc(&h->vc, kv) || dalloc(&h->kvs.k_hi, kv) || dalloc(&h->kvs.k_lo, kv) ||

@@ -267,6 +267,8 @@ class Q8BatchHandle:
     def __init__(self, device: int, file_bytes, max_rows: int = 1024, slots: int = 64, lib: C.CDLL | None = None,
                  kv_type: str | None = None, page_size: int = 16, pages: int | None = None):
         import numpy as np
+        if kv_type is not None and kv_type not in self.KV_TYPES:
+            raise ValueError(f"kv_type must be one of {', '.join(self.KV_TYPES)}")
         self.lib = lib or load()
         self._file = np.ascontiguousarray(file_bytes, dtype=np.uint8)
         h = C.c_void_p()

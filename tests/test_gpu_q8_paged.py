@@ -74,6 +74,23 @@ def test_pages_are_taken_and_returned(native, q8_model_bytes):
         h.close()
 
 
+def test_a_call_without_pages_changes_nothing(native, q8_model_bytes, oracle):
+    """Three slots start anew, but there are pages for two: the call fails, and all go on as they were."""
+    p = np.random.default_rng(9).integers(0, VOCAB, 12).tolist()
+    h = native.Q8BatchHandle(0, q8_model_bytes, max_rows=64, slots=3, kv_type="f32", page_size=8, pages=5)
+    try:
+        h.forward(p[:11], range(11), [0] * 11)
+        assert h.free_pages() == 3
+        with pytest.raises(RuntimeError):
+            h.forward(p[:9] * 3, list(range(9)) * 3, [0] * 9 + [1] * 9 + [2] * 9)
+        assert h.free_pages() == 3
+        close(h.forward(p[11:], [11], [0], [0])[0], oracle_prompt_logits(oracle, p))
+        h.forward(p[:9] * 2, list(range(9)) * 2, [0] * 9 + [1] * 9)
+        assert h.free_pages() == 1
+    finally:
+        h.close()
+
+
 @pytest.mark.parametrize("page_size,pages", [(16, None), (24, 4), (8, 10)])
 def test_streams_through_few_pages(native, q8_model_bytes, oracle, page_size, pages):
     """Seven sequences with budgets 3..12 through three slots and a pool that holds them all,

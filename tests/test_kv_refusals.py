@@ -142,3 +142,8 @@ def test_open_paged(native, capfd, kv_type, page_size, pages):
     out = C.c_void_p()
     assert native.load().mocha_q8b_open_paged(0, None, 0, 64, 2, kv_type, page_size, pages, C.byref(out)) == 1
     assert "mocha_q8b_open_paged" in capfd.readouterr().err
+
+
+def test_open_paged_type_by_name(native):
+    with pytest.raises(ValueError, match="kv_type"):
+        native.Q8BatchHandle(0, b"", kv_type="int8")
