@@ -11,7 +11,8 @@
  * calls enqueue their kernels on `stream` (NULL: the default stream) and return; they
  * neither allocate nor wait, so they can be captured into graphs, and lengths, tables and
  * positions are read on the device at replay.  They may be made with any device current
- * and leave it as it was.  They return 0 on success and 1 on an error, with a message on
+ * and leave it as it was; outputs must not overlap inputs but where that is said to be
+ * allowed.  They return 0 on success and 1 on an error, with a message on
  * stderr and nothing enqueued.
  *
  * Types: the pages, the rotated queries and the attention's queries and outputs have one
@@ -39,7 +40,7 @@ typedef struct {
 
 /* The sequences.  table[s * table_stride + i], i < table_width, is the page of positions
  * [i * page_size, (i + 1) * page_size) of sequence s; entries of positions that no call
- * needs are not used.  A needed page id outside [0, pages) reads as a page of zeros and is
+ * needs are not used.  A sequence has at most 2^30 positions.  A needed page id outside [0, pages) reads as a page of zeros and is
  * not written.  Where `status` is not NULL, *status becomes at least 1 when such a page, or
  * an append position that the table or the angles do not hold, was met, and 2 when a
  * bounded wait inside a kernel ran out, which leaves outputs unwritten (it is never reset). */

@@ -487,10 +487,13 @@ inline int check_scores(const char *who, const mocha_kv_pages *p, const mocha_kv
     return 0;
 }
 
+// Positions and rows, so that no sum or difference of two, a window or a tile overflows.
+constexpr int kMostPositions = 1 << 30;
+
 inline int max_len(const mocha_kv_pages *p, const mocha_kv_seqs *s)
 {
     const long long n = (long long)s->table_width * p->page_size;
-    return n > INT_MAX - 65536 ? INT_MAX - 65536 : (int)n;  // a tile past the last position must not overflow
+    return n > kMostPositions ? kMostPositions : (int)n;
 }
 
 inline Args make_args(const mocha_kv_pages *p, const mocha_kv_seqs *s, const mocha_kv_scores *z, const mocha_kv_rows *q,
@@ -515,7 +518,7 @@ inline Args make_args(const mocha_kv_pages *p, const mocha_kv_seqs *s, const moc
     a.heads = z->heads;
     a.group = z->heads / p->kv_heads;
     a.group_div = fast_div(a.group);
-    a.window = z->window;
+    a.window = z->window < a.max_len ? z->window : 0;  // a window that holds every position is none
     a.scale = z->scale;
     a.cap = z->cap;
     a.prefix = z->prefix;

@@ -1172,7 +1172,7 @@ extern "C" int mocha_kv_prefill(const mocha_kv_pages *pages, const mocha_kv_seqs
     const char *who = "mocha_kv_prefill";
     if (check_pages(who, pages) || check_seqs(who, seqs) || check_scores(who, pages, scores)) return 1;
     const int b = type_bytes(pages->type), d = pages->head_dim;
-    if (rows < 0) return fail(who, "rows must not be negative");
+    if (rows < 0 || rows > kMostPositions) return fail(who, "rows must not be negative, nor more than 2^30");
     if (check_rows(who, "q", q, b, d, rows) || check_rows(who, "out", out, b, d, rows)) return 1;
     if (seqs->seqs && (!seqs->kv_len || !q_start)) return fail(who, "null kv_len or q_start");
     DeviceGuard guard;

@@ -8,7 +8,8 @@
 The calls enqueue on torch's current stream of the pages' device and can be captured into
 CUDA graphs; outputs and workspaces that the caller does not pass come from torch's
 allocator, call by call.  Arguments that do not fit raise ValueError before anything is
-enqueued; an error from the library raises RuntimeError.  No reference counterpart.
+enqueued; an error from the library raises RuntimeError.  There are no gradients: a tensor
+that requires one is refused unless gradients are off.  No reference counterpart.
 """
 from __future__ import annotations
 
@@ -86,6 +87,8 @@ class KvPages:
             raise ValueError("k and v must be float32, float16 or bfloat16, of one type")
         if k.stride() != v.stride() or k.stride(3) != 1:
             raise ValueError("k and v must have the same strides, the last one 1")
+        if k.requires_grad or v.requires_grad:
+            raise ValueError("pages must not require gradients")
         if k.device.type != "cuda" or k.device != v.device:
             raise ValueError("k and v must be on one CUDA device")
         self.k, self.v = k, v
@@ -119,6 +122,8 @@ class KvPages:
         if (len(shape) != 3 or t.dtype is not dtype or t.get_device() != self._index or shape[0] != rows or
                 shape[2] != self.head_dim or (heads is not None and shape[1] != heads)):
             raise ValueError(f"{name} must be [{rows}, {heads or 'heads'}, {self.head_dim}] of {dtype} on the pages' device")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires a gradient, which these operators do not have")
         row, head, one = t.stride()
         if one != 1:
             raise ValueError(f"{name}: a head's values must be contiguous")
@@ -182,7 +187,8 @@ class KvPages:
                     cos.stride() != sin.stride() or cos.stride(1) != 1):
                 raise ValueError("cos and sin must be float32 [positions, rotated dims / 2] with the same strides on "
                                  "the pages' device")
-            rope = _Rope(cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0], 2 * cos.shape[1],
+            rope = _Rope(cos.data_ptr(), sin.data_ptr(), cos.stride(0) if cos.shape[0] > 1 else cos.shape[1], cos.shape[0],
+                         2 * cos.shape[1],
                          int(bool(interleaved)))
         seqs = self._seqs(table, None, status)
         if lib.mocha_kv_append(self._pages, C.addressof(seqs), rows, self._int(seq, "seq", rows),

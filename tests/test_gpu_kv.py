@@ -271,6 +271,62 @@ def test_prefill_more_rows_than_keys(kv):
         check(kv, [3, 0, 20], [10, 4, 25], 4, 2, 64, 8, F32, prefix=prefix)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("window", [190, 205, 2 ** 31 - 1])
+def test_windows_wider_than_the_sequence(kv, dtype, window):
+    """Rows at negative positions do not wrap a wide window round."""
+    check(kv, [3, 0, 200], [10, 4, 205], 4, 2, 64, 8, dtype, window=window)
+    check(kv, [3, 0, 200], None, 4, 2, 64, 8, dtype, window=window)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_calls_without_rows(kv, dtype):
+    k, v, table = pool([20], 2, 64, 8, dtype)
+    cache = kv.KvPages(k, v)
+    none, q = queries(0, 4, 64, dtype), queries(3, 4, 64, dtype)
+    out = torch.full_like(q, 7.0)
+    k0 = k.clone()
+    assert cache.decode(none, table[:0], ints([])).shape == (0, 4, 64)
+    assert cache.prefill(none, ints([0]), table[:0], ints([])).shape == (0, 4, 64)
+    assert cache.prefill(none, ints([0, 0]), table, ints([20])).shape == (0, 4, 64)
+    cache.prefill(q, ints([0]), table[:0], ints([]), out=out)
+    cache.prefill(q, ints([2, 2]), table, ints([20]), out=out)
+    assert (out == 7).all()
+    assert cache.append(none, none[:, :2], none[:, :2], ints([]), ints([]), table).shape == (0, 4, 64)
+    assert torch.equal(k.nan_to_num(0.0), k0.nan_to_num(0.0))
+
+
+_FIRST = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch, mocha_kv
+d = dict(device="cuda", dtype=torch.bfloat16)
+ints = lambda *x: torch.tensor(x, device="cuda", dtype=torch.int32)
+k, v = torch.randn(6, 2, 16, 64, **d), torch.randn(6, 2, 16, 64, **d)
+q, new = torch.randn(2, 8, 64, **d), torch.randn(2, 2, 64, **d)
+cache, table, lens = mocha_kv.KvPages(k, v), ints(5, 0, 3, 1, 4, 2).view(2, 3), ints(40, 17)
+start, seq, pos = ints(0, 1, 2), ints(0, 1), ints(39, 16)
+def step():
+    r = cache.append(q, new, new, seq, pos, table)
+    return cache.decode(r, table, lens), cache.prefill(r, start, table, lens)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = step()
+g.replay()
+torch.cuda.synchronize()
+want = step()
+assert all(torch.equal(a, b) and a.isfinite().all() for a, b in zip(got, want))
+"""
+
+
+def test_first_calls_of_a_process_captured(kv):
+    import os
+    import subprocess
+    import sys
+    subprocess.run([sys.executable, "-c", _FIRST, os.path.dirname(kv.__file__)], check=True, timeout=240)
+
+
 @pytest.mark.parametrize("dtype,lens,qlens", [(F32, [3000], [3]), (BF16, [20000, 200], [5, 2]), (F16, [9000], [130])])
 def test_prefill_split(kv, dtype, lens, qlens):
     check(kv, lens, qlens, 8, 2, 128, 64, dtype)
@@ -564,8 +620,10 @@ def test_refusals(kv):
         lambda: cache.prefill(q, start[:2], table, lens),
         lambda: cache.append(q, q[:, :1], q[:, :2], lens, lens, table),
         lambda: cache.append(q, q[:, :2], q[:, :2], lens, lens, table, cos=torch.zeros(9, 32, device=DEV)),
+        lambda: cache.decode(q.clone().requires_grad_(), table, lens),
         lambda: kv.KvPages(k, v[:, :1]),
         lambda: kv.KvPages(k, v.float()),
+        lambda: kv.KvPages(k.clone().requires_grad_(), v),
         lambda: kv.KvPages(k.cpu(), v.cpu()),
     ]
     for i, call in enumerate(bad):
@@ -586,6 +644,10 @@ def test_refusals(kv):
         with pytest.raises(RuntimeError):
             call()
     assert cache.decode(q, table, lens).isfinite().all()
+    with torch.no_grad():
+        assert cache.decode(q.clone().requires_grad_(), table, lens).isfinite().all()
+    one = torch.zeros(16, device=DEV).as_strided((1, 16), (3, 1))  # a table of one row has no stride between rows
+    cache.append(q, q[:, :2], q[:, :2], ints([0, 1]), ints([0, 0]), table, cos=one, sin=one)
 
 
 def test_c_calls_refuse_a_small_workspace(kv, native, capfd):
