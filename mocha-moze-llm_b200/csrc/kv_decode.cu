@@ -385,22 +385,6 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
         __syncwarp();
         if (left_in > 0) {
             issue(slot_in);
-            // the tile after that on its way into L2: what is in flight in shared memory alone
-            // does not cover the latency of loaded memory (128 sequences: 441 -> 405 us)
-            if (in.i + 1 < in.t.n) {
-                constexpr int LINES = ROW / 128;
-                const int kvh = w.hgroups == 1 ? in.hh : in.hh / w.hgroups;
-                const int jp = in.t.key(in.i + 1) + warp * KEYS + lane / LINES, pl = lane % LINES * 128;
-                if (in.sees(jp) && pl < a.d * (int)sizeof(T)) {
-                    const uint32_t sl = div(a.page, jp);
-                    const int id = __ldg(a.table + in.seq * a.table_stride + sl);
-                    if ((unsigned)id < (unsigned)a.pages) {
-                        const char *at = a.k + (id * a.ps + kvh * a.hs + (jp - (int)(sl * a.page.d)) * a.ts) * (long long)sizeof(T) + pl;
-                        asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
-                        asm volatile("prefetch.global.L2 [%0];" ::"l"(at + v_off));
-                    }
-                }
-            }
             left_in -= in.next(a, hh_n);
             look_up(in, pages);
         }
