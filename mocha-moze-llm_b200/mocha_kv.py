@@ -72,8 +72,7 @@ def _load() -> C.CDLL:
     return _lib
 
 
-def _stream(device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+_stream = torch._C._cuda_getCurrentRawStream  # current_stream(device).cuda_stream in 0.1 us in place of 1.3
 
 
 class KvPages:
