@@ -45,7 +45,8 @@ struct Ring {
     static constexpr int kStat = kWarps * kH * 8;                   // (m, l)
     static constexpr int kQ = kF32 ? kH * DP * 4 : 0;              // fp32: the unit's queries,
     static constexpr int kW = kF32 ? kWarps * kH * kKeys * 4 : 0;  // and a tile's weights
-    static constexpr int kTotal = kRings + kMerge + kStat + kQ + kW;
+    static constexpr int kShare = 8 * (kWarps + 2);
+    static constexpr int kTotal = kRings + kMerge + kStat + kQ + kW + kShare;
 };
 
 struct Work {
@@ -207,13 +208,16 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
     constexpr int ROW = DP * (int)sizeof(T);
     constexpr int NM = F32 ? H : 2 * NG, NACC = F32 ? H : NG * DP / 16;
     constexpr int PARTS = 32 / KEYS;                 // fp32: lanes that share a key's products
+    // All shared memory is dynamic, so that the rings start on a 128-byte line: behind 48 bytes of
+    // static variables each copy of a line was four requests to L2 and twice its bytes (442 us
+    // for 128 sequences that take 382).
     extern __shared__ __align__(128) unsigned char smem[];
     float *merge = reinterpret_cast<float *>(smem + R::kRings);
     float2 *stat = reinterpret_cast<float2 *>(smem + R::kRings + R::kMerge);
     float *sq = reinterpret_cast<float *>(smem + R::kRings + R::kMerge + R::kStat);
     float *sw = sq + R::kQ / 4;
-    __shared__ long long s_warp[kWarps], s_rem;
-    __shared__ int s_seq;
+    long long *s_warp = reinterpret_cast<long long *>(sw + R::kW / 4), &s_rem = s_warp[kWarps];
+    int &s_seq = *reinterpret_cast<int *>(s_warp + kWarps + 1);
     const Args &a = w.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int hh_n = a.kv_heads * w.hgroups;
