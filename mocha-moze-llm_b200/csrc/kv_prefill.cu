@@ -669,12 +669,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         u.start(a, bar.share, tokens);
         int i = bar.share.i, it = 0, edges = 0, units = 0, asked[2] = {0, 0};
         long long left = bar.share.end - bar.share.start;
+        // together, for lanes that part here meet the warp's next barrier apart
+        auto wait = [&](uint64_t *b, uint32_t parity) { return ok = __all_sync(0xffffffffu, mbar_wait(b, parity, &bar.abort)); };
         for (;; units++) {
             const bool more = left > 0;
             const int stop = more ? (int)min((long long)u.t.n, i + left) : 0, begin = i;
             const int tok0 = u.block * tokens, ntok = min(tokens, u.p.nq - tok0), pa = u.p.pos(tok0), pb = pa + ntok - 1;
-            ok = mbar_wait(&bar.unit_empty[units % kTcUnits], ((units / kTcUnits) & 1) ^ 1, &bar.abort);
-            if (!ok) break;
+            if (!wait(&bar.unit_empty[units % kTcUnits], ((units / kTcUnits) & 1) ^ 1)) break;
             if (lane == 0) {
                 TcUnit &d = bar.unit[units % kTcUnits];
                 d.ntok = more ? ntok : 0;
@@ -714,8 +715,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 for (int v = 0; v < 2 && ok; v++, it++) {
                     const int st = it % S::kStages;
-                    ok = mbar_wait(&bar.kv_empty[st], ((it / S::kStages) & 1) ^ 1, &bar.abort);
-                    if (!ok) break;
+                    if (!wait(&bar.kv_empty[st], ((it / S::kStages) & 1) ^ 1)) break;
                     const uint32_t dst = skv + st * S::kTile;
                     uint64_t *full = v && edge ? &bar.edge : &bar.kv_full[st];
                     if (lane == 0) mbar_expect_tx(full, (uint32_t)(boxes * box * DP * 2));
@@ -726,8 +726,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (!v && i == begin) {
                         // the queries, behind the first keys: once the unit before no longer reads its own
                         for (int x = 0; x < 2 && x * tok < ntok; x++) {
-                            ok = ok && mbar_wait(&bar.q_empty[x], (asked[x]++ & 1) ^ 1, &bar.abort);
-                            if (ok && lane == 0) {
+                            if (!wait(&bar.q_empty[x], (asked[x]++ & 1) ^ 1)) break;
+                            if (lane == 0) {
                                 mbar_expect_tx(&bar.q_full[x], (uint32_t)(DP * 2 * tok * a.group));
                                 for (int b = 0; b < DP / 64; b++)
                                     tma_load_4d(sq + x * S::kTile + b * (128 * 128), &maps.q, 64 * b, 0, u.kvh, u.p.q0 + tok0 + x * tok, &bar.q_full[x]);
@@ -736,8 +736,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     if (v && edge) {
                         // rows past the sequence's end hold anything: 0 * NaN must not reach the sums
-                        ok = mbar_wait(&bar.edge, edges & 1, &bar.abort);
-                        edges++;
+                        if (!wait(&bar.edge, edges++ & 1)) break;
                         const int r0 = max(keys, 0);
                         for (int e = lane; e < (128 - r0) * (DP / 8); e += 32) {
                             const int r = r0 + e / (DP / 8), c = e % (DP / 8);
