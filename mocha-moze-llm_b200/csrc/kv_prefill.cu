@@ -419,6 +419,7 @@ __global__ void __launch_bounds__(kThreads, Smem32<DP>::kCtas) k_prefill(const _
 constexpr int kTcThreads = 384;  // warps 0-3 and 4-7: weights of the two tiles; 8: products; 9: copies; 10, 11: none
 constexpr int kTcUnits = 4;      // units that the copies may be ahead
 constexpr int kTcKeys = 128;
+constexpr int kWaitPolls = 1 << 18;  // of 3.9 us each: a second
 
 struct Maps {
     CUtensorMap q, k, v;
@@ -480,6 +481,18 @@ MB_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, bool 
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
         "r"(a), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
+}
+
+// Waits for phase `parity` of `bar`; false when *abort is set (another role of the CTA gave
+// up) or after kWaitPolls polls.  Polls and not cycles, for the clock runs on while another
+// process has the GPU, and what is awaited does not.
+MB_DEV bool wait_for(uint64_t *bar, uint32_t parity, const volatile int *abort)
+{
+    if (mb::as::mbar_test(bar, parity)) return true;
+    for (int n = 0;;) {
+        if (mb::as::mbar_test(bar, parity)) return true;
+        if (*abort || ++n > kWaitPolls) return false;
+    }
 }
 
 MB_DEV bool elect_one()
@@ -670,7 +683,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int i = bar.share.i, it = 0, edges = 0, units = 0, asked[2] = {0, 0};
         long long left = bar.share.end - bar.share.start;
         // together, for lanes that part here meet the warp's next barrier apart
-        auto wait = [&](uint64_t *b, uint32_t parity) { return ok = __all_sync(0xffffffffu, mbar_wait(b, parity, &bar.abort)); };
+        auto wait = [&](uint64_t *b, uint32_t parity) { return ok = __all_sync(0xffffffffu, wait_for(b, parity, &bar.abort)); };
         for (;; units++) {
             const bool more = left > 0;
             const int stop = more ? (int)min((long long)u.t.n, i + left) : 0, begin = i;
@@ -761,7 +774,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         constexpr uint32_t id_qk = base | ((128u >> 3) << 17), id_pv = base | (1u << 16) | ((uint32_t)(DP >> 3) << 17);
         int it = 0, steps[2] = {0, 0}, asked[2] = {0, 0};  // steps: weights taken; asked: queries taken
         auto wait = [&](uint64_t *b, uint32_t parity) {
-            ok = ok && __all_sync(0xffffffffu, mbar_wait(b, parity, &bar.abort));
+            ok = ok && __all_sync(0xffffffffu, wait_for(b, parity, &bar.abort));
             tc_fence_after();
             return ok;
         };
@@ -848,7 +861,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         uint32_t step = 0, pairs = 0;
         // false when a wait has run out, here or elsewhere in the CTA
         auto wait = [&](uint64_t *b, uint32_t parity) {
-            ok = __all_sync(0xffffffffu, mbar_wait(b, parity, &bar.abort));
+            ok = __all_sync(0xffffffffu, wait_for(b, parity, &bar.abort));
             tc_fence_after();
             return ok;
         };
