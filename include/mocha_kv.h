@@ -43,7 +43,8 @@ typedef struct {
  * needs are not used.  A sequence has at most 2^30 positions.  A needed page id outside [0, pages) reads as a page of zeros and is
  * not written.  Where `status` is not NULL, *status becomes at least 1 when such a page, or
  * an append position that the table or the angles do not hold, was met, and 2 when a
- * bounded wait inside a kernel ran out, which leaves outputs unwritten (it is never reset). */
+ * bounded wait inside a kernel ran out (it is never reset); the rows concerned, outputs and
+ * lse, are then NaN, so that a call without `status` shows it too. */
 typedef struct {
     int seqs, table_width;
     long long table_stride;
@@ -117,6 +118,14 @@ int mocha_kv_decode(const mocha_kv_pages *pages, const mocha_kv_seqs *seqs, cons
 int mocha_kv_prefill(const mocha_kv_pages *pages, const mocha_kv_seqs *seqs, const mocha_kv_scores *scores, int rows,
                      const int *q_start, const mocha_kv_rows *q, const mocha_kv_rows *out, float *lse,
                      void *workspace, unsigned long long workspace_bytes, void *stream);
+
+/* mocha_kv_prefill for tests of status 2: waits give up after wait_polls polls of 4 us, in
+ * place of as many as take a second, and on 16-bit pages, where drop is not 0, CTA b does not copy the
+ * values of its (b % drop)-th tile of keys, which its other warps then wait for. */
+int mocha_kv_prefill_check(const mocha_kv_pages *pages, const mocha_kv_seqs *seqs, const mocha_kv_scores *scores,
+                           int rows, const int *q_start, const mocha_kv_rows *q, const mocha_kv_rows *out, float *lse,
+                           void *workspace, unsigned long long workspace_bytes, void *stream, int wait_polls,
+                           int drop);
 
 #ifdef __cplusplus
 }

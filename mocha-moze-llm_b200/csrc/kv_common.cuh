@@ -81,7 +81,9 @@ struct Args {
     float *lse;
     const int *q_start;  // prefill
     int rows;
-    int2 *note;   // [CTAs] c_end, or -1 where no unit is cut, and rows of the unit
+    int wait_polls;  // of a wait in the prompt kernel before it gives up
+    int drop;  // tests: CTA b never copies the values of its key tile b % drop, so that waits run out
+    int2 *note;   // [CTAs] c_end, or -1 where no unit is cut, and rows of the unit; -1 - rows from a CTA that gave up
     Meta *meta;   // [CTAs]
     float *part;  // [CTAs][2][part rows][2 + padded dim]: outputs of all rows, then (m, l) of all rows
 };
@@ -231,6 +233,16 @@ __device__ __forceinline__ void lone_row(const Args &a, int seq, int p, int head
     if (a.lse && lane == 0) a.lse[(long long)row * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
+// A row of a CTA that gave up: not a number, so that nobody takes it for a result.  By a warp.
+template <typename T>
+MB_DEV void lost_row(const Args &a, long long row, int head)
+{
+    const int lane = threadIdx.x & 31;
+    const float x = __int_as_float(0x7fffffff);
+    if (lane * 4 < a.d) store4(reinterpret_cast<T *>(a.out) + row * a.o_row + head * a.o_head + lane * 4, make_float4(x, x, x, x));
+    if (a.lse && lane == 0) a.lse[row * a.heads + head] = x;
+}
+
 // ---- asynchronous copies ----------------------------------------------------------------
 
 MB_DEV void cp_async16(uint32_t dst, const void *src, bool ok)
@@ -282,6 +294,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 2) k_join(const __grid_consta
     __shared__ Joined s_part[kJoinWarps][32];
     __shared__ int s_items[kJoinMetas], s_warp[kJoinWarps], s_total;
     __shared__ int2 s_note[kJoinMetas];
+    __shared__ bool s_gave_up[kJoinMetas];
     mb::as::griddep_launch();
     mb::as::griddep_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -289,7 +302,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 2) k_join(const __grid_consta
     static_assert(kJoinMetas <= 32 * kJoinWarps, "a thread per note");
     int n = 0;
     if (tid < metas) {
-        const int2 note = s_note[tid] = __ldcg(a.note + tid);
+        int2 note = __ldcg(a.note + tid);
+        s_gave_up[tid] = note.y < 0;
+        if (note.y < 0) note.y = -1 - note.y;
+        s_note[tid] = note;
         if (note.x >= 0) n = note.x - tid < kJoinSerial ? (note.y + kJoinWarps - 1) / kJoinWarps : note.y;
     }
     int incl = n;
@@ -316,6 +332,14 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 2) k_join(const __grid_consta
         const bool serial = c_end - c < kJoinSerial;
         const int r = serial ? (item - first) * kJoinWarps + warp : item - first;
         const bool there = r < note.y;
+        if (PREFILL) {
+            bool lost = false;
+            for (int b = c + lane; b <= c_end; b += 32) lost |= s_gave_up[b];
+            if (__any_sync(0xffffffffu, lost)) {  // a part is missing
+                if (there && (serial || warp == 0)) lost_row<T>(a, mt.row0 + r / mt.ng, mt.head0 + r % mt.ng);
+                continue;
+            }
+        }
         Joined x{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
         constexpr int U = 4;  // parts in flight per warp
         if (there)

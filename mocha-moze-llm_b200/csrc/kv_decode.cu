@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
     mb::as::griddep_wait();
     long long start, end, per;
     if (!find_share<R::kTile, kWarps>(w, hh_n, s_warp, &s_seq, &s_rem, &start, &end, &per)) {
-        if (tid == 0) a.note[blockIdx.x].x = -1;
+        if (tid == 0) a.note[blockIdx.x] = make_int2(-1, 0);
         return;
     }
     Walk<R::kTile> in;  // the next tile to load
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
         in.next(a, hh_n);
     }
     if (left <= 0) {
-        if (tid == 0) a.note[blockIdx.x].x = -1;
+        if (tid == 0) a.note[blockIdx.x] = make_int2(-1, 0);
         return;
     }
     int left_in = left;  // from tile `in` on

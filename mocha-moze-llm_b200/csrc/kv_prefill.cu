@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, Smem32<DP>::kCtas) k_prefill(const _
     mb::as::griddep_launch();
     mb::as::griddep_wait();
     if (!find_share<kKeys, kThreads>(a, tokens, min_tiles, share)) {
-        if (tid == 0) a.note[blockIdx.x].x = -1;
+        if (tid == 0) a.note[blockIdx.x] = make_int2(-1, 0);
         return;
     }
     const Share h = share.out;
@@ -484,14 +484,44 @@ MB_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, bool 
 }
 
 // Waits for phase `parity` of `bar`; false when *abort is set (another role of the CTA gave
-// up) or after kWaitPolls polls.  Polls and not cycles, for the clock runs on while another
-// process has the GPU, and what is awaited does not.
-MB_DEV bool wait_for(uint64_t *bar, uint32_t parity, const volatile int *abort)
+// up) or after the call's number of polls.  Polls and not cycles, for the clock runs on while
+// another process has the GPU, and what is awaited does not.
+MB_DEV bool wait_for(const Args &a, uint64_t *bar, uint32_t parity, const volatile int *abort)
 {
     if (mb::as::mbar_test(bar, parity)) return true;
     for (int n = 0;;) {
         if (mb::as::mbar_test(bar, parity)) return true;
-        if (*abort || ++n > kWaitPolls) return false;
+        if (*abort || ++n > a.wait_polls) return false;
+    }
+}
+
+// The share of a CTA that gave up: its finished units' rows, and a note for the join.  Called
+// by all threads.
+template <int T, typename E>
+MB_DEV void lost_share(const Args &a, const Share &h, int tokens)
+{
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int2 note = make_int2(-1, -1);
+    Units<T> u;
+    u.start(a, h, tokens);
+    int i = h.i;
+    for (long long left = h.end - h.start; left > 0; i = 0) {
+        const int tok0 = u.block * tokens, ntok = min(tokens, u.p.nq - tok0), stop = (int)min((long long)u.t.n, i + left);
+        if (i == 0 && stop < u.t.n) {
+            note = make_int2((int)div64(h.end - 1 + (u.t.n - stop), h.per), -1 - ntok * a.group);
+            if (threadIdx.x == 0) a.meta[blockIdx.x] = Meta{u.p.q0 + tok0, u.kvh * a.group, a.group, u.seq, u.p.pos(tok0)};
+        } else if (i == 0) {
+            for (int r = warp; r < ntok * a.group; r += warps) {
+                const int t = div(a.group_div, r);
+                lost_row<E>(a, u.p.q0 + tok0 + t, u.kvh * a.group + r - t * a.group);
+            }
+        }
+        left -= stop - i + (stop == u.t.n ? kUnitEnd : 0);
+        if (left > 0) u.next(a, tokens);
+    }
+    if (threadIdx.x == 0) {
+        a.note[blockIdx.x] = note;
+        if (a.status) atomicMax(a.status, 2);
     }
 }
 
@@ -660,8 +690,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // swizzled tiles are laid out by address: their base has to be a multiple of 1024
     const bool any = find_share<kTcKeys, kTcThreads>(a, tokens, min_tiles, share), placed = (smem_u32(smem) & 1023) == 0;
     if (!any || !placed) {
-        if (!placed && tid == 0 && a.status) atomicMax(a.status, 2);
-        if (tid == 0) a.note[blockIdx.x].x = -1;
+        if (any) lost_share<kTcKeys, T>(a, share.out, tokens);
+        else if (tid == 0) a.note[blockIdx.x] = make_int2(-1, 0);
         return;
     }
     if (tid == 0) bar.share = share.out;
@@ -683,7 +713,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int i = bar.share.i, it = 0, edges = 0, units = 0, asked[2] = {0, 0};
         long long left = bar.share.end - bar.share.start;
         // together, for lanes that part here meet the warp's next barrier apart
-        auto wait = [&](uint64_t *b, uint32_t parity) { return ok = __all_sync(0xffffffffu, wait_for(b, parity, &bar.abort)); };
+        auto wait = [&](uint64_t *b, uint32_t parity) { return ok = __all_sync(0xffffffffu, wait_for(a, b, parity, &bar.abort)); };
         for (;; units++) {
             const bool more = left > 0;
             const int stop = more ? (int)min((long long)u.t.n, i + left) : 0, begin = i;
@@ -729,6 +759,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int v = 0; v < 2 && ok; v++, it++) {
                     const int st = it % S::kStages;
                     if (!wait(&bar.kv_empty[st], ((it / S::kStages) & 1) ^ 1)) break;
+                    if (v && a.drop && it / 2 == blockIdx.x % a.drop) continue;
                     const uint32_t dst = skv + st * S::kTile;
                     uint64_t *full = v && edge ? &bar.edge : &bar.kv_full[st];
                     if (lane == 0) mbar_expect_tx(full, (uint32_t)(boxes * box * DP * 2));
@@ -774,7 +805,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         constexpr uint32_t id_qk = base | ((128u >> 3) << 17), id_pv = base | (1u << 16) | ((uint32_t)(DP >> 3) << 17);
         int it = 0, steps[2] = {0, 0}, asked[2] = {0, 0};  // steps: weights taken; asked: queries taken
         auto wait = [&](uint64_t *b, uint32_t parity) {
-            ok = ok && __all_sync(0xffffffffu, wait_for(b, parity, &bar.abort));
+            ok = ok && __all_sync(0xffffffffu, wait_for(a, b, parity, &bar.abort));
             tc_fence_after();
             return ok;
         };
@@ -861,7 +892,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         uint32_t step = 0, pairs = 0;
         // false when a wait has run out, here or elsewhere in the CTA
         auto wait = [&](uint64_t *b, uint32_t parity) {
-            ok = __all_sync(0xffffffffu, wait_for(b, parity, &bar.abort));
+            ok = __all_sync(0xffffffffu, wait_for(a, b, parity, &bar.abort));
             tc_fence_after();
             return ok;
         };
@@ -1061,10 +1092,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     __syncthreads();
     if (bar.abort) {
-        // a wait ran out: no notes for the join, and the copies in flight land first
+        // a wait ran out: the copies in flight land first
         if (tid == 0) {
-            a.note[blockIdx.x].x = -1;
-            if (a.status) atomicMax(a.status, 2);
             const long long t0 = clock64();
             while (clock64() - t0 < kWaitCycles / 64) {
             }
@@ -1075,7 +1104,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_after();
         tmem_free(tmem, 512);
     }
-    if (!bar.bad || bar.abort) return;
+    if (bar.abort) {
+        lost_share<kTcKeys, T>(a, bar.share, tokens);
+        return;
+    }
+    if (!bar.bad) return;
     // rows of whole units that are not finite, once more without the keys that they do not see
     Units<kTcKeys> u;
     u.start(a, bar.share, tokens);
@@ -1186,11 +1219,12 @@ extern "C" int mocha_kv_workspace(const mocha_kv_pages *pages, int heads, int pr
     return 0;
 }
 
-extern "C" int mocha_kv_prefill(const mocha_kv_pages *pages, const mocha_kv_seqs *seqs, const mocha_kv_scores *scores,
-                                int rows, const int *q_start, const mocha_kv_rows *q, const mocha_kv_rows *out,
-                                float *lse, void *workspace, unsigned long long workspace_bytes, void *stream)
+namespace {
+
+int prefill(const char *who, const mocha_kv_pages *pages, const mocha_kv_seqs *seqs, const mocha_kv_scores *scores, int rows,
+            const int *q_start, const mocha_kv_rows *q, const mocha_kv_rows *out, float *lse, void *workspace,
+            unsigned long long workspace_bytes, void *stream, int wait_polls, int drop)
 {
-    const char *who = "mocha_kv_prefill";
     if (check_pages(who, pages) || check_seqs(who, seqs) || check_scores(who, pages, scores)) return 1;
     const int b = type_bytes(pages->type), d = pages->head_dim;
     if (rows < 0 || rows > kMostPositions) return fail(who, "rows must not be negative, nor more than 2^30");
@@ -1202,6 +1236,8 @@ extern "C" int mocha_kv_prefill(const mocha_kv_pages *pages, const mocha_kv_seqs
     Args a = make_args(pages, seqs, scores, q, out, lse);
     a.q_start = q_start;
     a.rows = rows;
+    a.wait_polls = wait_polls;
+    a.drop = drop;
     if (!workspace || !aligned(workspace) || workspace_bytes < kv::prefill_workspace(pages->type, d))
         return fail(who, "workspace missing, not 16-byte aligned or smaller than mocha_kv_workspace says");
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -1212,4 +1248,24 @@ extern "C" int mocha_kv_prefill(const mocha_kv_pages *pages, const mocha_kv_seqs
     case MOCHA_KV_F16: return narrow ? run_tc<__half, 64>(a, pages, workspace, dev, s) : run_tc<__half, 128>(a, pages, workspace, dev, s);
     default: return narrow ? run_tc<__nv_bfloat16, 64>(a, pages, workspace, dev, s) : run_tc<__nv_bfloat16, 128>(a, pages, workspace, dev, s);
     }
+}
+
+}  // namespace
+
+extern "C" int mocha_kv_prefill(const mocha_kv_pages *pages, const mocha_kv_seqs *seqs, const mocha_kv_scores *scores,
+                                int rows, const int *q_start, const mocha_kv_rows *q, const mocha_kv_rows *out,
+                                float *lse, void *workspace, unsigned long long workspace_bytes, void *stream)
+{
+    return prefill("mocha_kv_prefill", pages, seqs, scores, rows, q_start, q, out, lse, workspace, workspace_bytes, stream,
+                   kWaitPolls, 0);
+}
+
+extern "C" int mocha_kv_prefill_check(const mocha_kv_pages *pages, const mocha_kv_seqs *seqs, const mocha_kv_scores *scores,
+                                      int rows, const int *q_start, const mocha_kv_rows *q, const mocha_kv_rows *out,
+                                      float *lse, void *workspace, unsigned long long workspace_bytes, void *stream,
+                                      int wait_polls, int drop)
+{
+    const char *who = "mocha_kv_prefill_check";
+    if (wait_polls < 0 || drop < 0) return fail(who, "wait_polls and drop must not be negative");
+    return prefill(who, pages, seqs, scores, rows, q_start, q, out, lse, workspace, workspace_bytes, stream, wait_polls, drop);
 }

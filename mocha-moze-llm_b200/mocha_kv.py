@@ -55,6 +55,8 @@ _SIGS = {
                         C.c_ulonglong, C.c_void_p],
     "mocha_kv_prefill": [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                          C.c_void_p, C.c_ulonglong, C.c_void_p],
+    "mocha_kv_prefill_check": [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                               C.c_void_p, C.c_void_p, C.c_ulonglong, C.c_void_p, C.c_int, C.c_int],
 }
 
 _lib = None

@@ -125,6 +125,12 @@ def test_prefill_rows(kv, capfd):
     assert "q_start" in capfd.readouterr().err
 
 
+@pytest.mark.parametrize("polls,drop", [(-1, 0), (1, -1)])
+def test_prefill_check(kv, capfd, polls, drop):
+    assert kv._load().mocha_kv_prefill_check(None, None, None, 0, None, None, None, None, None, 0, None, polls, drop) == 1
+    assert "wait_polls" in capfd.readouterr().err
+
+
 def test_workspace(kv):
     lib = kv._load()
     got = C.c_ulonglong()
