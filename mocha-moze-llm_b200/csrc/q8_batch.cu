@@ -1883,8 +1883,12 @@ int generate_impl(mocha_q8b *h, int nseq, const int *prompts, int prompt_len, co
     const int wave = std::min(h->slots, std::max(1, h->max_rows / prompt_len));
     if (wave < 1) return 1;
     if (h->out_stride < max_new) {
+        // the captured step holds the old buffer and its stride
+        if (h->g_step) cudaGraphExecDestroy(h->g_step);
+        h->g_step = nullptr;
         if (h->out_tokens) cudaFree(h->out_tokens);
         h->out_tokens = nullptr;
+        h->out_stride = 0;
         if (dalloc(&h->out_tokens, (size_t)h->slots * max_new)) return 1;
         h->out_stride = max_new;
     }
