@@ -9,13 +9,15 @@ The calls enqueue on torch's current stream of the pages' device and can be capt
 CUDA graphs; outputs and workspaces that the caller does not pass come from torch's
 allocator, call by call.  Arguments that do not fit raise ValueError before anything is
 enqueued; an error from the library raises RuntimeError.  There are no gradients: a tensor
-that requires one is refused unless gradients are off.  No reference counterpart.
+that requires one is refused unless gradients are off, and so is one with a tangent of
+forward mode.  No reference counterpart.
 """
 from __future__ import annotations
 
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 import mocha_native
 
@@ -62,6 +64,20 @@ _SIGS = {
 _lib = None
 
 
+def _no_gradient(names, *tensors):
+    if forward_ad._current_level < 0:
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                break
+        else:
+            return
+    for name, t in zip(names.split(), tensors):
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires a gradient, which these operators do not have")
+        if t is not None and forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} has a tangent, which these operators do not carry on")
+
+
 def _load() -> C.CDLL:
     global _lib
     if _lib is None:
@@ -88,8 +104,7 @@ class KvPages:
             raise ValueError("k and v must be float32, float16 or bfloat16, of one type")
         if k.stride() != v.stride() or k.stride(3) != 1:
             raise ValueError("k and v must have the same strides, the last one 1")
-        if k.requires_grad or v.requires_grad:
-            raise ValueError("pages must not require gradients")
+        _no_gradient("k v", k, v)
         if k.device.type != "cuda" or k.device != v.device:
             raise ValueError("k and v must be on one CUDA device")
         self.k, self.v = k, v
@@ -123,8 +138,6 @@ class KvPages:
         if (len(shape) != 3 or t.dtype is not dtype or t.get_device() != self._index or shape[0] != rows or
                 shape[2] != self.head_dim or (heads is not None and shape[1] != heads)):
             raise ValueError(f"{name} must be [{rows}, {heads or 'heads'}, {self.head_dim}] of {dtype} on the pages' device")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{name} requires a gradient, which these operators do not have")
         row, head, one = t.stride()
         if one != 1:
             raise ValueError(f"{name}: a head's values must be contiguous")
@@ -192,6 +205,7 @@ class KvPages:
                          2 * cos.shape[1],
                          int(bool(interleaved)))
         seqs = self._seqs(table, None, status)
+        _no_gradient("q k v q_out cos sin pages.k pages.v", q, k, v, q_out, cos, sin, self.k, self.v)
         if lib.mocha_kv_append(self._pages, C.addressof(seqs), rows, self._int(seq, "seq", rows),
                                self._int(pos, "pos", rows), _TYPES[k.dtype], heads, qr and C.addressof(qr),
                                C.addressof(kr), C.addressof(vr), orr and C.addressof(orr), C.addressof(rope),
@@ -212,6 +226,7 @@ class KvPages:
         orr = self._rows(out, "out", self.dtype, n, heads)
         seqs = self._seqs(table, kv_len, status)
         scores = self._scores(heads, n, scale, window, prefix, cap, slopes)
+        _no_gradient("q slopes out lse pages.k pages.v", q, slopes, out, lse, self.k, self.v)
         size, space = self._space(lib, heads, 0)
         if lib.mocha_kv_decode(self._pages, C.addressof(seqs), C.addressof(scores), C.addressof(qr), C.addressof(orr),
                                self._lse(lse, n, heads), space.data_ptr(), size,
@@ -232,6 +247,7 @@ class KvPages:
         orr = self._rows(out, "out", self.dtype, rows, heads)
         seqs = self._seqs(table, kv_len, status)
         scores = self._scores(heads, n, scale, window, prefix, cap, slopes)
+        _no_gradient("q slopes out lse pages.k pages.v", q, slopes, out, lse, self.k, self.v)
         size, space = self._space(lib, heads, 1)
         if lib.mocha_kv_prefill(self._pages, C.addressof(seqs), C.addressof(scores), rows,
                                 self._int(q_start, "q_start", n + 1), C.addressof(qr), C.addressof(orr),

@@ -1,4 +1,5 @@
-"""The paged key/value operators at the edges of what they take: waits that run out."""
+"""The paged key/value operators at the edges of what they take: waits that run out, tensors
+that gradients are asked of."""
 import ctypes
 
 import pytest
@@ -45,3 +46,58 @@ def test_waits_that_run_out(kv, dtype, dim):
         # drop 1 stops every CTA; 70 the first ones and those from 70 on, of the 134 that have shares of 6
         assert lost.any() == (drop > 0) and lost.all() >= (drop == 1) and not (drop == 70 and lost.all())
     assert torch.equal(cache.prefill(q, start, table, ints(lens)), want)
+
+
+# ---- gradients -------------------------------------------------------------------------
+
+def test_gradients_and_tangents_are_refused(kv):
+    """Every floating tensor of every call, by reverse and by forward mode; none of them would
+    get anything."""
+    k, v, table = pool([40, 40], 2, 64, 16, BF16)
+    cache = kv.KvPages(k, v)
+    lens, start, seq, pos = ints([40, 40]), ints([0, 1, 2]), ints([0, 1]), ints([3, 4])
+    q, new = queries(2, 4, 64, BF16), queries(2, 2, 64, BF16)
+    cos, sin = torch.ones(9, 32, device=DEV), torch.zeros(9, 32, device=DEV)
+    slopes = torch.ones(4, device=DEV)
+
+    def calls(x):
+        """name -> the call with that tensor put through x"""
+        lse = torch.zeros(2, 4, device=DEV)
+        out = torch.zeros_like(q)
+        return {
+            "append q": lambda: cache.append(x(q), new, new, seq, pos, table, cos=cos, sin=sin),
+            "append k": lambda: cache.append(q, x(new), new, seq, pos, table, cos=cos, sin=sin),
+            "append v": lambda: cache.append(q, new, x(new), seq, pos, table, cos=cos, sin=sin),
+            "append cos": lambda: cache.append(q, new, new, seq, pos, table, cos=x(cos), sin=sin),
+            "append sin": lambda: cache.append(q, new, new, seq, pos, table, cos=cos, sin=x(sin)),
+            "append q_out": lambda: cache.append(q, new, new, seq, pos, table, cos=cos, sin=sin, q_out=x(out)),
+            "decode q": lambda: cache.decode(x(q), table, lens),
+            "decode slopes": lambda: cache.decode(q, table, lens, slopes=x(slopes)),
+            "decode out": lambda: cache.decode(q, table, lens, out=x(out)),
+            "decode lse": lambda: cache.decode(q, table, lens, lse=x(lse)),
+            "prefill q": lambda: cache.prefill(x(q), start, table, lens),
+            "prefill slopes": lambda: cache.prefill(q, start, table, lens, slopes=x(slopes)),
+            "prefill lse": lambda: cache.prefill(q, start, table, lens, lse=x(lse)),
+            "pages k": lambda: kv.KvPages(x(k), v).decode(q, table, lens),
+            "pages v": lambda: kv.KvPages(k, x(v)).decode(q, table, lens),
+        }
+
+    for call in calls(lambda t: t).values():
+        call()
+    for call in calls(lambda t: t.clone().requires_grad_()).values():
+        with pytest.raises(ValueError):
+            call()
+        with torch.no_grad():
+            call()
+    with torch.autograd.forward_ad.dual_level():
+        for call in calls(lambda t: torch.autograd.forward_ad.make_dual(t.clone(), torch.ones_like(t))).values():
+            with pytest.raises(ValueError):
+                call()
+        cache.decode(q, table, lens, slopes=slopes)
+    with pytest.raises((ValueError, RuntimeError)):
+        torch.func.jvp(lambda t: cache.decode(t, table, lens), (q,), (q,))
+    with torch.no_grad():
+        late = kv.KvPages(k.clone().requires_grad_(), v)
+        late.decode(q, table, lens)
+    with pytest.raises(ValueError):
+        late.decode(q, table, lens)
