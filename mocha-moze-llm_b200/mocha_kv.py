@@ -149,6 +149,8 @@ class KvPages:
                     not slopes.is_contiguous()):
                 raise ValueError(f"slopes must be a contiguous float32 vector of {heads} on the pages' device")
             slopes = slopes.data_ptr()
+        if not 0 <= window < 1 << 31:  # ctypes would keep the low 32 bits
+            window = -1 if window < 0 else (1 << 31) - 1
         return _Scores(heads, window, self.head_dim ** -0.5 if scale is None else scale, cap,
                        None if prefix is None else self._int(prefix, "prefix", n), slopes)
 

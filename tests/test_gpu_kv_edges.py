@@ -101,3 +101,20 @@ def test_gradients_and_tangents_are_refused(kv):
         late.decode(q, table, lens)
     with pytest.raises(ValueError):
         late.decode(q, table, lens)
+
+
+# ---- options ---------------------------------------------------------------------------
+
+def test_windows_past_32_bits(kv):
+    """A window that no 32-bit number holds is wider than any sequence, or negative."""
+    k, v, table = pool([40, 9], 2, 64, 16, BF16)
+    cache = kv.KvPages(k, v)
+    lens, q, start = ints([40, 9]), queries(2, 4, 64, BF16), ints([0, 1, 2])
+    for window in (2 ** 31, 2 ** 32 + 5, 2 ** 63 - 1, 2 ** 64 + 1):
+        assert torch.equal(cache.decode(q, table, lens, window=window), cache.decode(q, table, lens))
+        assert torch.equal(cache.prefill(q, start, table, lens, window=window), cache.prefill(q, start, table, lens))
+    for window in (-1, -2 ** 32 + 5, -2 ** 63):
+        with pytest.raises(RuntimeError):
+            cache.decode(q, table, lens, window=window)
+        with pytest.raises(RuntimeError):
+            cache.prefill(q, start, table, lens, window=window)
