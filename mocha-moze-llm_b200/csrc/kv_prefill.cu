@@ -596,12 +596,13 @@ MB_DEV void add2(float &d0, float &d1, float a0, float a1)
 // cap tanh(k s) + bias of a row of scores, bias = base - slope c for column c, where cap is in
 // log2.  Where all of a warp's |k s| are within tanh_of's polynomial, as those of ordinary
 // scores under an ordinary cap are, on the FMA units alone: its coefficients take up k and cap.
-MB_DEV void cap_scores(float (&s)[128], float cap, float k, float slope, float base)
+// Only rows that exist (`there`) have a say: what the others hold is left over from other calls.
+MB_DEV void cap_scores(float (&s)[128], float cap, float k, float slope, float base, bool there)
 {
     float big = 0.f;
 #pragma unroll
     for (int c = 0; c < 128; c += 2) big = fmaxf(big, fmaxf(fabsf(s[c]), fabsf(s[c + 1])));
-    if (fabsf(k) > 256.f || __any_sync(0xffffffffu, big * fabsf(k) > kTanhPart)) {  // k^8 has to be finite
+    if (fabsf(k) > 256.f || __any_sync(0xffffffffu, there && big * fabsf(k) > kTanhPart)) {  // k^8 has to be finite
 #pragma unroll
         for (int c = 0; c < 128; c++) s[c] = fmaf(cap, tanh_of(s[c] * k), fmaf(-slope, (float)c, base));
     } else {
@@ -926,7 +927,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             const bool ahead = a.slopes && j0 < pre && j0 + kTcKeys > p0 + 1;
                             const float by = ahead ? 0.f : slope, base = by * (float)(p - j0);
                             if (a.cap > 0.f) {
-                                cap_scores(s, a.cap * kLog2e, a.scale / a.cap, by, base);
+                                cap_scores(s, a.cap * kLog2e, a.scale / a.cap, by, base, t < tok && xt + t < d.ntok);
                             } else {
 #pragma unroll
                                 for (int c = 0; c < 128; c++) s[c] = fmaf(s[c], a.scale * kLog2e, fmaf(-by, (float)c, base));

@@ -118,3 +118,21 @@ def test_windows_past_32_bits(kv):
             cache.decode(q, table, lens, window=window)
         with pytest.raises(RuntimeError):
             cache.prefill(q, start, table, lens, window=window)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [36, 5])
+def test_caps_do_not_see_other_calls(kv, dtype, rows):
+    """The same bits whatever ran before: a group of 7 heads leaves the last two of a tile's 128
+    rows without queries, a short piece more, and what a call before left there is no score."""
+    k, v, table = pool([600], 2, 64, 16, dtype)
+    cache = kv.KvPages(k, v)
+    lens, start = ints([600]), ints([0, rows])
+    q = queries(rows, 14, 64, dtype, scale=0.5)
+    full = queries(600, 16, 64, dtype, 3)
+    got = []
+    for size in (0.0, 1e3, 1.0):
+        for _ in range(3):
+            cache.prefill(full * size, ints([0, 600]), table, lens)
+        got.append(cache.prefill(q, start, table, lens, cap=30.0))
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
