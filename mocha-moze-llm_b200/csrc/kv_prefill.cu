@@ -602,12 +602,15 @@ MB_DEV void cap_scores(float (&s)[128], float cap, float k, float slope, float b
     float big = 0.f;
 #pragma unroll
     for (int c = 0; c < 128; c += 2) big = fmaxf(big, fmaxf(fabsf(s[c]), fabsf(s[c + 1])));
-    if (fabsf(k) > 256.f || __any_sync(0xffffffffu, there && big * fabsf(k) > kTanhPart)) {  // k^8 has to be finite
+    const float kk = k * k, c0 = kTanh0 * cap * k, c1 = kTanh1 * cap * k * kk, c2 = kTanh2 * cap * k * kk * kk,
+                c3 = kTanh3 * cap * k * kk * kk * kk, c4 = kTanh4 * cap * k * kk * kk * kk * kk;
+    // the coefficients and the scores' squares have to be normal numbers: c4 within these bounds
+    // holds |k| between 2^-18 and 2^17
+    const bool normal = fabsf(c4) >= 0x1p-120f && fabsf(c4) <= 0x1p100f;
+    if (!normal || __any_sync(0xffffffffu, there && big * fabsf(k) > kTanhPart)) {
 #pragma unroll
         for (int c = 0; c < 128; c++) s[c] = fmaf(cap, tanh_of(s[c] * k), fmaf(-slope, (float)c, base));
     } else {
-        const float kk = k * k, c0 = kTanh0 * cap * k, c1 = kTanh1 * cap * k * kk, c2 = kTanh2 * cap * k * kk * kk,
-                    c3 = kTanh3 * cap * k * kk * kk * kk, c4 = kTanh4 * cap * k * kk * kk * kk * kk;
 #pragma unroll
         for (int c = 0; c < 128; c += 2) {
             float t0, t1, y0, y1;

@@ -136,3 +136,23 @@ def test_caps_do_not_see_other_calls(kv, dtype, rows):
             cache.prefill(full * size, ints([0, 600]), table, lens)
         got.append(cache.prefill(q, start, table, lens, cap=30.0))
     assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+@pytest.mark.parametrize("scale,cap,size", [(2.0 ** -30, 50.0, 12000.0), (2.0 ** -39, 1.0, 2.0 ** 17),
+                                            (2.0 ** 10, 2.0 ** -10, 2.0 ** -42), (0.125, 50.0, 9e-5)])
+def test_caps_over_scores_of_any_size(kv, prefill, scale, cap, size):
+    """Products far from 1 under a small or large scale: scores of a tenth of the cap and up to
+    half of it, where tanh is neither its argument nor 1."""
+    k, v, table = pool([300], 2, 64, 16, BF16)
+    k *= 2.0 ** 16
+    cache = kv.KvPages(k, v)
+    q = queries(40, 4, 64, BF16, scale=size)
+    z = (ref.gather(k, table, 0, 300)[0] @ q[:, 0].double().T * scale / cap).abs()
+    assert 0.05 < z.median() < 0.2 and z.max() < 0.6, (float(z.median()), float(z.max()))
+    want, _, tol, _ = ref.attend(q, ref.gather(k, table, 0, 300), ref.gather(v, table, 0, 300), range(260, 300), scale,
+                                 cap=cap, dtype=BF16)
+    if prefill:
+        close(cache.prefill(q, ints([0, 40]), table, ints([300]), scale=scale, cap=cap), want, tol)
+    else:
+        close(cache.decode(q[-1:].contiguous(), table, ints([300]), scale=scale, cap=cap), want[-1:], tol[-1:])
