@@ -23,8 +23,6 @@
 // first keys) and the join.  One sequence of 777 in fp32: 10.7 us, all of it latency.  A
 // prefetch of the next tile into L2 cost 10 % at the power limit; halves of a tile as copy
 // groups of their own changed nothing.
-#include <type_traits>
-
 #include "kv_common.cuh"
 
 namespace {
@@ -465,7 +463,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         s[t][n][e] = fmaf(s[t][n][e], k2, -m[2 * n + (e & 1)]);
-                        past |= s[t][n][e] > 8.f;
+                        past |= s[t][n][e] > 8.f + kLift<T>;
                     }
             if (__any_sync(0xffffffffu, past)) {
 #pragma unroll
@@ -477,7 +475,8 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) by = fmaxf(by, __shfl_xor_sync(0xffffffffu, by, o));
                     const bool first = !(seen >> i & 1);
-                    if (first ? by > -INFINITY : by > 0.f) {
+                    if (first ? by > -INFINITY : by > kLift<T>) {
+                        by -= kLift<T>;
                         const float f = first ? 0.f : ex2(-by);
                         seen |= 1u << i;
                         m[i] += by;

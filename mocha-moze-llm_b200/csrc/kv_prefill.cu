@@ -4,8 +4,6 @@
 // row r of the unit is token r / group, head r % group, so the heads of a group share the
 // key and value tiles and a short piece still fills a tile.  Its key tiles are shared out
 // over the CTAs (kv_common.cuh).
-#include <type_traits>
-
 #include "kv_common.cuh"
 
 namespace {
@@ -973,7 +971,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                 }
                             }
                         }
-                        const float sub = m == -INFINITY ? 0.f : -m * k2;
+                        const float sub = m == -INFINITY ? 0.f : fmaf(-m, k2, kLift<T>);
                         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int b = 0; b < 4; b++) {
@@ -1073,10 +1071,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 if (mine) {
                     if (!whole) {
-                        part[(size_t)256 * DP + 2 * at] = m == -INFINITY ? m : m * k2;
+                        part[(size_t)256 * DP + 2 * at] = m == -INFINITY ? m : fmaf(m, k2, -kLift<T>);
                         part[(size_t)256 * DP + 2 * at + 1] = l;
                     } else {
-                        if (a.lse) a.lse[row * a.heads + head] = m == -INFINITY ? m : (m * k2 + log2f(l)) * kLn2;
+                        if (a.lse) a.lse[row * a.heads + head] = m == -INFINITY ? m : (fmaf(m, k2, -kLift<T>) + log2f(l)) * kLn2;
                         if (bad) bar.bad = 1;
                     }
                 }

@@ -1,6 +1,7 @@
 """The paged key/value operators at the edges of what they take: waits that run out, tensors
 that gradients are asked of."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -156,3 +157,43 @@ def test_caps_over_scores_of_any_size(kv, prefill, scale, cap, size):
         close(cache.prefill(q, ints([0, 40]), table, ints([300]), scale=scale, cap=cap), want, tol)
     else:
         close(cache.decode(q[-1:].contiguous(), table, ints([300]), scale=scale, cap=cap), want[-1:], tol[-1:])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("prefill", [False, True])
+@pytest.mark.parametrize("top", [0.0, 1.0])
+def test_many_weights_far_below_the_largest(kv, prefill, dtype, top):
+    """One key 25.5 powers of two above 131071 others, whose weights together are W = 0.28 % of its
+    own, in so many sequences (over the same pages) that whole ones fall to one CTA: with a value
+    of `top` against theirs of -1 the output is (top - W) / (1 + W).  It may be off by
+      u |o|, its own rounding;
+      n 2^-32: an fp16 weight is off by at most 2^-25, the largest being 2^7 (bf16: 2^-8 W);
+      n 2^-24 times the largest sum on the way, top + W, for a product that is added to an fp32
+      sum loses what lies below that sum's last place (beside a top of 1, more than all of W);
+      60 2^-24 W, the exponents' last places (scores of 25.5), and 2^-22 W for the rest.
+    lse is a sum of n fp32 weights, at most 2048 of them one after the other."""
+    n, page = 131072, 64
+    seqs, rows = (160, 256) if prefill else (640, 1)
+    k = torch.zeros(n // page, 1, page, 64, device=DEV, dtype=dtype)
+    v = torch.full_like(k, -1.0)
+    k[..., 0] = -1.0
+    k[0, 0, 0, 0] = 0.0
+    v[0, 0, 0] = top
+    table = torch.arange(n // page, device=DEV, dtype=torch.int32).repeat(seqs, 1)
+    q = torch.zeros(seqs * rows, 1, 64, device=DEV, dtype=dtype)
+    q[:, 0, 0] = 1.0
+    lens = ints([n] * seqs)
+    cache = kv.KvPages(k, v)
+    lse = torch.empty(seqs * rows, 1, device=DEV)
+    scale = 25.5 * math.log(2.0)
+    if prefill:
+        out = cache.prefill(q, ints(range(0, seqs * rows + 1, rows)), table, lens, scale=scale, lse=lse)
+    else:
+        out = cache.decode(q, table, lens, scale=scale, lse=lse)
+    w = torch.arange(n - rows, n, device=DEV, dtype=torch.float64).repeat(seqs) * 2.0 ** -25.5
+    want = ((top - w) / (1 + w))[:, None, None]
+    most = float(w.max())
+    weights = n * 2.0 ** -32 if dtype == F16 else 2.0 ** -8 * most
+    tol = ref.unit(dtype) * want.abs() + weights + n * 2.0 ** -24 * (top + most) + (60 * 2.0 ** -24 + 2.0 ** -22) * most
+    close(out, want, tol)
+    assert float((lse[:, 0].double() - torch.log1p(w)).abs().max()) <= 2048 * 2.0 ** -24 + 60 * 2.0 ** -24 * most + 2.0 ** -22
