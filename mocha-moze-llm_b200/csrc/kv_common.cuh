@@ -175,6 +175,20 @@ MB_DEV T from_f32(float x)
     return (T)x;
 }
 
+// Zero if four values are finite, NaN else.
+MB_DEV float load_zero4(const float *p)
+{
+    const float4 x = *reinterpret_cast<const float4 *>(p);
+    return fmaf(x.x, 0.f, fmaf(x.y, 0.f, fmaf(x.z, 0.f, x.w * 0.f)));
+}
+template <typename T>
+MB_DEV float load_zero4(const T *p)
+{
+    const uint2 r = *reinterpret_cast<const uint2 *>(p);
+    const T *x = reinterpret_cast<const T *>(&r);
+    return fmaf(to_f32(x[0]), 0.f, fmaf(to_f32(x[1]), 0.f, fmaf(to_f32(x[2]), 0.f, to_f32(x[3]) * 0.f)));
+}
+
 MB_DEV void store4(float *p, float4 x) { *reinterpret_cast<float4 *>(p) = x; }
 MB_DEV void store4(__half *p, float4 x)
 {
@@ -187,9 +201,44 @@ MB_DEV void store4(__nv_bfloat16 *p, float4 x)
     *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<uint2 *>(h);
 }
 
-// One row of a prompt's attention by a warp, reading only the keys that the row sees: for
-// the rows to which a tile's matrix product carried an infinite or NaN value of a key that
-// they do not see (0 * inf).  Rare, so written for size.
+// Whether a value that is not finite lies at a key which a prompt's row at position p does not
+// see, in the tiles of T keys of its unit, whose rows stand at [pa, pb]: only then can it have
+// reached the row's output (0 * inf).  By a warp, a key per lane; keys the row sees are not read.
+template <typename T, int TILE>
+__device__ __forceinline__ bool unseen_values(const Args &a, int seq, int p, int head, int pa, int pb)
+{
+    const int lane = threadIdx.x & 31, len = seq_len(a, seq), pre = seq_prefix(a, seq, len);
+    const int kvh = div(a.group_div, head), lo = a.window ? max(p - a.window + 1, 0) : 0;
+    Tiles<TILE> t;
+    t.set(a, len, pre, pa, min(pb + 1, len) - 1);
+    const int end = min(t.n * TILE + (t.lo_t - t.pre_t) * TILE, len);
+    bool bad = false;
+    // past the prefix, before the window, after the row
+#pragma unroll 1
+    for (int part = 0; part < 3 && !bad; part++) {
+        const int j0 = part == 0 ? pre : part == 1 ? t.lo_t * TILE : max(p + 1, t.lo_t * TILE);
+        const int j1 = part == 0 ? min(t.pre_t * TILE, len) : part == 1 ? min(lo, end) : end;
+#pragma unroll 1
+        for (int jb = j0; jb < j1 && !bad; jb += 32) {
+            const int j = jb + lane;
+            float worst = 0.f;
+            if (j < j1 && !visible(j, p, len, pre, a.window)) {
+                const int id = __ldg(a.table + (long long)seq * a.table_stride + div(a.page, j));
+                if ((unsigned)id < (unsigned)a.pages) {
+                    const T *v = reinterpret_cast<const T *>(a.v) + id * a.ps + kvh * a.hs + (long long)(j - div(a.page, j) * a.page.d) * a.ts;
+#pragma unroll 4
+                    for (int i = 0; i < a.d; i += 4) worst += load_zero4(v + i);
+                }
+            }
+            bad = __any_sync(0xffffffffu, !(worst == 0.f));
+        }
+    }
+    return bad;
+}
+
+// One row of a prompt's attention by a warp, reading only the keys that the row sees, where
+// unseen_values says so.  Rare, so written for size.  The row's lse is right without it: masked
+// scores are replaced, not multiplied.
 template <typename T>
 __device__ __forceinline__ void lone_row(const Args &a, int seq, int p, int head, int row)
 {
@@ -200,11 +249,12 @@ __device__ __forceinline__ void lone_row(const Args &a, int seq, int p, int head
     const float slope = a.slopes ? a.slopes[head] : 0.f;
     float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
     const int hi = min(p + 1, len), lo = max(a.window ? max(p - a.window + 1, 0) : 0, pre);
+    bool known = false;  // every value of the row is NaN, whatever else it sees
 #pragma unroll 1
     for (int part = 0; part < 2; part++) {
         const int j0 = part ? lo : 0, j1 = part ? hi : pre;
 #pragma unroll 1
-        for (int jb = j0; jb < j1; jb += 32) {
+        for (int jb = j0; jb < j1 && !known; jb += 32) {
             const int j = jb + lane;
             float z = -INFINITY;
             long long at = -1;
@@ -223,7 +273,7 @@ __device__ __forceinline__ void lone_row(const Args &a, int seq, int p, int head
             const float f = exp2f(m - ms), e = j < j1 ? exp2f(z - ms) : 0.f;
             m = mn;
             l = l * f + mb::warp_sum(e);
-            #pragma unroll
+#pragma unroll
             for (int i = 0; i < 4; i++) acc[i] *= f;
 #pragma unroll 1
             for (int t = 0; t < min(32, j1 - jb); t++) {
@@ -234,13 +284,16 @@ __device__ __forceinline__ void lone_row(const Args &a, int seq, int p, int head
                     for (int i = 0; i < 4; i++)
                         if (i < per) acc[i] = fmaf(w, to_f32(reinterpret_cast<const T *>(a.v)[vt + lane + 32 * i]), acc[i]);
             }
+            bool nan = true;
+#pragma unroll
+            for (int i = 0; i < 4; i++) nan &= i >= per || isnan(acc[i]);
+            known = isnan(l) || (l > 0.f && __all_sync(0xffffffffu, nan));
         }
     }
     T *o = reinterpret_cast<T *>(a.out) + row * a.o_row + head * a.o_head;
 #pragma unroll
     for (int i = 0; i < 4; i++)
         if (i < per) o[lane + 32 * i] = from_f32<T>(l == 0.f ? 0.f : acc[i] / l);
-    if (a.lse && lane == 0) a.lse[(long long)row * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // A row of a CTA that gave up: not a number, so that nobody takes it for a result.  By a warp.
@@ -392,21 +445,21 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 2) k_join(const __grid_consta
             __syncthreads();
         }
         if (there && (serial || warp == 0)) {
-            const float inv = x.l == 0.f ? 0.f : 1.f / x.l;
+            const float inv = 1.f / x.l;
             const int t = r / mt.ng, head = mt.head0 + r - t * mt.ng;
             const long long row = mt.row0 + t;
-            x.acc = make_float4(x.acc.x * inv, x.acc.y * inv, x.acc.z * inv, x.acc.w * inv);
-            bool alone = false;
+            x.acc = x.l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                               : make_float4(x.acc.x * inv, x.acc.y * inv, x.acc.z * inv, x.acc.w * inv);
+            if (lane * 4 < a.d) store4(reinterpret_cast<T *>(a.out) + row * a.o_row + head * a.o_head + lane * 4, x.acc);
+            if (a.lse && lane == 0)
+                a.lse[row * a.heads + head] = x.l == 0.f ? -INFINITY : ((x.m == -INFINITY ? 0.f : x.m) + log2f(x.l)) * kLn2;
             if (PREFILL) {
                 const bool bad = !(isfinite(x.acc.x) && isfinite(x.acc.y) && isfinite(x.acc.z) && isfinite(x.acc.w));
-                alone = __any_sync(0xffffffffu, bad && lane * 4 < a.d);
-            }
-            if (alone) {
-                lone_row<T>(a, mt.seq, mt.pos0 + t, head, (int)row);
-            } else {
-                if (lane * 4 < a.d) store4(reinterpret_cast<T *>(a.out) + row * a.o_row + head * a.o_head + lane * 4, x.acc);
-                if (a.lse && lane == 0)
-                    a.lse[row * a.heads + head] = x.l == 0.f ? -INFINITY : ((x.m == -INFINITY ? 0.f : x.m) + log2f(x.l)) * kLn2;
+                if (__any_sync(0xffffffffu, bad && lane * 4 < a.d) &&
+                    unseen_values<T, sizeof(T) == 4 ? 64 : 128>(a, mt.seq, mt.pos0 + t, head, mt.pos0, mt.pos0 + note.y / mt.ng - 1)) {
+                    __syncwarp();
+                    lone_row<T>(a, mt.seq, mt.pos0 + t, head, (int)row);
+                }
             }
         }
     }

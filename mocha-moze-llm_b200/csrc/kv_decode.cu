@@ -659,10 +659,10 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
                         y.w = fmaf(z.w, f, y.w);
                     }
                     if (whole) {
-                        const float inv = L == 0.f ? 0.f : 1.f / L;
+                        const float inv = 1.f / L;
                         if (cc * 4 < a.d)
                             store4(reinterpret_cast<T *>(a.out) + seq * a.o_row + (h0 + h) * a.o_head + cc * 4,
-                                   make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+                                   L == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
                         if (a.lse && cc == 0) a.lse[(long long)seq * a.heads + h0 + h] = L == 0.f ? -INFINITY : (ms + log2f(L)) * kLn2;
                     } else {
                         *reinterpret_cast<float4 *>(part + (size_t)h * DP + cc * 4) = y;

@@ -344,20 +344,17 @@ __global__ void __launch_bounds__(kThreads, Smem32<DP>::kCtas) k_prefill(const _
 #pragma unroll
             for (int o = 1; o < 16; o <<= 1) l[y] += __shfl_xor_sync(0xffffffffu, l[y], o);
             bool bad = false;
-            const float inv = !whole ? 1.f : l[y] == 0.f ? 0.f : 1.f / l[y];
+            const float inv = !whole ? 1.f : 1.f / l[y];
 #pragma unroll
             for (int c = 0; c < DP / 16; c++) {
-                acc[y][c] *= inv;
+                acc[y][c] = whole && l[y] == 0.f ? 0.f : acc[y][c] * inv;
                 bad |= !isfinite(acc[y][c]);
             }
 #pragma unroll
             for (int o = 1; o < 16; o <<= 1) bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
             if (r >= nrow) continue;
             const long long row = u.p.q0 + tok0 + t;
-            if (whole && bad) {
-                if (tx == 0) s_bad[r] = 1;
-                continue;
-            }
+            if (whole && bad && tx == 0) s_bad[r] = 1;
 #pragma unroll
             for (int c = 0; c < DP / 64; c++) {
                 const int at = tx * 4 + 64 * c;
@@ -377,8 +374,9 @@ __global__ void __launch_bounds__(kThreads, Smem32<DP>::kCtas) k_prefill(const _
             __syncthreads();
             for (int r = warp; r < nrow; r += kThreads / 32)
                 if (s_bad[r]) {
-                    const int t = div(a.group_div, r);
-                    lone_row<float>(a, u.seq, pa + t, u.kvh * a.group + r - t * a.group, u.p.q0 + tok0 + t);
+                    const int t = div(a.group_div, r), head = u.kvh * a.group + r - t * a.group;
+                    if (unseen_values<float, kKeys>(a, u.seq, pa + t, head, pa, pb))
+                        lone_row<float>(a, u.seq, pa + t, head, u.p.q0 + tok0 + t);
                 }
         }
         if (left <= 0 && tid == 0) {
@@ -1020,8 +1018,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const int at = (xt + t) * a.group + g;
                 const long long row = d.row0 + xt + t;
                 float *part = a.part + ((size_t)blockIdx.x * 2 + (d.first == 0 ? 1 : 0)) * ((size_t)256 * (DP + 2));
-                // a row whose maximum is still -infinity has seen nothing
-                const float inv = !whole ? 1.f : m == -INFINITY ? 0.f : 1.f / l;
+                const bool none = whole && l == 0.f;  // has seen nothing, or scores of -infinity alone
+                const float inv = !whole ? 1.f : 1.f / l;
                 bool bad = false;
                 // 128 bytes of a row at a time; the four lanes of a quad write their rows' lines together
                 unsigned char *base = whole ? reinterpret_cast<unsigned char *>(a.out) + (row * a.o_row + head * a.o_head) * 2
@@ -1045,7 +1043,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
 #pragma unroll
                         for (int e = 0; e < 32; e++) {
-                            o[e] *= inv;
+                            o[e] = none ? 0.f : o[e] * inv;
                             bad |= !isfinite(o[e]);
                         }
                         if (whole) {
@@ -1074,7 +1072,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         part[(size_t)256 * DP + 2 * at] = m == -INFINITY ? m : fmaf(m, k2, -kLift<T>);
                         part[(size_t)256 * DP + 2 * at + 1] = l;
                     } else {
-                        if (a.lse) a.lse[row * a.heads + head] = m == -INFINITY ? m : (fmaf(m, k2, -kLift<T>) + log2f(l)) * kLn2;
+                        if (a.lse) a.lse[row * a.heads + head] = none ? -INFINITY : ((m == -INFINITY ? 0.f : fmaf(m, k2, -kLift<T>)) + log2f(l)) * kLn2;
                         if (bad) bar.bad = 1;
                     }
                 }
@@ -1123,7 +1121,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const T *o = reinterpret_cast<const T *>(a.out) + row * a.o_row + head * a.o_head;
                 bool bad = false;
                 for (int e = lane; e < a.d; e += 32) bad |= !isfinite(to_f32(o[e]));
-                if (__any_sync(0xffffffffu, bad)) lone_row<T>(a, u.seq, u.p.pos(tok0 + t), head, row);
+                const int p0 = u.p.pos(tok0);
+                if (__any_sync(0xffffffffu, bad) && unseen_values<T, kTcKeys>(a, u.seq, p0 + t, head, p0, p0 + ntok - 1))
+                    lone_row<T>(a, u.seq, p0 + t, head, row);
             }
         left -= u.t.n - i + kUnitEnd;
         if (left > 0) u.next(a, tokens);

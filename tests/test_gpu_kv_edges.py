@@ -197,3 +197,105 @@ def test_many_weights_far_below_the_largest(kv, prefill, dtype, top):
     tol = ref.unit(dtype) * want.abs() + weights + n * 2.0 ** -24 * (top + most) + (60 * 2.0 ** -24 + 2.0 ** -22) * most
     close(out, want, tol)
     assert float((lse[:, 0].double() - torch.log1p(w)).abs().max()) <= 2048 * 2.0 ** -24 + 60 * 2.0 ** -24 * most + 2.0 ** -22
+
+
+# ---- infinite and NaN values -----------------------------------------------------------
+
+def plain(q, k, v, positions, window=0, prefix=0):
+    """The formula by torch in 64 bits, so that infinities and NaN go where they go."""
+    rows, heads, dim = q.shape
+    group = heads // k.shape[0]
+    k, v = k.repeat_interleave(group, 0), v.repeat_interleave(group, 0)
+    z = torch.einsum("rhd,hjd->hrj", q.double(), k) * dim ** -0.5
+    p, j = torch.tensor(list(positions), device=DEV)[:, None], torch.arange(k.shape[1], device=DEV)
+    seen = (j <= p) & ((p - j < window) if window else True) | (j < prefix)
+    out = torch.empty(rows, heads, dim, dtype=torch.float64, device=DEV)
+    for r in range(rows):
+        at = seen[r].nonzero().flatten()
+        if len(at) == 0 or not (z[:, r, at] > -math.inf).any():
+            out[r] = 0.0
+            continue
+        out[r] = torch.einsum("hj,hjd->hd", torch.softmax(z[:, r, at], -1), v[:, at])
+    return out
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("where", ["seen by all", "seen by some", "one dim", "both", "values everywhere", "keys too"])
+@pytest.mark.parametrize("window,prefix", [(0, 0), (70, 3)])
+def test_values_that_are_not_finite(kv, dtype, where, window, prefix):
+    """Infinities and NaN in keys and values that rows see, do not see, or both, beside finite ones:
+    what a row sees shows in its dims as the formula has it, what it does not see nowhere."""
+    n, rows = 300, 170
+    k, v, table = pool([n], 2, 64, 16, dtype, fill=0.0)
+
+    def put(t, pos, value, dims=slice(None)):
+        t[int(table[0, pos // 16]), :, pos % 16, dims] = value
+
+    if where == "seen by all":
+        put(v, 1, math.nan)
+    if where in ("seen by some", "both"):
+        put(v, 200, math.inf), put(v, 231, math.nan, slice(3, 9))
+    if where in ("one dim", "both"):
+        put(v, 2, math.inf, slice(17, 18)), put(v, 140, -math.inf, slice(17, 20))
+    if where in ("values everywhere", "keys too"):
+        v.fill_(math.nan)
+    if where == "keys too":
+        put(k, 150, math.nan), put(k, 151, math.inf)
+    q, lse, lse0 = queries(rows, 6, 64, dtype), torch.zeros(rows, 6, device=DEV), torch.zeros(rows, 6, device=DEV)
+    more = dict(window=window, prefix=ints([prefix]) if prefix else None)
+    cache = kv.KvPages(k, v)
+    out = cache.prefill(q, ints([0, rows]), table, ints([n]), lse=lse, **more)
+    kv.KvPages(k, torch.zeros_like(v)).prefill(q, ints([0, rows]), table, ints([n]), lse=lse0, **more)
+    kk, vv = ref.gather(k, table, 0, n), ref.gather(v, table, 0, n)
+    want = plain(q, kk, vv, range(n - rows, n), window, prefix)
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out.isinf(), want.isinf()) and torch.equal(out[out.isinf()].double(), want[want.isinf()])
+    _, _, tol, _ = ref.attend(q, torch.nan_to_num(kk, 0, 0, 0), torch.nan_to_num(vv, 0, 0, 0), range(n - rows, n), 0.125, window,
+                              prefix, dtype=dtype)
+    ok = want.isfinite()
+    close(out[ok], want[ok], tol[ok])
+    assert torch.equal(lse.nan_to_num(7.0), lse0.nan_to_num(7.0))  # the values are no part of it
+    one = cache.decode(q[-1:].contiguous(), table, ints([n]), **more)[0]
+    assert torch.equal(one.isnan(), want[-1].isnan())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scores_of_minus_infinity_over_nan_values(kv, dtype):
+    """Rows whose visible scores are all -infinity are zeros, whatever the values hold."""
+    for n, rows in ((40, 1), (40, 30), (3000, 2)):
+        k, v, table = pool([n], 1, 64, 8, dtype)
+        k.fill_(1.0), v.fill_(math.nan)
+        q = torch.full((rows, 2, 64), -math.inf, device=DEV, dtype=dtype)
+        cache = kv.KvPages(k, v)
+        assert (cache.prefill(q, ints([0, rows]), table, ints([n])) == 0).all()
+        assert (cache.decode(q[:1].contiguous(), table, ints([n])) == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_nan_does_not_cost_a_prompt_its_speed(kv, dtype):
+    """A NaN that every row sees makes every row NaN: each is looked at once more, but not done
+    once more (some 100 times the call's time)."""
+    n = 4096 if dtype == BF16 else 1024
+    k, v, table = pool([n], 2, 64, 64, dtype)
+    q = queries(n, 8, 64, dtype)
+    start, lens = ints([0, n]), ints([n])
+    cache = kv.KvPages(k, v)
+    out = torch.empty_like(q)
+
+    def time():
+        best = math.inf
+        for _ in range(3):
+            a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+            a.record()
+            cache.prefill(q, start, table, lens, out=out)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    usual = time()
+    assert out.isfinite().all()
+    v[int(table[0, 0]), :, 0] = math.nan
+    slow = time()
+    print("ms", usual, slow)
+    assert out.isnan().all() and slow < 30 * usual
