@@ -695,6 +695,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         return;
     }
     if (tid == 0) bar.share = share.out;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // queries are copied to where the search kept its sums
     if (warp == 8) tmem_alloc(&bar.tmem, 512);
     tc_fence_before();
     __syncthreads();
