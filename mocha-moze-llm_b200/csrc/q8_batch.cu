@@ -1092,11 +1092,12 @@ __global__ void __launch_bounds__(NT) k_attn_limbs(const T *__restrict__ att, Li
                                threadIdx.x & 15);
 }
 
-// A decode step's lengths: row i holds position pos[i].
-__global__ void k_lengths(const int *__restrict__ pos, int n, int *kv_len)
+// A decode step's lengths: row i holds position pos[i]; none where its slot has no pages, that
+// is for a row that waits for a sequence.
+__global__ void k_lengths(const int *__restrict__ pos, const int *__restrict__ table, int width, int n, int *kv_len)
 {
     pdl_enter();
-    for (int i = threadIdx.x; i < n; i += blockDim.x) kv_len[i] = pos[i] + 1;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) kv_len[i] = table[(size_t)i * width] < 0 ? 0 : pos[i] + 1;
 }
 
 // ---- engine -------------------------------------------------------------------------
@@ -1471,7 +1472,7 @@ int enqueue_forward(mocha_q8b *h, Rows rows, int n, bool decode_set, const int *
 {
     const PlanSet &ps = decode_set ? h->dec : h->pre;
     cudaStream_t s = h->stream;
-    if (h->paged && graph_step && pdl(k_lengths, 1, 256, 0, s, rows.pos, n, h->paged->dec_len)) return 1;
+    if (h->paged && graph_step && pdl(k_lengths, 1, 256, 0, s, rows.pos, h->paged->dec_table, h->paged->width, n, h->paged->dec_len)) return 1;
     if (pdl(k_embed_norm, n, NT, 0, s, h->m.embed, rows, h->m.layer[0].attn_norm, h->x, h->lx)) return 1;
     mb::tc::Split sp;
     for (int l = 0; l < LAYERS; l++) {
