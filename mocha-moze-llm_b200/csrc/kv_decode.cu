@@ -11,8 +11,11 @@
 //
 // 16-bit types: scores are K q^T and outputs V^T p^T by m16n8k16 products, so the heads of
 // the group are the narrow side of 8 and no lane computes on padding when a group has 8.
-// The weights are rounded to the cache's type for the second product; their sum is taken
-// before that, in fp32.  fp32: the same tiles on the FMA units, a lane holding half a key's
+// For the second product a weight is the sum of two values of the cache's type, so that it
+// keeps twice its bits: the outputs are off by their own rounding alone, where weights of one
+// value each added up to 40 % to the error, and the time grows by 1 % (groups of 8, 64
+// sequences or 128), 2 % (windows) and 6 to 8 % (32 and 64 heads a kv head), as memory is what
+// bounds the kernel.  fp32: the same tiles on the FMA units, a lane holding half a key's
 // products with 8 heads.  Either way the value that weights are taken from is renewed only
 // when a score passes it by 2^8, which a vote finds: no shuffles and no rescaling on most
 // tiles.
@@ -152,6 +155,21 @@ MB_DEV uint32_t pack2(float x, float y)
         return *reinterpret_cast<const uint32_t *>(&h);
     }
 }
+
+// A weight as the sum of two values: what its leading bits hold, and the rest.  The rest is
+// at least 2^-16 of the weight, so that neither is zero or negative and an infinite value that
+// a row sees stays infinite (fp16: under weights down to 2^-15 of the largest).
+template <typename T>
+MB_DEV uint32_t cut2(float x, float y)
+{
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value)
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    else
+        asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    return r;
+}
+MB_DEV float rest(float x, float cut) { return fmaxf(x - cut, x * 0x1p-16f); }
 
 // The share of this CTA: its first tile as (sequence, tile within the sequence) in *s_seq
 // and *s_rem, and [start, end) in tiles of the whole call.
@@ -494,7 +512,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
                     }
                 }
             }
-            uint32_t pt[MT][NG][2];
+            uint32_t ph[MT][NG][2], pl[MT][NG][2];  // weights to the type, and what that leaves of them
 #pragma unroll
             for (int n = 0; n < NG; n++) {
 #pragma unroll
@@ -504,8 +522,14 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
                     for (int e = 0; e < 4; e++) z[e] = ex2(z[e]);
                     l[2 * n] += z[0] + z[2];
                     l[2 * n + 1] += z[1] + z[3];
-                    pt[t][n][0] = transpose8(pack2<T>(z[0], z[1]));
-                    pt[t][n][1] = transpose8(pack2<T>(z[2], z[3]));
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float x = z[2 * e], y = z[2 * e + 1];
+                        const uint32_t hi = cut2<T>(x, y);
+                        const T *h = reinterpret_cast<const T *>(&hi);
+                        ph[t][n][e] = transpose8(hi);
+                        pl[t][n][e] = transpose8(pack2<T>(rest(x, to_f32(h[0])), rest(y, to_f32(h[1]))));
+                    }
                 }
             }
 #pragma unroll
@@ -515,7 +539,10 @@ __global__ void __launch_bounds__(Ring<T, DP, NG>::kThreads, Ring<T, DP, NG>::kC
                     uint32_t vf[4];
                     ldsm4_t(slot + t * 16 * ROW + v_at[d], vf);
 #pragma unroll
-                    for (int n = 0; n < NG; n++) mma<T>(acc[n * (DP / 16) + d], vf, pt[t][n][0], pt[t][n][1]);
+                    for (int n = 0; n < NG; n++) {
+                        mma<T>(acc[n * (DP / 16) + d], vf, ph[t][n][0], ph[t][n][1]);
+                        mma<T>(acc[n * (DP / 16) + d], vf, pl[t][n][0], pl[t][n][1]);
+                    }
                 }
         } else {
             // scores: lane = key x part of the dims (32 of them), all heads.  The parts start

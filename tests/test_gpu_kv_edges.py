@@ -299,3 +299,28 @@ def test_a_nan_does_not_cost_a_prompt_its_speed(kv, dtype):
     slow = time()
     print("ms", usual, slow)
     assert out.isnan().all() and slow < 30 * usual
+
+
+# ---- roundings -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lens,heads,kvh,dim,more", [
+    ([1, 2, 40, 300, 3000], 6, 2, 64, {}), ([777], 32, 4, 128, {}), ([130, 2000], 24, 2, 96, {}),
+    ([130, 900], 40, 1, 128, {"window": 400, "prefix": 5}), ([1500, 9], 4, 4, 32, {"cap": 20.0}),
+])
+def test_decode_rounds_its_outputs_alone(kv, dtype, lens, heads, kvh, dim, more):
+    """Single-token attention in 16 bits: u |o| for the output, 2^-16 A for weights in two parts (the
+    second at most 2u of the weight and rounded by u of itself: 2^-15 in bf16), n 2^-32 of the largest
+    value for fp16's last bit, and what the same formula in fp32 may be off by; no u A for weights
+    of 16 bits."""
+    k, v, table = pool(lens, kvh, dim, 16, dtype)
+    q = queries(len(lens), heads, dim, dtype)
+    window, prefix, cap = (more.get(x, 0) for x in ("window", "prefix", "cap"))
+    out = kv.KvPages(k, v).decode(q, table, ints(lens), window=window, cap=cap, prefix=ints([prefix] * len(lens)))
+    for s, n in enumerate(lens):
+        kk, vv = ref.gather(k, table, s, n), ref.gather(v, table, s, n)
+        args = ([n - 1], dim ** -0.5, window, min(prefix, n), cap)
+        want, _, tol, _ = ref.attend(q[s:s + 1], kk, vv, *args)
+        size = ref.attend(q[s:s + 1], kk, vv.abs(), *args)[0]
+        u = ref.unit(dtype)
+        close(out[s:s + 1], want, u * want.abs() + max(2.0 ** -16, 2 * u * u) * size + n * 2.0 ** -32 * vv.abs().max() + tol)
