@@ -93,3 +93,38 @@ def rotate(x, cos, sin, interleaved):
     tol[..., ia] = 2 * w * ((a * cos).abs() + (b * sin).abs())
     tol[..., ib] = 2 * w * ((a * sin).abs() + (b * cos).abs())
     return out, tol
+
+
+def capped(q, k, v, positions, scale, cap, slopes=None, dtype=torch.float32):
+    """`attend` under a cap, with the bound that holds where scores pass it: a product that is off
+    by w (dim + 4) scale sum |q k| moves the capped score by no more than tanh moves over that
+    interval (nothing, where it is flat).  tanh by 1 - 2 / (1 + 2^y) is off by at most 10 w of
+    itself where it starts, at 0.54 (2^y: 4 w, and 2 w for y; the quotient: 4 w; of 0.46, and w
+    for the difference), less after it and below, so that z is off by 10 w |z|, and by 8 w |z| as
+    there.  (out, tol)"""
+    rows, heads, dim = q.shape
+    kv = k.shape[0]
+    out = torch.zeros(rows, heads, dim, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    u, w = unit(dtype), 2.0 ** -24
+    wide = dtype == torch.float32
+    for r in range(rows):
+        p = int(positions[r])
+        for h in range(heads):
+            kk, vv = k[h // (heads // kv), :p + 1], v[h // (heads // kv), :p + 1]
+            x = q[r, h].double()
+            z = (kk @ x) * scale
+            off = w * (dim + 4) * (kk.abs() @ x.abs()) * abs(scale)
+            low, z, high = (cap * torch.tanh(y / cap) for y in (z - off, z, z + off))
+            d = torch.maximum((high - z).abs(), (z - low).abs()) + 18 * w * z.abs()
+            if slopes is not None:
+                bias = float(slopes[h]) * (p - torch.arange(p + 1, device=q.device))
+                z, d = z - bias, d + 8 * w * bias.abs()
+            m = z.max()
+            pr = torch.exp(z - m)
+            pr = pr / pr.sum()
+            out[r, h] = pr @ vv
+            rel = 2 * (8 * w * m.abs() + (2.0 ** -21 if wide else u / 8)) + 2 * (p + 1) * w + (0 if wide else u)
+            # a weight is off by its score's error and by the sum's, the weights' mean of them all
+            tol[r, h] = u * out[r, h].abs() + 2 * (pr * d.expm1()) @ vv.abs() + ((pr * d.expm1()).sum() * 2 + rel) * (pr @ vv.abs())
+    return out, tol + torch.finfo(dtype).tiny

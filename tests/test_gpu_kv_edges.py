@@ -324,3 +324,22 @@ def test_decode_rounds_its_outputs_alone(kv, dtype, lens, heads, kvh, dim, more)
         size = ref.attend(q[s:s + 1], kk, vv.abs(), *args)[0]
         u = ref.unit(dtype)
         close(out[s:s + 1], want, u * want.abs() + max(2.0 ** -16, 2 * u * u) * size + n * 2.0 ** -32 * vv.abs().max() + tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("prefill", [False, True])
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("scale,cap", [(4e4, 100.0), (-1e9, 1e-9), (3.0, 4.0), (-0.7, 0.25), (0.125, 50.0), (2.0 ** 40, 2.0 ** -40)])
+def test_caps_that_scores_reach(kv, prefill, dtype, slopes, scale, cap):
+    """Scores around a cap and far past it, under a bound that stays far below the outputs."""
+    n, rows = 200, 60
+    k, v, table = pool([n], 2, 64, 16, dtype)
+    q = queries(rows, 4, 64, dtype)
+    sl = torch.tensor([0.5, 0.125, 0.03, 0.004], device=DEV) if slopes else None
+    want, tol = ref.capped(q, ref.gather(k, table, 0, n), ref.gather(v, table, 0, n), range(n - rows, n), scale, cap, sl, dtype)
+    assert float(tol.median()) < 0.1 * float(want.abs().median())
+    cache = kv.KvPages(k, v)
+    if prefill:
+        close(cache.prefill(q, ints([0, rows]), table, ints([n]), scale=scale, cap=cap, slopes=sl), want, tol)
+    else:
+        close(cache.decode(q[-1:].contiguous(), table, ints([n]), scale=scale, cap=cap, slopes=sl), want[-1:], tol[-1:])
