@@ -343,3 +343,22 @@ def test_caps_that_scores_reach(kv, prefill, dtype, slopes, scale, cap):
         close(cache.prefill(q, ints([0, rows]), table, ints([n]), scale=scale, cap=cap, slopes=sl), want, tol)
     else:
         close(cache.decode(q[-1:].contiguous(), table, ints([n]), scale=scale, cap=cap, slopes=sl), want[-1:], tol[-1:])
+
+
+# ---- strides ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_broadcast_queries_and_pages(kv, dtype):
+    """One query row for all rows, and one page under several ids (strides of 0): as if copied."""
+    k, v, table = pool([70, 33], 2, 64, 16, dtype)
+    cache = kv.KvPages(k, v)
+    lens, start = ints([70, 33]), ints([0, 7, 12])
+    q = queries(1, 4, 64, dtype)
+    for n, call in ((12, lambda x: cache.prefill(x, start, table, lens)), (2, lambda x: cache.decode(x, table, lens))):
+        assert torch.equal(call(q.expand(n, 4, 64)), call(q.expand(n, 4, 64).contiguous()))
+    q = queries(12, 4, 64, dtype)
+    k1, v1 = (queries(2, 16, 64, dtype, seed=s).view(1, 2, 16, 64).expand(5, 2, 16, 64) for s in (3, 4))
+    wide, copied = kv.KvPages(k1, v1), kv.KvPages(k1.contiguous(), v1.contiguous())
+    ids = ints([4, 0, 2, 1, 3, 1, 0, 2, 2, 4]).view(2, 5)
+    for call in (lambda c: c.prefill(q, start, ids, lens), lambda c: c.decode(q[:2], ids, lens)):
+        assert torch.equal(call(wide), call(copied))
