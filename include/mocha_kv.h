@@ -16,7 +16,10 @@
  * stderr and nothing enqueued.
  *
  * Types: the pages, the rotated queries and the attention's queries and outputs have one
- * type, fp32, fp16 or bf16; products are summed in fp32 and softmax statistics are fp32.
+ * type, fp32, fp16 or bf16; products are summed in fp32 and softmax statistics are fp32.  On
+ * 16-bit pages mocha_kv_prefill rounds the softmax weights to the pages' type for the product
+ * with the values, which adds up to 40 % to the error that the outputs' own rounding makes;
+ * mocha_kv_decode keeps twice the bits of them, and on fp32 pages they are fp32.
  * Alignment: the base pointers of pages, queries, keys, values and outputs are multiples
  * of 16 bytes, their strides multiples of 16 bytes, and a head's values are contiguous.
  * head_dim is a multiple of 32 up to 128, page_size a multiple of 8 up to 65536. */

@@ -7,8 +7,9 @@
 // rotated values apart: the two ends of eight pairs (i, i + dims/2), or twice four
 // interleaved pairs, or values that are only copied, likewise far apart.  Threads go along a
 // token's heads, so each of a warp's accesses covers whole lines in every layout, and the
-// token's slot, page and angles are L1 hits after the first thread's.  16381 rows of 32 + 16
-// heads of 128, bf16: 57.6 us, 5.6 TB/s; one row of 14 + 4 heads of 64: 2 us, a launch.
+// token's slot, page and angles are L1 hits after the first thread's.  12810 rows of 32 + 16
+// heads of 128, bf16: 57 us, 5.6 TB/s; from fp32 74.8 us, 6.4 TB/s; one row of 14 + 4 heads of
+// 64: 2 us, a launch.
 #include "kv_common.cuh"
 
 namespace {
@@ -38,10 +39,12 @@ struct Append {
 };
 
 // Heads of a thread, which share its angles and addresses, once half as many threads still
-// fill half the card: 32 + 16 heads of 128 take 4.9 us (1024 rows), 18.0 (4096) and 71.5
+// fill half the card: 32 + 16 heads of 128, bf16, take 4.9 us (1024 rows), 18.0 (4096) and 71.5
 // (16384) with two heads, 5.5, 21.3 and 83.4 with one; at 512 rows 3.75 and 3.65.  Four and
 // eight heads measured 3 to 20 % worse up to 4096 rows.  64 registers at most, for 32 warps of
-// an SM: with 68 and 24 warps the 16384 rows took 79.9 us, with 48 and spills 76 to 79.
+// an SM: with 68 and 24 warps the 16384 rows took 79.9 us, with 48 and spills 76 to 79.  From
+// fp32, where 64 registers spill 40 to 60 bytes a thread, 12810 rows take 74.8 us with them and
+// 78.0 with 84, 4287 rows 27.5 and 28.4, and from fp32 to fp32 99.7 and 100.7.
 constexpr int kHeads = 2;
 
 MB_DEV void load4(const float *p, float *x)

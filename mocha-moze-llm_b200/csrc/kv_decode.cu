@@ -13,17 +13,17 @@
 // the group are the narrow side of 8 and no lane computes on padding when a group has 8.
 // For the second product a weight is the sum of two values of the cache's type, so that it
 // keeps twice its bits: the outputs are off by their own rounding alone, where weights of one
-// value each added up to 40 % to the error, and the time grows by 1 % (groups of 8, 64
-// sequences or 128), 2 % (windows) and 6 to 8 % (32 and 64 heads a kv head), as memory is what
-// bounds the kernel.  fp32: the same tiles on the FMA units, a lane holding half a key's
+// value each added up to 40 % to the error.  Memory bounds the kernel up to groups of 8, whose
+// time grows by 1 % (64 and 128 sequences) or 2 % (windows); 16 heads a kv head take 5 % longer,
+// 32 and 64 take 7 to 11 %.  fp32: the same tiles on the FMA units, a lane holding half a key's
 // products with 8 heads.  Either way the value that weights are taken from is renewed only
 // when a score passes it by 2^8, which a vote finds: no shuffles and no rescaling on most
 // tiles.
 //
-// Measured: 128 sequences up to 8192 long, 8 kv heads of 128, 2.41 GB: 378 us, 6.4 TB/s, with
-// the card at its power limit; two of 40,001 and 131,071, 0.18 GB: 36 us, 4.9 TB/s; 64 up to
-// 2047 of 64 dims, 0.14 GB: 31 us, 4.6 TB/s, of which some 9 us are the start (lengths, pages,
-// first keys) and the join.  One sequence of 777 in fp32: 10.7 us, all of it latency.  A
+// Measured: 128 sequences up to 8192 long, 8 kv heads of 128, 2.41 GB: 380 us, 6.3 TB/s, with
+// the card at its power limit; two of 40,001 and 131,071, 0.18 GB: 37 us, 4.8 TB/s; 64 up to
+// 2047 of 64 dims, 0.14 GB: 32 us, 4.5 TB/s, of which some 9 us are the start (lengths, pages,
+// first keys) and the join.  One sequence of 777 in fp32: 10.4 us, all of it latency.  A
 // prefetch of the next tile into L2 cost 10 % at the power limit; halves of a tile as copy
 // groups of their own changed nothing.
 #include "kv_common.cuh"
@@ -66,7 +66,8 @@ struct Work {
 
 // What a unit's end counts for in a share, in tiles: the warps' meeting and the next unit's
 // start.  Without it the CTAs with the shortest sequences were last (64 sequences up to
-// 2047: the slowest 41 us, half of them 32).
+// 2047: 39.3 us for 32.1; windows 45.2 for 37.5).  2 is the same for 16-bit pages and worse for
+// 64 fp32 sequences (33.5 for 31.1).
 constexpr int kUnitEnd = 1;
 
 // A walk along a CTA's tiles; j is the tile's first key.
@@ -142,18 +143,6 @@ MB_DEV void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-template <typename T>
-MB_DEV uint32_t pack2(float x, float y)
-{
-    if constexpr (std::is_same<T, __half>::value) {
-        const __half2 h = __floats2half2_rn(x, y);
-        return *reinterpret_cast<const uint32_t *>(&h);
-    } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-        return *reinterpret_cast<const uint32_t *>(&h);
-    }
 }
 
 // A weight as the sum of two values: what its leading bits hold, and the rest.  The rest is
@@ -720,7 +709,7 @@ struct Plan {
         const char *who = "mocha_kv_decode";
         w.unit_heads = R::kH;
         w.hgroups = (w.a.group + R::kH - 1) / R::kH;
-        w.min_tiles = 1;
+        w.min_tiles = 1;  // 2: one fp32 sequence of 777 in 12.1 us for 10.4, the others as they are
         w.one_page = page_size % R::kKeys == 0;
         lay_out(w.a, space, kCtas);
         static std::atomic<unsigned long long> allowed{0};
@@ -732,7 +721,11 @@ struct Plan {
 };
 
 // Calls f with the plan for a type, group and dim: units of all heads of a group up to 32
-// (16-bit), of 4 or 8 (fp32, where a wider group's heads read the keys again, from L2).
+// (16-bit), of 4 or 8 (fp32, where a wider group's heads read the keys again, from L2).  Units of
+// 16 heads in place of 32, each reading the keys: with 128 dims, where 32 heads spill (414 bytes a
+// thread), faster while a sequence's keys stay in L2 (64 sequences up to 8192, one kv head: 76 us
+// for 89), slower past it (128 sequences up to 16000, two kv heads: 516 for 472); with 64 dims
+// slower throughout (49 for 41).
 template <typename F>
 auto with_plan(int type, int group, int d, F f)
 {

@@ -13,7 +13,6 @@ using namespace kv;
 // A sequence's rows and keys.
 struct Piece {
     int q0, nq, len, pre, blocks;
-    template <int TOKENS_DIV = 0>
     MB_DEV void load(const Args &a, int s, int tokens)
     {
         q0 = min(max(__ldg(a.q_start + s), 0), a.rows);
@@ -46,7 +45,10 @@ struct ShareSmem {
     Share out;
 };
 
-// What a unit's end counts for in a share, in tiles: outputs, and the next unit's start.
+// What a unit's end counts for in a share, in tiles: outputs, and the next unit's start.  With 0,
+// 1 and 3 the prompt of 8192 takes 528, 493 and 467 us for 464, that of 1024 25.1, 24.6 and 24.9
+// for 23.9; the pieces after long texts 42.8, 41.6 and 39.9 for 40.8; every option 222, 219 and
+// 218 for 219.
 constexpr int kUnitEnd = 2;
 
 // Tiles of sequence s per kv head with its units' ends, by a warp.
@@ -166,8 +168,10 @@ MB_DEV bool find_share(const Args &a, int tokens, int min_tiles, ShareSmem &sm)
 
 // ---- fp32 ------------------------------------------------------------------------------
 // Products on the FMA units: 64 rows x 64 keys, 256 threads of 4 x 4 scores and 4 rows x
-// dim / 16 outputs.  Bound by them on long prompts; five pieces of up to 70 tokens after up to 600: 31 us, mostly the
-// latency of a few tiles in line.
+// dim / 16 outputs.  Bound by their operands' way out of shared memory, which four barriers a
+// tile leave idle at times: the FMA units run at 28 %.  Five pieces of up to 70 tokens after up
+// to 600: 31 us, of which 2 find the shares, 2.5 are the first keys' way, two tiles in line take 6
+// to 8 each, the unit's end 1.6 and the join 5.
 constexpr int kRows = 64, kKeys = 64, kThreads = 256;
 
 template <int DP>
@@ -398,12 +402,13 @@ __global__ void __launch_bounds__(kThreads, Smem32<DP>::kCtas) k_prefill(const _
 // weights.  Scores S = Q K^T and outputs O += P V are accumulated in TMEM; P goes back to
 // TMEM over the scores it came from and is the second product's first operand there.  While
 // the warps of one tile work on its weights the tensor core has the other tile's products,
-// so the products (4 * 128 * 128 * dim operations per tile and key tile) bound the kernel
-// as long as the weights of a tile take no longer than the other's products.
+// so the products (4 * 128 * 128 * dim operations per tile and key tile) are the floor.  The
+// two chains, products and weights, still wait for one another: at 8192 tokens the tensor pipe is
+// busy for 58 % of the time and the exponential unit for 60 %.
 //
 // The maximum that a row's weights are taken from is renewed only when it is exceeded by
-// 2^8, so outputs are rescaled a few times per row and not per tile; weights then are at
-// most 2^8, sums and outputs stay exact to their type.
+// 2^8, so outputs are rescaled a few times per row and not per tile.  Weights are rounded to 16
+// bits once (kLift in kv_common.cuh has the reason), after their sums, which are fp32.
 //
 // Measured: a prompt of 8192, 32 heads of 128, causal: 465 us, 1.18 PFLOP/s; after a second of
 // it the card is at its power limit and it takes 540.  A prompt of 1024, 14 heads of 64: 24 us, of
@@ -411,7 +416,10 @@ __global__ void __launch_bounds__(kThreads, Smem32<DP>::kCtas) k_prefill(const _
 // Two pieces of 16 tokens after 65,521, 134 MB: 41 us; the tiles come at memory's rate, the start
 // and the ends of units are the rest.  Two threads per row (750 us) and a thread per tile for
 // the products (650 us) were worse; exponentials on the FMA units, an eighth to a half of them,
-// measured from 1 % better to 5 % worse.
+// measured from 1 % better to 5 % worse.  With a cap or a bias the warps of weights, which then
+// spill 36 to 48 bytes a thread, are what a step waits for: six prompts with every option, 212 us,
+// have the tensor pipe busy for 21 % of the time, the exponential unit for 24 %, and 38 % of the
+// issue slots used.
 constexpr int kTcThreads = 384;  // warps 0-3 and 4-7: weights of the two tiles; 8: products; 9: copies; 10, 11: none
 constexpr int kTcUnits = 4;      // units that the copies may be ahead
 constexpr int kTcKeys = 128;
@@ -560,19 +568,6 @@ MB_DEV void tmem_st16f(uint32_t addr, const float (&x)[16])
                  KV_F8(x, 8), "r"(addr));
 }
 MB_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// Two roundings in one instruction.
-template <typename T>
-MB_DEV uint32_t pack16(float x, float y)
-{
-    if constexpr (std::is_same<T, __half>::value) {
-        const __half2 h = __floats2half2_rn(x, y);
-        return *reinterpret_cast<const uint32_t *>(&h);
-    } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-        return *reinterpret_cast<const uint32_t *>(&h);
-    }
-}
 
 // Pairs of fp32 operations in one instruction, each rounded to nearest.
 MB_DEV void fma2(float &d0, float &d1, float a0, float a1, float b0, float b1, float c0, float c1)
@@ -982,7 +977,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                 e0 = ex2(e0);
                                 e1 = ex2(e1);
                                 add2(sum[(2 * e) & 3], sum[(2 * e + 1) & 3], e0, e1);
-                                w[e] = pack16<T>(e0, e1);
+                                w[e] = pack2<T>(e0, e1);
                             }
                             tmem_st16(ts + 16 * b, w);
                             if (b & 1) {
@@ -1049,7 +1044,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                         if (whole) {
 #pragma unroll
-                            for (int e = 0; e < 16; e++) w[16 * c + e] = pack16<T>(o[2 * e], o[2 * e + 1]);
+                            for (int e = 0; e < 16; e++) w[16 * c + e] = pack2<T>(o[2 * e], o[2 * e + 1]);
                         } else {
 #pragma unroll
                             for (int e = 0; e < 32; e++) w[e] = __float_as_uint(o[e]);
