@@ -159,10 +159,13 @@ MB_DEV float tanh_of(float x)
 // kernel rounds them once: with the rest of each in a second product the outputs' error falls
 // by a sixth (1024 tokens) to a quarter (8192), to that of their own rounding, and the call takes
 // 6 % (1024 tokens), 13 % (short pieces after long texts), 20 % (every option) and 36 % (8192)
-// longer.  The single-token kernel has the second product, for it costs 1 to 2 %.  They are taken 2^kLift above the value that they are relative to, and pass it by 2^8 before it is
-// renewed: fp16's then reach from 2^15, half its range, down to its last bit, 2^-24, so that
-// one is lost only 2^-32 below the largest, and 131071 of those are 2^-15 of the sum (fp32 sums lose as much).  bf16
-// has fp32's range.
+// longer.  The single-token kernel has the second product: there it costs 1 to 2 % (wide groups:
+// kv_decode.cu).
+//
+// They are taken 2^kLift above the value that they are relative to, and pass it by 2^8 before it
+// is renewed: fp16's then reach from 2^15, half its range, down to its last bit, 2^-24, so that
+// one is lost only 2^-32 below the largest, and 131071 of those are 2^-15 of the sum (fp32 sums
+// lose as much).  bf16 has fp32's range.
 template <typename T>
 constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
 
