@@ -150,10 +150,8 @@ MB_DEV float tanh_small(float x)
     const float t = x * x;
     return x * fmaf(fmaf(fmaf(fmaf(kTanh4, t, kTanh3), t, kTanh2), t, kTanh1), t, kTanh0);
 }
-MB_DEV float tanh_of(float x)
-{
-    return fabsf(x) <= kTanhPart ? tanh_small(x) : 1.f - __fdividef(2.f, 1.f + ex2(x * (2.f * kLog2e)));
-}
+MB_DEV float tanh_large(float x) { return 1.f - __fdividef(2.f, 1.f + ex2(x * (2.f * kLog2e))); }
+MB_DEV float tanh_of(float x) { return fabsf(x) <= kTanhPart ? tanh_small(x) : tanh_large(x); }
 
 // Weights are rounded to the cache's 16-bit type for the product with the values.  The prompt
 // kernel rounds them once: with the rest of each in a second product the outputs' error falls

@@ -587,20 +587,28 @@ MB_DEV void add2(float &d0, float &d1, float a0, float a1)
 // cap tanh(k s) + bias of a row of scores, bias = base - slope c for column c, where cap is in
 // log2.  Where all of a warp's |k s| are within tanh_of's polynomial, as those of ordinary
 // scores under an ordinary cap are, on the FMA units alone: its coefficients take up k and cap.
-// Only rows that exist (`there`) have a say: what the others hold is left over from other calls.
+// The other way rounds such scores alike, bit by bit, for what the vote sees are also scores of
+// keys that no row sees and that anything may lie in.  Rows that do not exist have no say.
 MB_DEV void cap_scores(float (&s)[128], float cap, float k, float slope, float base, bool there)
 {
     float big = 0.f;
 #pragma unroll
     for (int c = 0; c < 128; c += 2) big = fmaxf(big, fmaxf(fabsf(s[c]), fabsf(s[c + 1])));
-    const float kk = k * k, c0 = kTanh0 * cap * k, c1 = kTanh1 * cap * k * kk, c2 = kTanh2 * cap * k * kk * kk,
-                c3 = kTanh3 * cap * k * kk * kk * kk, c4 = kTanh4 * cap * k * kk * kk * kk * kk;
+    const float kk = k * k;
+    float c0 = kTanh0 * cap * k, c1 = kTanh1 * cap * k * kk, c2 = kTanh2 * cap * k * kk * kk,
+          c3 = kTanh3 * cap * k * kk * kk * kk, c4 = kTanh4 * cap * k * kk * kk * kk * kk;
     // the coefficients and the scores' squares have to be normal numbers: c4 within these bounds
-    // holds |k| between 2^-18 and 2^17
+    // holds |k| between 2^-18 and 2^17.  Elsewhere the polynomial takes k s.
     const bool normal = fabsf(c4) >= 0x1p-120f && fabsf(c4) <= 0x1p100f;
     if (!normal || __any_sync(0xffffffffu, there && big * fabsf(k) > kTanhPart)) {
+        const float f = normal ? 1.f : k;
+        if (!normal) c0 = kTanh0 * cap, c1 = kTanh1 * cap, c2 = kTanh2 * cap, c3 = kTanh3 * cap, c4 = kTanh4 * cap;
 #pragma unroll
-        for (int c = 0; c < 128; c++) s[c] = fmaf(cap, tanh_of(s[c] * k), fmaf(-slope, (float)c, base));
+        for (int c = 0; c < 128; c++) {
+            const float x = s[c] * k, a = s[c] * f, t = fmaf(a, a, 0.f), bias = fmaf(-slope, (float)c, base);
+            const float y = fmaf(fmaf(fmaf(fmaf(c4, t, c3), t, c2), t, c1), t, c0);
+            s[c] = fabsf(x) <= kTanhPart ? fmaf(a, y, bias) : fmaf(cap, tanh_large(x), bias);
+        }
     } else {
 #pragma unroll
         for (int c = 0; c < 128; c += 2) {

@@ -139,6 +139,34 @@ def test_caps_do_not_see_other_calls(kv, dtype, rows):
     assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("prefill", [False, True])
+def test_caps_do_not_see_other_keys(kv, dtype, prefill):
+    """The same bits whatever lies behind the sequence's end in its last page, in pages that its
+    window has left, in other caches, and at positions that a row does not see."""
+    n, rows = 420, 30 if prefill else 1
+    k, v, table = pool([n], 2, 64, 16, dtype, fill=0.0)
+    cache = kv.KvPages(k, v)
+    other = kv.KvPages(torch.zeros_like(k), torch.zeros_like(v))
+    far = torch.arange(len(k), device=DEV, dtype=torch.int32).view(1, -1)
+    q = queries(rows, 4, 64, dtype, scale=0.5)
+    seen_by_last = k[int(table[0, 26]), :, 1:4].clone()
+    got = []
+    for size in (0.0, 1e3, -30.0):
+        k[int(table[0, 26]), :, 4:] = size  # 420 = 26 * 16 + 4
+        k[int(table[0, 2])] = size  # positions 32 .. 47, before the window
+        k[int(table[0, 26]), :, 1:4] = size if prefill else seen_by_last  # the last three, which the rows before do not see
+        other.k.fill_(size)
+        big = queries(300, 4, 64, dtype, 7)
+        other.prefill(big, ints([0, 300]), far, ints([16 * len(k)]))
+        other.decode(big[:1], far, ints([16 * len(k)]))
+        if prefill:
+            got.append(cache.prefill(q, ints([0, rows]), table, ints([n]), cap=30.0, window=300)[:rows - 3])
+        else:
+            got.append(cache.decode(q, table, ints([n]), cap=30.0, window=300))
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
 @pytest.mark.parametrize("prefill", [False, True])
 @pytest.mark.parametrize("scale,cap,size", [(2.0 ** -30, 50.0, 12000.0), (2.0 ** -39, 1.0, 2.0 ** 17),
                                             (2.0 ** 10, 2.0 ** -10, 2.0 ** -42), (0.125, 50.0, 9e-5)])
