@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, Smem32<DP>::kCtas) k_prefill(const _
 // the warps of one tile work on its weights the tensor core has the other tile's products,
 // so the products (4 * 128 * 128 * dim operations per tile and key tile) are the floor.  The
 // two chains, products and weights, still wait for one another: at 8192 tokens the tensor pipe is
-// busy for 58 % of the time and the exponential unit for 60 %.
+// busy for 57 % of the time and the exponential unit for 60 %.
 //
 // The maximum that a row's weights are taken from is renewed only when it is exceeded by
 // 2^8, so outputs are rescaled a few times per row and not per tile.  Weights are rounded to 16
